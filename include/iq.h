@@ -47,13 +47,13 @@ enum { IQ_INT8 = 0, IQ_INT4 = 1 };
 /* Error codes (negative). */
 enum {
     IQ_OK = 0,
-    IQ_EKIND = -1,      /* kind is neither IQ_INT8 nor IQ_INT4 */
+    IQ_EKIND = -1,      /* kind is neither IQ_INT8 nor IQ_INT4 (a cache's type: IQ_KV_*) */
     IQ_ESHAPE = -2,     /* inconsistent or unsupported sizes */
     IQ_ENULL = -3,      /* a required pointer is NULL */
     IQ_ETOOLARGE = -4,  /* problem exceeds the workspace limits */
     IQ_ENOMEM = -5,     /* workspace allocation failed */
     IQ_EDEVICE = -6,    /* no usable gfx950 device, or not the chain's device */
-    IQ_EALIAS = -7      /* a chain stage's output overlaps its input */
+    IQ_EALIAS = -7      /* an output overlaps an input */
 };
 
 /* gpu::QuantView (kernels/ops/ops.cuh:166-172), byte-compatible on LP64:
@@ -215,6 +215,99 @@ int iq_chain_create(const iq_stage* stages, int n, iq_chain** out);
 /* Enqueues one run of the whole program on `stream`. */
 int iq_chain_run(const iq_chain* chain, void* stream);
 void iq_chain_destroy(iq_chain* chain);
+
+/* ------------------------------------------------ the cache of a decode step
+ * A paged key/value cache, the attention of one new token a sequence over
+ * it, and eviction from it.  No counterparts in the reference's quantised
+ * path; iq_attn_decode's output is what a chain stage with IQ_IN_PLAIN reads
+ * (the o projection), its q and the appended k, v are what the q|k|v stage
+ * writes.
+ *
+ * A sequence's token t (0 <= t < its length) lies in slot t % page_size of
+ * page table[b][t / page_size]; its key vector for key/value head h starts at
+ *   k + page * page_stride + slot * slot_stride + h * head_stride
+ * (in elements; v alike), head_dim contiguous values.  Any order of pages,
+ * slots and heads in memory can be described, and pages may be shared between
+ * sequences as long as nothing writes them.  k, v 16-byte aligned, the strides
+ * multiples of 8, head_dim a multiple of 8 in 8..256. */
+enum { IQ_KV_BF16 = 0, IQ_KV_F16 = 1 };
+
+typedef struct iq_kv {
+    int32_t type;                              /* IQ_KV_BF16, IQ_KV_F16 */
+    int32_t kv_heads, head_dim, page_size;     /* page_size: any number of slots >= 1 */
+    int64_t pages;                             /* in the pool, < 2^31 */
+    int64_t page_stride, slot_stride, head_stride;
+    void* k;
+    void* v;
+} iq_kv;
+
+/* Adds T tokens to the cache: k, v fp32 [T][kv_heads][head_dim] are written
+ * to slot slots[t] = page * page_size + slot (rounded to the cache's type,
+ * to nearest even), q fp32 [T][q_heads][head_dim] goes to q_out; q and k with
+ * rotary embedding on their first rot_dim values (pairs i, i + rot_dim/2
+ * turned by positions[t] * freqs[i], freqs double [rot_dim/2]; angles in
+ * 64 bits, so far positions keep their precision).  rot_dim: a multiple of 8
+ * up to head_dim, or 0 (no rotation; positions and freqs unused).  A slot
+ * outside the pool (e.g. -1, a padded row) writes nothing to the cache; two
+ * tokens of one call must not have the same slot.  q_out may be q itself;
+ * another overlap of q_out with q, k or v is refused (IQ_EALIAS).  q and q_out
+ * may be NULL with q_heads = 0. */
+int iq_kv_append(const float* q, const float* k, const float* v, const int64_t* positions, const int64_t* slots,
+                 int64_t T, int q_heads, const double* freqs, int rot_dim, const iq_kv* kv, float* q_out,
+                 void* stream);
+
+/* Attention of one token a sequence over its cached tokens:
+ *   p[b,h,t] = softmax over t < lens[b] of scale * q[b,h] . key[b,t,h / g]
+ *   out[b,h] = sum_t p[b,h,t] value[b,t,h / g],   g = q_heads / kv_heads
+ * q, out fp32 [B][q_heads][head_dim] (out must not overlap q), table int32
+ * [B][table_ld] of which the first max_pages entries of a row may be used
+ * (entries past a sequence's last page are not read), lens int32 [B], 1 <= B
+ * <= 1024.  Scores, softmax and sums are fp32; the 16-bit keys and values
+ * are exact.  Keys and values past a sequence's length have no influence,
+ * whatever they hold.
+ * weights (may be NULL): fp32 [B][kv_heads][weights_ld], weights_ld >=
+ * max_pages * page_size; weights[b][j][t] += sum over the heads h of key/value
+ * head j of p[b,h,t], for t < lens[b]; the rest is left as it was.
+ * A sequence of length 0 gives zeros.  A length below 0 or above max_pages *
+ * page_size gives NaN (its weights are left as they were), as does a page id
+ * outside [0, pages) or a non-finite q, key or value that is attended to. */
+int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t max_pages,
+                   const int32_t* lens, int B, int q_heads, float scale, float* out, float* weights,
+                   int64_t weights_ld, void* stream);
+
+/* Cuts every sequence of more than `budget` tokens to `budget`, for each
+ * key/value head by itself: of its n = lens[b] tokens stay the newest `recent`
+ * (0 <= recent <= budget) and, of the n - recent older ones, the budget -
+ * recent of the largest weights[b][h][t] (equal ones: the lower t; NaN counts
+ * as less than any number).  With cut = budget - recent: a kept older token
+ * below cut stays where it is, the kept ones above it fill the free places
+ * below cut, both in ascending order, and the newest follow in their order.
+ * weights move along, and weights[b][h][t] = 0 for budget <= t < n, so that a
+ * slot appended later starts at 0.  new_lens[b] = min(lens[b], budget) for
+ * every head alike (the pages past it are free); it must not overlap lens.
+ * Pages must not be shared between the sequences of a call.  A sequence whose
+ * length is below 0 or above max_pages * page_size, or any of whose first
+ * ceil(n / page_size) page ids lies outside [0, pages), is left as it is and
+ * its new length is its old one.  1 <= B <= 1024, budget >= 1; table, lens and
+ * weights as above. */
+int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t max_pages, const int32_t* lens,
+                int B, int64_t budget, int64_t recent, float* weights, int64_t weights_ld, int32_t* new_lens,
+                void* stream);
+
+/* Log probabilities over rows of logits, fp32 [T][V] with `ld` >= V floats
+ * from row to row (V < 2^31):
+ *   logprob[t]  log softmax(row t)[tokens[t]]; NaN for a token outside [0, V)
+ *   entropy[t]  -sum p log p
+ *   top_ids[t][i], top_logprobs[t][i], i < top <= 64: the `top` largest, by
+ *               value descending, equal ones by id ascending
+ * tokens and logprob are NULL together, entropy may be NULL, top_ids and
+ * top_logprobs are NULL with top = 0; at least one output is asked for and
+ * top <= V.  A logit of -inf has probability 0 and log probability -inf.  A
+ * row that holds NaN or +inf, or nothing but -inf, has no distribution: its
+ * log probabilities and entropy are NaN (its ids are still ranked, NaN as the
+ * largest). */
+int iq_logprobs(const float* logits, int64_t ld, int64_t T, int64_t V, const int64_t* tokens, int top,
+                float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs, void* stream);
 
 /* Reserve the workspace of (device, null stream) (done lazily by the first
  * call that needs it).  Call before capturing a graph.  Returns 0 or an

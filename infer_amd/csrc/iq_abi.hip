@@ -378,13 +378,13 @@ int iq_quantize(const uint16_t* w_bf16, int64_t rows, int64_t cols, int kind, ui
 const char* iq_error_string(int code) {
     switch (code) {
         case IQ_OK: return "ok";
-        case IQ_EKIND: return "iq: quant kind must be IQ_INT8 (0) or IQ_INT4 (1)";
+        case IQ_EKIND: return "iq: quant kind must be IQ_INT8 (0) or IQ_INT4 (1), a cache's type IQ_KV_BF16 (0) or IQ_KV_F16 (1)";
         case IQ_ESHAPE: return "iq: inconsistent or unsupported shape";
         case IQ_ENULL: return "iq: required pointer is NULL";
         case IQ_ETOOLARGE: return "iq: problem exceeds workspace limits";
         case IQ_ENOMEM: return "iq: workspace allocation failed";
         case IQ_EDEVICE: return "iq: no usable device (or not the device the chain was made on)";
-        case IQ_EALIAS: return "iq: a chain stage's output overlaps its input";
+        case IQ_EALIAS: return "iq: an output overlaps an input";
         default: break;
     }
     if (code > 0) return hipGetErrorString(static_cast<hipError_t>(code));

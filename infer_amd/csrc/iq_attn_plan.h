@@ -1,0 +1,48 @@
+// iq_attn_plan.h -- how a batch's cached tokens are split over workgroups:
+// arithmetic shared by the kernels of iq_attn.hip, their host side and the
+// CPU tests (plain C++: g++ compiles it on its own).
+//
+// Lengths are known on the device only.  Every sequence is cut into chunks
+// of the same number of 32-token tiles, C, chosen from the batch's total so
+// that all chunks of all key/value head tiles are about `target` work items:
+// a long sequence beside short ones gets as many workgroups as its share of
+// the tokens.  A sequence always has one chunk at least (an empty one's
+// writes its zeros).
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+
+#if defined(__HIPCC__)
+#define IQ_HD __host__ __device__ __forceinline__
+#else
+#define IQ_HD inline
+#endif
+
+namespace iq {
+
+constexpr int kAttnTile = 32;   // tokens a wave multiplies at a time
+constexpr int kAttnWaves = 4;   // waves of a workgroup: a chunk's tiles are dealt to them in turn
+
+IQ_HD uint32_t attn_tiles(int32_t len) { return (uint32_t(len) + kAttnTile - 1) / kAttnTile; }
+
+// Tiles of a chunk: `total` tiles of all sequences, `heads` head tiles each
+// (total * heads < 2^31), in whole rounds of the workgroup's waves.
+IQ_HD uint32_t attn_chunk_tiles(uint32_t total, uint32_t heads, uint32_t target) {
+    const uint32_t c = (total * heads + target - 1) / target;
+    return c <= kAttnWaves ? uint32_t(kAttnWaves) : (c + kAttnWaves - 1) / kAttnWaves * kAttnWaves;
+}
+
+IQ_HD uint32_t attn_chunks(uint32_t tiles, uint32_t c) { return tiles <= c ? 1 : (tiles + c - 1) / c; }
+
+// Bounds over all lengths up to `cap` tokens: work items, and those of
+// sequences with more than one chunk (which have a partial result each).
+// chunks <= tiles / C + 1 each, C >= total * heads / target; a sequence of
+// more than one chunk has tiles > C, so at most 2 tiles / C of them.
+inline int64_t attn_max_items(int64_t B, int64_t heads, int64_t cap, int64_t target) {
+    const int64_t most = (int64_t(attn_tiles(int32_t(cap))) + kAttnWaves - 1) / kAttnWaves;
+    return std::min(B * heads * most, target + B * heads);
+}
+inline int64_t attn_max_partials(int64_t target) { return 2 * target; }
+
+}  // namespace iq

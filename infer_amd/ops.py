@@ -19,6 +19,7 @@ fallback: without libiq.so every entry point raises.
 import ctypes
 import enum
 import os
+import typing
 
 import torch
 
@@ -61,10 +62,28 @@ class IqStage(ctypes.Structure):
     ]
 
 
+class IqKv(ctypes.Structure):
+    """iq_kv (include/iq.h): a paged key/value cache."""
+    _fields_ = [
+        ("type", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("pages", ctypes.c_int64),
+        ("page_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+    ]
+
+
 # Every function include/iq.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _VP = ctypes.POINTER(IqView)
+_KV = ctypes.POINTER(IqKv)
+_INT = ctypes.c_int
 SIGNATURES = {
     "iq_gemv": ([_P, _VP, _P, ctypes.c_int, _I64, _I64, _P, _P], ctypes.c_int),
     "iq_gemv_noalloc": ([_P, _VP, _P, ctypes.c_int, _I64, _I64, _P, _P], ctypes.c_int),
@@ -80,6 +99,10 @@ SIGNATURES = {
     "iq_chain_create": ([ctypes.POINTER(IqStage), ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
     "iq_chain_run": ([_P, _P], ctypes.c_int),
     "iq_chain_destroy": ([_P], None),
+    "iq_kv_append": ([_P, _P, _P, _P, _P, _I64, _INT, _P, _INT, _KV, _P, _P], _INT),
+    "iq_attn_decode": ([_P, _KV, _P, _I64, _I64, _P, _INT, _INT, ctypes.c_float, _P, _P, _I64, _P], _INT),
+    "iq_kv_evict": ([_KV, _P, _I64, _I64, _P, _INT, _I64, _I64, _P, _I64, _P, _P], _INT),
+    "iq_logprobs": ([_P, _I64, _I64, _I64, _P, _INT, _P, _P, _P, _P, _P], _INT),
     "iq_init": ([ctypes.c_int], ctypes.c_int),
     "iq_init_stream": ([ctypes.c_int, _P], ctypes.c_int),
     "iq_error_string": ([ctypes.c_int], ctypes.c_char_p),
@@ -291,6 +314,226 @@ def linear(x, W, bias=None, stream=None):
     y = torch.empty(T, W.rows, dtype=torch.float32, device=x.device)
     launch_linear_q(x.contiguous(), W, bias, T, K, W.rows, y, stream)
     return y
+
+
+# ------------------------------------------------ the cache of a decode step
+KV_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+class KvCache:
+    """A paged key/value cache (include/iq.h, iq_kv) over two tensors k, v of
+    [pages, page_size, kv_heads, head_dim], torch.bfloat16 or torch.float16,
+    which it keeps alive.  Any memory order of pages, slots and heads (a
+    permuted view, a slice of a larger tensor) whose rows of head_dim values
+    are contiguous, with the same strides for k and v."""
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("KvCache: k and v must be [pages, page_size, kv_heads, head_dim] of one shape and type")
+        if k.dtype not in KV_TYPES:
+            raise TypeError("KvCache: k and v must be torch.bfloat16 or torch.float16")
+        # (the stride over a single page, slot or head means nothing)
+        strides = [[0 if n == 1 else s for n, s in zip(t.shape, t.stride())] for t in (k, v)]
+        if strides[0] != strides[1] or strides[0][3] not in (0, 1):
+            raise ValueError("KvCache: k and v need the same strides and contiguous rows of head_dim values")
+        self.k, self.v = k, v
+        self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
+        self.device = k.get_device()
+        if v.get_device() != self.device:
+            raise ValueError("KvCache: k and v must be on one device")
+        self._c = IqKv(KV_TYPES[k.dtype], self.kv_heads, self.head_dim, self.page_size, self.pages,
+                       *strides[0][:3], k.data_ptr(), v.data_ptr())
+
+    @property
+    def c(self):
+        return ctypes.byref(self._c)
+
+
+def alloc_kv(pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
+    """An empty cache (zeros) in the order [pages, page_size, kv_heads, head_dim]."""
+    shape = (pages, page_size, kv_heads, head_dim)
+    return KvCache(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+
+def rope_freqs(rot_dim, theta, device="cuda"):
+    """theta^(-2i / rot_dim), i < rot_dim / 2, in double: kv_append's freqs."""
+    return torch.tensor([theta ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)], dtype=torch.float64,
+                        device=device)
+
+
+def _need(what, name, t, dtype, numel=None):
+    """A contiguous tensor of this type (and number of elements)."""
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+    if not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        raise ValueError(f"{what}: {name} must be contiguous" + ("" if numel is None else f" with {numel} elements"))
+
+
+def _on_device(what, device, *tensors):
+    """Every tensor on `device`, which is the current CUDA device."""
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{what}: tensors on different devices")
+    if device < 0 or device != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors must be on the current CUDA device")
+
+
+def _new(stream, make, *args, **kw):
+    """An output made here: from the memory of the stream that writes it."""
+    if stream is None:
+        return make(*args, **kw)
+    with torch.cuda.stream(stream):
+        return make(*args, **kw)
+
+
+def kv_append(q, k, v, positions, slots, freqs, cache, q_out=None, stream=None):
+    """Rotary embedding of q [T, heads, head_dim] (into q_out, may be q) and
+    k [T, kv_heads, head_dim] at positions [T], k and v [T, kv_heads, head_dim]
+    into cache slots [T] = page * page_size + slot (outside the pool: not
+    stored; all others different).  fp32 inputs, int64 positions and slots,
+    freqs: rope_freqs, or None (no rotation; positions may be None).  q may be
+    None (cache only).  Returns q_out.  include/iq.h, iq_kv_append."""
+    what = "kv_append"
+    T, d = slots.numel(), cache.head_dim
+    _need(what, "slots", slots, torch.int64)
+    _need(what, "k", k, torch.float32, T * cache.kv_heads * d)
+    _need(what, "v", v, torch.float32, T * cache.kv_heads * d)
+    rot = 0
+    if freqs is not None:
+        _need(what, "freqs", freqs, torch.float64)
+        _need(what, "positions", positions, torch.int64, T)
+        rot = 2 * freqs.numel()
+    heads = 0
+    if q is not None:
+        heads = q.numel() // max(1, T * d)
+        _need(what, "q", q, torch.float32, T * heads * d)
+        if q_out is not None:
+            _need(what, "q_out", q_out, torch.float32, T * heads * d)
+    _on_device(what, cache.device, q, k, v, positions if rot else None, slots, freqs, q_out)
+    if q is not None and q_out is None:
+        q_out = _new(stream, torch.empty_like, q)
+    rc = lib().iq_kv_append(_ptr(q), _ptr(k), _ptr(v), _ptr(positions) if rot else None, _ptr(slots), T, heads,
+                            _ptr(freqs) if rot else None, rot, cache.c, _ptr(q_out) if heads else None,
+                            _stream(stream))
+    _check(rc, "iq_kv_append")
+    return q_out
+
+
+def _check_table(what, table, lens):
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{what}: table must be int32 [sequences, pages] with contiguous rows")
+    B, pages = table.shape
+    _need(what, "lens", lens, torch.int32, B)
+    ld = table.stride(0) if B > 1 else pages
+    return B, pages, ld
+
+
+def _check_sums(what, weights, B, kv_heads):
+    """fp32 [sequences, kv_heads, tokens], sequences and heads packed."""
+    if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, kv_heads):
+        raise ValueError(f"{what}: weights must be float32 [sequences, kv_heads, tokens]")
+    if not weights.is_contiguous():
+        raise ValueError(f"{what}: weights must be contiguous")
+    return weights.shape[2]
+
+
+def attn_decode(q, cache, table, lens, out=None, weights=None, scale=None, stream=None):
+    """Attention of one token a sequence, q [B, heads, head_dim] fp32, over
+    the first lens[b] (int32 [B]) tokens in the pages table[b] (int32 [B,
+    pages]) of the cache; heads / kv_heads query heads share a key/value head.
+    scale: head_dim^-0.5 by default.  weights: fp32 [B, kv_heads, tokens],
+    tokens >= pages * page_size; every cached token's attention weight, summed
+    over the heads that share it, is added to it.  Returns out, shaped as q.
+    include/iq.h, iq_attn_decode."""
+    what = "attn_decode"
+    B, pages, ld = _check_table(what, table, lens)
+    d = cache.head_dim
+    heads = q.numel() // max(1, B * d)
+    _need(what, "q", q, torch.float32, B * heads * d)
+    wld = 0 if weights is None else _check_sums(what, weights, B, cache.kv_heads)
+    if out is not None:
+        _need(what, "out", out, torch.float32, B * heads * d)
+    _on_device(what, cache.device, q, table, lens, out, weights)
+    if out is None:
+        out = _new(stream, torch.empty_like, q)
+    rc = lib().iq_attn_decode(_ptr(q), cache.c, _ptr(table), ld, pages, _ptr(lens), B, heads,
+                              d ** -0.5 if scale is None else scale, _ptr(out), _ptr(weights), wld, _stream(stream))
+    _check(rc, "iq_attn_decode")
+    return out
+
+
+def kv_evict(cache, table, lens, weights, budget, recent, new_lens=None, stream=None):
+    """Cuts every sequence of more than `budget` tokens to `budget`, for each
+    key/value head by itself: the newest `recent` stay and, of the others,
+    those of the largest weights (fp32 [B, kv_heads, tokens], which move along;
+    entries past the budget become 0).  Returns new_lens (int32 [B]), min(lens,
+    budget): the pages past it are free.  include/iq.h, iq_kv_evict."""
+    what = "kv_evict"
+    B, pages, ld = _check_table(what, table, lens)
+    wld = _check_sums(what, weights, B, cache.kv_heads)
+    if new_lens is not None:
+        _need(what, "new_lens", new_lens, torch.int32, B)
+    _on_device(what, cache.device, table, lens, weights, new_lens)
+    if new_lens is None:
+        new_lens = _new(stream, torch.empty_like, lens)
+    rc = lib().iq_kv_evict(cache.c, _ptr(table), ld, pages, _ptr(lens), B, int(budget), int(recent), _ptr(weights),
+                           wld, _ptr(new_lens), _stream(stream))
+    _check(rc, "iq_kv_evict")
+    return new_lens
+
+
+class LogProbs(typing.NamedTuple):
+    """logprobs' outputs; top_ids and top_logprobs are None with top = 0,
+    logprob is None without tokens (or is not written, in a given buffer)."""
+    logprob: typing.Optional[torch.Tensor]
+    entropy: typing.Optional[torch.Tensor]
+    top_ids: typing.Optional[torch.Tensor]
+    top_logprobs: typing.Optional[torch.Tensor]
+
+
+def alloc_logprobs(T, top=0, device="cuda"):
+    """Buffers for logprobs' outputs of T rows."""
+    f = dict(dtype=torch.float32, device=device)
+    return LogProbs(torch.empty(T, **f), torch.empty(T, **f),
+                    torch.empty(T, top, dtype=torch.int64, device=device) if top else None,
+                    torch.empty(T, top, **f) if top else None)
+
+
+def logprobs(logits, tokens=None, top=0, out=None, stream=None):
+    """For rows of logits [T, V] fp32 (any row stride): the log probability of
+    tokens[t] (int64 [T]; NaN outside [0, V)), the entropy, and the `top` (<=
+    64) most likely ids with their log probabilities (equal logits: the lower
+    id first).  out: alloc_logprobs(T, top).  Returns LogProbs.
+    include/iq.h, iq_logprobs."""
+    what = "logprobs"
+    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"{what}: logits must be float32 [T, V] with contiguous rows")
+    T, V = logits.shape
+    ld = logits.stride(0) if T > 1 else V
+    if tokens is not None:
+        _need(what, "tokens", tokens, torch.int64, T)
+    if out is None:
+        out = _new(stream, alloc_logprobs, T, top, device=logits.device)
+    lp, ent, ids, tlp = out
+    if tokens is None:
+        lp = None
+    elif lp is None:
+        raise ValueError(f"{what}: out has no logprob")
+    for name, t, dt, n in (("logprob", lp, torch.float32, T), ("entropy", ent, torch.float32, T)):
+        if t is not None:
+            _need(what, name, t, dt, n)
+    if top:
+        if ids is None or tlp is None:
+            raise ValueError(f"{what}: out has no top_ids and top_logprobs")
+        _need(what, "top_ids", ids, torch.int64, T * top)
+        _need(what, "top_logprobs", tlp, torch.float32, T * top)
+    else:
+        ids = tlp = None
+    _on_device(what, logits.get_device(), logits, tokens, lp, ent, ids, tlp)
+    rc = lib().iq_logprobs(_ptr(logits), ld, T, V, _ptr(tokens), int(top), _ptr(lp), _ptr(ent), _ptr(ids), _ptr(tlp),
+                           _stream(stream))
+    _check(rc, "iq_logprobs")
+    return LogProbs(lp, ent, ids, tlp)
 
 
 def init(device=0, stream=None):
