@@ -1,99 +1,480 @@
 // iq_attn.hip -- attention of one new token a sequence over a paged cache.
+//
+// With g query heads on a key/value head, every cached element is used by g
+// products of each kind, and an element is 2 bytes: on the vector units that
+// is 7 multiply-adds for Qwen2.5-7B where HBM delivers one element per two
+// cycles and lane, too many beside the unpacking; on the matrix cores the up
+// to 16 heads of a group are the 16 columns of one product and cost nothing.
+// What bounds the operator is the read of the cache.
+//
+//   scores  S^T[token][head] = K[token][d] . q^T[d][head]
+//   sums    O^T[d][head]    += V^T[d][token] . P^T[token][head]
+//
+// both as 16 x 16 x 32 MFMAs on the 16-bit cache as it is.  q and p are fp32:
+// for a bf16 cache each is cut exactly into three bf16 terms (8 + 8 + 8 bits)
+// and multiplied three times, for fp16 into two fp16 terms (22 bits, scaled
+// so that nothing becomes subnormal): the products stay at fp32 precision and
+// still take a small part of the matrix cores' time.
+//
+// A wave takes 32 tokens at a time: their K and V rows come in whole rows (16
+// bytes a lane, 16 lanes a row at d = 128) into registers while the previous
+// tile is multiplied, then through the wave's own part of LDS (no barrier)
+// into operand order: K rows by 16-byte reads, V transposed by
+// ds_read_b64_tr_b16.  The scores' result order (head = lane % 16, tokens
+// 4 (lane / 16) + 0..3 of either half) is used as the second product's
+// operand order, so P never leaves its lane.  Maximum and sum run along
+// (one pass); a new maximum rescales the 16 x d sums.
+//
+// The batch's tokens are split into chunks of equal size over all sequences
+// (iq_attn_plan.h); a workgroup of 4 waves has one chunk of one head tile,
+// joins its waves in LDS, and writes the result if the sequence has no other
+// chunk, else the chunk's maximum, sum and unnormalised rows, which
+// attn_join_kernel adds up.  Nothing is kept between calls and no order of
+// additions depends on timing.
+#include <algorithm>
+
+#include "iq_attn_plan.h"
 #include "iq_kv.h"
 
 namespace iq {
 namespace {
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
 
 struct AttnArgs {
     KvView c;
     KvTable t;
     const float* q;
     float* out;
-    float* w;
-    int64_t wld;
-    float* ml;  // [B][hq][2]: running maximum and sum of every head
-    int hq, group;
-    float scale;
+    int hq, group, B;
+    int ht;           // 16-head tiles of a group
+    uint32_t nh;      // hk * ht
+    uint32_t target;
+    float mul;        // scale * log2(e): scores in powers of two
+    float* ml;        // [partials][16][2]: a chunk's maximum and sum of every head
+    float* part;      // [partials][16][d]
+    uint2* plan;      // [B]: chunks, first partial
+    float* sc;        // scores [B][hk][cap][group] for the weights, or null
+    float* fin;       // [B][hq][2]: maximum and sum of every head, for the weights
 };
 
-// The score of token tok (or -inf past the end).
-template <int TYPE>
-__device__ float score(const AttnArgs& a, const float* q, int b, int j, int tok, bool* bad) {
-    const int p = tok / a.c.ps, id = a.t.table[b * a.t.ld + p];
-    if (id < 0 || id >= a.c.pages) {
-        *bad = true;
-        return 0.0f;
-    }
-    const uint16_t* k = reinterpret_cast<const uint16_t*>(a.c.k) + id * a.c.pstr + int64_t(tok - p * a.c.ps) * a.c.sstr +
-                        j * a.c.hstr;
-    float s = 0.0f;
-    for (int i = 0; i < a.c.d; i++) s = fmaf(kv_to_f32<TYPE>(k[i]), q[i], s);
-    return s * a.scale;
+// --------------------------------------------------- sums over a wave (DPP)
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+    return v + uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROW_MASK, 0xf, true));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = dpp_add<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8: within 16 lanes
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+    return uint32_t(__builtin_amdgcn_readlane(int(v), lane));
 }
 
-// One wave per (head, sequence), 64 tokens at a time.
+struct Item {
+    int b, n;            // sequence and its length (as given)
+    uint32_t j, c, chunks, first;  // chunk, tiles of a chunk, chunks of the sequence, its first partial
+};
+
+// The (sequence, chunk) number w of the batch's plan; false past the last.
+// Every wave finds it from the lengths by itself (64 sequences a step).
+__device__ bool find_item(const AttnArgs& a, uint32_t w, Item* it) {
+    const int lane = threadIdx.x & 63;
+    auto length = [&](int b) { return b < a.B ? a.t.lens[b] : 0; };
+    auto tiles_of = [&](int n) { return n < 0 || n > a.t.cap ? 0u : attn_tiles(n); };
+    int n = length(lane);
+    uint32_t total = lane_of(wave_scan(tiles_of(n)), 63);
+    for (int b0 = 64; b0 < a.B; b0 += 64) total += lane_of(wave_scan(tiles_of(length(b0 + lane))), 63);
+    const uint32_t c = attn_chunk_tiles(total, a.nh, a.target);
+    uint32_t before = 0, first = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        if (b0) n = length(b0 + lane);
+        const uint32_t k = b0 + lane < a.B ? attn_chunks(tiles_of(n), c) : 0;
+        const uint32_t upto = wave_scan(k), many = k > 1 ? k : 0, pupto = wave_scan(many);
+        const uint64_t past = __ballot(w < before + upto);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            it->b = b0 + l;
+            it->n = __builtin_amdgcn_readlane(n, l);
+            it->chunks = lane_of(k, l);
+            it->j = w - before - (lane_of(upto, l) - it->chunks);
+            it->first = first + lane_of(pupto, l) - lane_of(many, l);
+            it->c = c;
+            return true;
+        }
+        before += lane_of(upto, 63);
+        first += lane_of(pupto, 63);
+    }
+    return false;
+}
+
+// ------------------------------------------------------- operands of q and p
 template <int TYPE>
-__global__ __launch_bounds__(64) void attn_simple_kernel(AttnArgs a) {
-    __shared__ float q[256], ps[64];
-    __shared__ int64_t off[64];
-    const int h = blockIdx.x, b = blockIdx.y, j = h / a.group, lane = threadIdx.x, d = a.c.d;
-    const int n = a.t.lens[b];
-    for (int i = lane; i < d; i += 64) q[i] = a.q[(int64_t(b) * a.hq + h) * d + i];
+struct Terms;
+
+// x = t0 + t1 + t2 exactly, each the upper 16 bits of what is left.
+template <>
+struct Terms<IQ_KV_BF16> {
+    static constexpr int N = 3;
+    static constexpr float kUp = 0.0f;
+    static __device__ __forceinline__ void cut(const float (&x)[8], s16x8_t (&t)[N]) {
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = x[i];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            u32x4_t u;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t lo = __float_as_uint(r[2 * i]), hi = __float_as_uint(r[2 * i + 1]);
+                u[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+                if (k + 1 < N) {
+                    r[2 * i] -= __uint_as_float(lo & 0xffff0000u);
+                    r[2 * i + 1] -= __uint_as_float(hi & 0xffff0000u);
+                }
+            }
+            t[k] = __builtin_bit_cast(s16x8_t, u);
+        }
+    }
+    static __device__ __forceinline__ float4_t mma(s16x8_t a, s16x8_t b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+    }
+};
+
+// x = t0 + t1 to 22 bits.  p is scaled by 2^12 (and its sum with it), so that
+// what the terms drop stays below 2^-36 of the largest p.
+template <>
+struct Terms<IQ_KV_F16> {
+    static constexpr int N = 2;
+    static constexpr float kUp = 12.0f;
+    static __device__ __forceinline__ void cut(const float (&x)[8], s16x8_t (&t)[N]) {
+        half8_t h, l;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            h[i] = _Float16(x[i]);
+            l[i] = _Float16(x[i] - float(h[i]));
+        }
+        t[0] = __builtin_bit_cast(s16x8_t, h);
+        t[1] = __builtin_bit_cast(s16x8_t, l);
+    }
+    static __device__ __forceinline__ float4_t mma(s16x8_t a, s16x8_t b, float4_t c) {
+        return mfma16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
+    }
+};
+
+// DP: head_dim rounded up to 32, 64, 128 or 256.
+template <int TYPE, int DP>
+__global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel(AttnArgs a) {
+    using T = Terms<TYPE>;
+    constexpr int CH = DP / 8, RPI = 64 / CH, NI = kAttnTile / RPI;  // 16-byte chunks of a row, rows of a load, loads
+    constexpr int KC = DP / 32, VT = DP / 16;                       // steps of the first product, tiles of the second
+    constexpr int ROWB = DP * 2, KVB = kAttnTile * ROWB;
+    __shared__ __align__(16) char lds[kAttnWaves][2 * KVB];
+    __shared__ float wm[kAttnWaves][16], wl[kAttnWaves][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
+    Item it;
+    const uint32_t hidx = blockIdx.x % a.nh;
+    if (!find_item(a, blockIdx.x / a.nh, &it)) return;
+    const int b = it.b, n = it.n, d = a.c.d;
+    const int j = int(hidx) / a.ht, h0 = int(hidx) % a.ht * 16, gh = min(16, a.group - h0);
+    float* out = a.out + (int64_t(b) * a.hq + j * a.group + h0) * d;
+    if (hidx == 0 && it.j == 0 && threadIdx.x == 0) a.plan[b] = make_uint2(it.chunks, it.first);
+    if (n <= 0 || n > a.t.cap) {
+        const float x = n == 0 ? 0.0f : __builtin_nanf("");
+        for (int i = threadIdx.x; i < gh * d; i += 64 * kAttnWaves) out[i] = x;
+        return;
+    }
+    const int t0 = int(it.j * it.c) * kAttnTile, t1 = min(n, t0 + int(it.c) * kAttnTile);
+    const int ntiles = (t1 - t0 + kAttnTile - 1) / kAttnTile;
+
+    // row r of a tile: element offset of its (page, slot), 0 where there is none
+    bool poison = false;
+    const int32_t* table = a.t.table + b * a.t.ld;
+    auto row_offset = [&](int tile) -> int64_t {
+        const int tok = t0 + tile * kAttnTile + (lane & 31);
+        if (tok >= t1) return 0;
+        const uint32_t p = uint32_t(tok) / uint32_t(a.c.ps), s = uint32_t(tok) - p * uint32_t(a.c.ps);
+        const int32_t id = table[p];
+        const bool ok = id >= 0 && id < a.c.pages;
+        poison |= !ok;
+        return ok ? id * a.c.pstr + int64_t(s) * a.c.sstr : 0;
+    };
+    // chunks past the row's end repeat its first one (q is 0 there, and the
+    // sums of those columns are not written)
+    const int ch = lane % CH, chsrc = ch * 8 < d ? ch : 0;
+    const int64_t lane_off = j * a.c.hstr + chsrc * 8;
+    const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.c.k) + lane_off;
+    const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.c.v) + lane_off;
+    u32x4_t kr[NI], vr[NI];
+    auto load = [&](int64_t off) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int64_t o = __shfl(off, i * RPI + lane / CH);
+            kr[i] = *reinterpret_cast<const u32x4_t*>(kp + o);
+            vr[i] = *reinterpret_cast<const u32x4_t*>(vp + o);
+        }
+    };
+    // Chunk c of row r lies at chunk c ^ swizzle(r) of the row's place: the 16
+    // rows that a K read, and the 4 x 4 rows of which a V read takes 32 bytes,
+    // then fall on different banks.
+    constexpr int RPB = 256 / ROWB > 1 ? 256 / ROWB : 1;  // rows across the banks
+    auto ksw = [](int r) { return (r / RPB) & (CH < 16 ? CH - 1 : 15); };
+    auto vsw = [](int r) { return ((r / RPB) & (CH < 16 ? CH / 2 - 1 : 7)) * 2; };
+    char* kl = lds[wave];
+    char* vl = lds[wave] + KVB;
+
+    // q: column = head, 8 values of each 32-value step a lane
+    s16x8_t qt[KC][T::N];
+    float mul = a.mul;
+    {
+        const float* q = a.q + (int64_t(b) * a.hq + j * a.group + h0 + (col < gh ? col : 0)) * d;
+        float x[KC][8];
+        float big = 0.0f;
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            const int e = c * 32 + g * 8;
+            const bool in = col < gh && e < d;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[c][i] = in ? q[e + i] : 0.0f;
+                big = fmaxf(big, fabsf(x[c][i]));
+            }
+        }
+        if constexpr (TYPE == IQ_KV_F16) {
+            // the head's largest value to 2^13..2^14, undone on the scores
+            big = fmaxf(big, __shfl_xor(big, 16));
+            big = fmaxf(big, __shfl_xor(big, 32));
+            const int e = max(int(__float_as_uint(big) >> 23), 27) - 127;
+            const float up = __uint_as_float(uint32_t(127 + 13 - e) << 23);
+            mul *= __uint_as_float(uint32_t(127 - 13 + e) << 23);
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[c][i] *= up;
+        }
+#pragma unroll
+        for (int c = 0; c < KC; c++) T::cut(x[c], qt[c]);
+    }
+
+    float4_t o[VT];
+#pragma unroll
+    for (int i = 0; i < VT; i++) o[i] = float4_t{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    float* sc = a.sc ? a.sc + ((int64_t(b) * a.c.hk + j) * a.t.cap) * a.group + h0 + col : nullptr;
+
+    if (wave < ntiles) load(row_offset(wave));
+    int64_t off_next = wave + kAttnWaves < ntiles ? row_offset(wave + kAttnWaves) : 0;
+    for (int tile = wave; tile < ntiles; tile += kAttnWaves) {
+        const int tk = t0 + tile * kAttnTile;  // first token
+        const bool whole = tk + kAttnTile <= t1;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int r = i * RPI + lane / CH;
+            *reinterpret_cast<u32x4_t*>(kl + r * ROWB + (ch ^ ksw(r)) * 16) = kr[i];
+            // (a row past the end may hold anything: 0 times NaN is NaN)
+            const u32x4_t zero = {0, 0, 0, 0};
+            *reinterpret_cast<u32x4_t*>(vl + r * ROWB + (ch ^ vsw(r)) * 16) = whole || tk + r < t1 ? vr[i] : zero;
+        }
+        if (tile + kAttnWaves < ntiles) {
+            load(off_next);
+            if (tile + 2 * kAttnWaves < ntiles) off_next = row_offset(tile + 2 * kAttnWaves);
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        float s[8];
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+            float4_t acc = {0, 0, 0, 0};
+            const int r = hf * 16 + col;
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const s16x8_t kv = *reinterpret_cast<const s16x8_t*>(kl + r * ROWB + ((c * 4 + g) ^ ksw(r)) * 16);
+#pragma unroll
+                for (int k = 0; k < T::N; k++) acc = T::mma(kv, qt[c][k], acc);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int tok = tk + hf * 16 + g * 4 + i;
+                float x = acc[i] * mul;
+                if (!whole && tok >= t1) x = -INFINITY;
+                s[hf * 4 + i] = x;
+            }
+        }
+        if (sc && col < gh) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int tok = tk + (i >> 2) * 16 + g * 4 + (i & 3);
+                if (tok < t1) sc[int64_t(tok) * a.group] = s[i];
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < VT; i++) o[i] *= al;
+        }
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i] = __builtin_amdgcn_exp2f(s[i] - (m - T::kUp));
+            l += p[i];
+        }
+        s16x8_t pt[T::N];
+        T::cut(p, pt);
+#pragma unroll
+        for (int v = 0; v < VT; v++) {
+            if (v * 16 >= d) break;
+            // rows 4g..4g+3 of either half: lane 4r + c of 16 gives row r's
+            // 8-byte piece c, lane i gets the 4 rows' value of column i
+            s16x8_t av;
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int r = hf * 16 + g * 4 + col / 4;
+                const int at = r * ROWB + ((v * 2 + (col & 3) / 2) ^ vsw(r)) * 16 + (col & 1) * 8;
+                const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(
+                        (__attribute__((address_space(3))) char*)(vl) + at));
+#pragma unroll
+                for (int i = 0; i < 4; i++) av[hf * 4 + i] = x[i];
+            }
+#pragma unroll
+            for (int k = 0; k < T::N; k++) o[v] = T::mma(av, pt[k], o[v]);
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // the waves' results; the tiles' places are free once every wave is here
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (__any(poison)) l = __builtin_nanf("");
     __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
-    bool bad = n < 0 || n > a.t.cap;
-    for (int t0 = 0; !bad && t0 < n; t0 += 64) {
-        const int tok = t0 + lane;
-        const float s = tok < n ? score<TYPE>(a, q, b, j, tok, &bad) : -INFINITY;
-        if (__any(bad)) {
-            bad = true;
-            break;
-        }
-        float mx = s;
-        for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-        const float mn = fmaxf(m, mx), al = expf(m - mn), p = expf(s - mn);
-        float sum = p;
-        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-        l = l * al + sum;
-        m = mn;
-        ps[lane] = p;
-        if (tok < n) {
-            const int pg = tok / a.c.ps;
-            off[lane] = a.t.table[b * a.t.ld + pg] * a.c.pstr + int64_t(tok - pg * a.c.ps) * a.c.sstr + j * a.c.hstr;
-        }
-        __syncthreads();
-        for (int r = 0; r < 4; r++) o[r] *= al;
-        for (int i = 0; i < min(64, n - t0); i++) {
-            const uint16_t* v = reinterpret_cast<const uint16_t*>(a.c.v) + off[i];
-            for (int r = 0; r < 4; r++)
-                if (r * 64 + lane < d) o[r] = fmaf(ps[i], kv_to_f32<TYPE>(v[r * 64 + lane]), o[r]);
-        }
-        __syncthreads();
+    constexpr int OST = DP + 4;
+    static_assert(16 * OST * 4 <= 2 * KVB, "a wave's sums fit its tiles' place");
+    float* ol = reinterpret_cast<float*>(lds[wave]);
+#pragma unroll
+    for (int v = 0; v < VT; v++) *reinterpret_cast<float4_t*>(ol + col * OST + v * 16 + g * 4) = o[v];
+    if (g == 0) {
+        wm[wave][col] = m;
+        wl[wave][col] = l;
     }
-    const float inv = bad ? __builtin_nanf("") : (n == 0 ? 0.0f : 1.0f / l);
-    for (int r = 0; r < 4; r++)
-        if (r * 64 + lane < d) a.out[(int64_t(b) * a.hq + h) * d + r * 64 + lane] = n == 0 ? 0.0f : o[r] * inv;
-    if (a.w && lane == 0) {
-        a.ml[(int64_t(b) * a.hq + h) * 2] = m;
-        a.ml[(int64_t(b) * a.hq + h) * 2 + 1] = bad ? __builtin_nanf("") : l;
+    __syncthreads();
+    const bool alone = it.chunks == 1;
+    const int64_t slot = (int64_t(it.first) + it.j) * a.nh + hidx;
+    for (int i = threadIdx.x; i < gh * (d / 4); i += 64 * kAttnWaves) {
+        const int h = i / (d / 4), e = i % (d / 4) * 4;
+        float M = wm[0][h];
+#pragma unroll
+        for (int w = 1; w < kAttnWaves; w++) M = fmaxf(M, wm[w][h]);
+        float L = 0.0f;
+        float4_t x = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; w++) {
+            const float f = __builtin_amdgcn_exp2f(wm[w][h] - M);
+            L += wl[w][h] * f;
+            x += *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(lds[w]) + h * OST + e) * f;
+        }
+        float* to;
+        if (alone) {
+            const float inv = 1.0f / L;
+            x *= inv;
+            to = out + h * d + e;
+        } else {
+            to = a.part + slot * 16 * d + h * d + e;
+        }
+        if (e == 0) {
+            float* f = alone ? a.fin + (int64_t(b) * a.hq + j * a.group + h0 + h) * 2 : a.ml + slot * 32 + h * 2;
+            f[0] = M;
+            f[1] = L;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) to[r] = x[r];
+    }
+}
+
+// One workgroup per (head, sequence): the chunks' sums, each times 2^(its
+// maximum - the largest), in chunk order within 256 / (d / 4 rounded to a
+// power of two) runs that are then added in order.
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    __shared__ float4_t xs[256];
+    __shared__ float ls[256];
+    const int b = blockIdx.y, head = blockIdx.x, d = a.c.d, tid = threadIdx.x;
+    if (a.t.lens[b] <= 0 || a.t.lens[b] > a.t.cap) return;
+    const uint2 pl = a.plan[b];
+    if (pl.x < 2) return;
+    const int j = head / a.group, hg = head % a.group, hidx = j * a.ht + hg / 16, h = hg % 16;
+    const int64_t s0 = int64_t(pl.y) * a.nh + hidx;
+    auto ml = [&](int i) { return reinterpret_cast<const float2*>(a.ml)[(s0 + int64_t(i) * a.nh) * 16 + h]; };
+    const int n = int(pl.x);
+    float M = -INFINITY;
+    for (int i = tid & 63; i < n; i += 64) M = fmaxf(M, ml(i).x);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    int w = 2;  // 16-byte pieces of a row, to a power of two
+    while (w * 4 < d) w *= 2;
+    const int e = tid % w * 4, run = tid / w, runs = 256 / w;
+    float L = 0.0f;
+    float4_t x = {0, 0, 0, 0};
+    if (e < d) {
+#pragma unroll 4
+        for (int i = run; i < n; i += runs) {
+            const float2 v = ml(i);
+            const float f = __builtin_amdgcn_exp2f(v.x - M);
+            L += v.y * f;
+            x += *reinterpret_cast<const float4_t*>(a.part + (s0 + int64_t(i) * a.nh) * 16 * d + h * d + e) * f;
+        }
+    }
+    xs[tid] = x;
+    ls[tid] = L;
+    __syncthreads();
+    if (run == 0 && e < d) {
+        for (int r = 1; r < runs; r++) {
+            x += xs[r * w + tid];
+            L += ls[r * w + tid];
+        }
+        const float inv = 1.0f / L;
+        float* out = a.out + (int64_t(b) * a.hq + head) * d + e;
+#pragma unroll
+        for (int r = 0; r < 4; r++) out[r] = x[r] * inv;
+        if (e == 0) {
+            float* f = a.fin + (int64_t(b) * a.hq + head) * 2;
+            f[0] = M;
+            f[1] = L;
+        }
+    }
+}
+
+// weights[b][j][t] += sum over the group's heads, in order, of 2^(score -
+// maximum) / sum.
+__global__ __launch_bounds__(256) void attn_weights_kernel(AttnArgs a, float* weights, int64_t wld, float up) {
+    const int b = blockIdx.z, j = blockIdx.y, n = a.t.lens[b];
+    if (n > a.t.cap) return;
+    const int64_t row = int64_t(b) * a.c.hk + j;
+    for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < n; t += int64_t(gridDim.x) * 256) {
+        const float* s = a.sc + (row * a.t.cap + t) * a.group;
+        const float* f = a.fin + (int64_t(b) * a.hq + j * a.group) * 2;
+        float sum = 0.0f;
+        for (int h = 0; h < a.group; h++) sum += __builtin_amdgcn_exp2f(s[h] - (f[2 * h] - up)) / f[2 * h + 1];
+        weights[row * wld + t] += sum;
     }
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(256) void weights_simple_kernel(AttnArgs a) {
-    const int j = blockIdx.x, b = blockIdx.y, d = a.c.d;
-    const int n = a.t.lens[b];
-    if (n < 0 || n > a.t.cap) return;
-    for (int tok = threadIdx.x; tok < n; tok += 256) {
-        float sum = 0.0f;
-        for (int g = 0; g < a.group; g++) {
-            const int64_t h = int64_t(b) * a.hq + j * a.group + g;
-            bool bad = false;
-            const float s = score<TYPE>(a, a.q + h * d, b, j, tok, &bad);
-            sum += expf(s - a.ml[2 * h]) / a.ml[2 * h + 1];
-        }
-        a.w[(int64_t(b) * a.c.hk + j) * a.wld + tok] += sum;
-    }
+void launch_attn(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    if (a.c.d <= 32) attn_kernel<TYPE, 32><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else if (a.c.d <= 64) attn_kernel<TYPE, 64><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else if (a.c.d <= 128) attn_kernel<TYPE, 128><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else attn_kernel<TYPE, 256><<<grid, 64 * kAttnWaves, 0, s>>>(a);
 }
 
 }  // namespace
@@ -112,28 +493,49 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
     if (!q || !out) return IQ_ENULL;
     if (q_heads < 1 || q_heads > 16384 || q_heads % a.c.hk || !std::isfinite(scale)) return IQ_ESHAPE;
     if (weights && weights_ld < a.t.cap) return IQ_ESHAPE;
-    const int64_t bytes = int64_t(B) * q_heads * a.c.d * 4;
-    if (iq::ranges_overlap(q, bytes, out, bytes)) return IQ_EALIAS;
+    const int64_t row = int64_t(q_heads) * a.c.d;
+    if (iq::ranges_overlap(q, B * row * 4, out, B * row * 4)) return IQ_EALIAS;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     iq::Workspace* ws = nullptr;
     const hipError_t e = iq::get_workspace(s, &ws);
     if (e != hipSuccess) return e == hipErrorOutOfMemory ? IQ_ENOMEM : int(e);
-    a.q = q;
-    a.out = out;
-    a.w = weights;
-    a.wld = weights_ld;
-    a.ml = ws->partials;
     a.hq = q_heads;
     a.group = q_heads / a.c.hk;
-    a.scale = scale;
-    if (int64_t(B) * q_heads * 2 > ws->part_floats) return IQ_ETOOLARGE;
-    const dim3 g1(static_cast<unsigned>(q_heads), static_cast<unsigned>(B)), g2(static_cast<unsigned>(a.c.hk), static_cast<unsigned>(B));
-    if (kv->type == IQ_KV_BF16) {
-        iq::attn_simple_kernel<IQ_KV_BF16><<<g1, 64, 0, s>>>(a);
-        if (weights) iq::weights_simple_kernel<IQ_KV_BF16><<<g2, 256, 0, s>>>(a);
-    } else {
-        iq::attn_simple_kernel<IQ_KV_F16><<<g1, 64, 0, s>>>(a);
-        if (weights) iq::weights_simple_kernel<IQ_KV_F16><<<g2, 256, 0, s>>>(a);
+    a.ht = (a.group + 15) / 16;
+    a.nh = uint32_t(a.c.hk * a.ht);
+    a.mul = scale * 1.44269504088896340736f;
+    // two workgroups a CU (what the LDS of d <= 128 holds)
+    a.target = uint32_t(2 * iq::device_cu_count());
+    const int64_t capt = iq::attn_tiles(a.t.cap);
+    // the workspace's partial sums: plan | final (maximum, sum) | chunks' | rows;
+    // its GEMM operand area: the scores that the weights are made of
+    const int64_t slots = iq::attn_max_partials(a.target);
+    int64_t step = B;
+    step = std::min<int64_t>(step, (int64_t(1) << 30) / (capt * a.nh));
+    if (weights) step = std::min<int64_t>(step, int64_t(ws->gx_bytes / 4) / (int64_t(a.t.cap) * q_heads));
+    const int64_t fin = (step * q_heads * 2 + 63) / 64 * 64;
+    if (step < 1 || 2 * iq::kMaxSeqs + fin + slots * 16 * (2 + a.c.d) > ws->part_floats) return IQ_ETOOLARGE;
+    a.plan = reinterpret_cast<uint2*>(ws->partials);
+    a.fin = ws->partials + 2 * iq::kMaxSeqs;
+    a.ml = a.fin + fin;
+    a.part = a.ml + slots * 32;
+    a.sc = weights ? static_cast<float*>(ws->gx) : nullptr;
+    for (int b0 = 0; b0 < B; b0 += int(step)) {
+        a.B = int(std::min<int64_t>(step, B - b0));
+        a.q = q + b0 * row;
+        a.out = out + b0 * row;
+        a.t.table = table + b0 * table_ld;
+        a.t.lens = lens + b0;
+        const int64_t grid = iq::attn_max_items(a.B, a.nh, a.t.cap, a.target);
+        if (kv->type == IQ_KV_BF16) iq::launch_attn<IQ_KV_BF16>(a, unsigned(grid), s);
+        else iq::launch_attn<IQ_KV_F16>(a, unsigned(grid), s);
+        if (capt > iq::kAttnWaves)  // (else no sequence has two chunks)
+            iq::attn_join_kernel<<<dim3(unsigned(q_heads), unsigned(a.B)), 256, 0, s>>>(a);
+        if (weights) {
+            const int64_t blocks = std::min<int64_t>((a.t.cap + 255) / 256, 1024);
+            iq::attn_weights_kernel<<<dim3(unsigned(blocks), unsigned(a.c.hk), unsigned(a.B)), 256, 0, s>>>(
+                a, weights + int64_t(b0) * a.c.hk * weights_ld, weights_ld, kv->type == IQ_KV_F16 ? 12.0f : 0.0f);
+        }
     }
     return int(hipGetLastError());
 }

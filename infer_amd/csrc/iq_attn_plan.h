@@ -14,7 +14,7 @@
 #include <cstdint>
 
 #if defined(__HIPCC__)
-#define IQ_HD __host__ __device__ __forceinline__
+#define IQ_HD __host__ __device__ inline
 #else
 #define IQ_HD inline
 #endif
