@@ -200,7 +200,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     auto row_offset = [&](int tile) -> int64_t {
         const int tok = t0 + tile * kAttnTile + (lane & 31);
         if (tok >= t1) return 0;
-        const uint32_t p = uint32_t(tok) / uint32_t(a.c.ps), s = uint32_t(tok) - p * uint32_t(a.c.ps);
+        const uint32_t p = page_of(uint32_t(tok), a.c.div), s = uint32_t(tok) - p * uint32_t(a.c.ps);
         const int32_t id = table[p];
         const bool ok = id >= 0 && id < a.c.pages;
         poison |= !ok;

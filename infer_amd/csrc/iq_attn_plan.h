@@ -1,6 +1,7 @@
-// iq_attn_plan.h -- how a batch's cached tokens are split over workgroups:
-// arithmetic shared by the kernels of iq_attn.hip, their host side and the
-// CPU tests (plain C++: g++ compiles it on its own).
+// iq_attn_plan.h -- a token's page, and how a batch's cached tokens are split
+// over workgroups: arithmetic shared by the kernels of iq_kv.hip and
+// iq_attn.hip, their host side and the CPU tests (plain C++: g++ compiles it
+// on its own).
 //
 // Lengths are known on the device only.  Every sequence is cut into chunks
 // of the same number of 32-token tiles, C, chosen from the batch's total so
@@ -20,6 +21,21 @@
 #endif
 
 namespace iq {
+
+// Division by a page size: n / d = (n * mul) >> (31 + shift) for every n <
+// 2^31, where 2^(shift - 1) < d <= 2^shift and mul = ceil(2^(31 + shift) / d)
+// (mul * d exceeds 2^(31 + shift) by less than d <= 2^shift, n times that by
+// less than 2^(31 + shift)).
+struct PageDiv {
+    uint32_t mul, shift;
+};
+inline PageDiv page_div(uint32_t d) {
+    PageDiv p{0, 0};
+    while ((uint64_t(1) << p.shift) < d) p.shift++;
+    p.mul = uint32_t(((uint64_t(1) << (31 + p.shift)) + d - 1) / d);
+    return p;
+}
+IQ_HD uint32_t page_of(uint32_t n, PageDiv p) { return uint32_t((uint64_t(n) * p.mul) >> (31 + p.shift)); }
 
 constexpr int kAttnTile = 32;   // tokens a wave multiplies at a time
 constexpr int kAttnWaves = 4;   // waves of a workgroup: a chunk's tiles are dealt to them in turn

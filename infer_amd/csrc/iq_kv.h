@@ -5,6 +5,7 @@
 #include <cmath>
 
 #include "../../include/iq.h"
+#include "iq_attn_plan.h"
 #include "iq_internal.h"
 
 namespace iq {
@@ -15,6 +16,7 @@ struct KvView {
     int64_t pages, pstr, sstr, hstr;
     const char* k;
     const char* v;
+    PageDiv div;  // by ps
 };
 
 // A batch's block table: row b's page ids at table + b * ld, at most
@@ -72,6 +74,7 @@ inline int check_kv(const iq_kv* kv, KvView* out) {
     out->hstr = stride[2];
     out->k = static_cast<const char*>(kv->k);
     out->v = static_cast<const char*>(kv->v);
+    out->div = page_div(uint32_t(kv->page_size));
     return IQ_OK;
 }
 

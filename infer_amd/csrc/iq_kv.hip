@@ -112,14 +112,20 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 // budget.  That is what the call has to move; keeping the order of all rows
 // would move everything behind the first evicted one.
 //
-// evict_plan_kernel (one workgroup per sequence and head) finds the cut-th
-// largest sum by three histogram passes over its bits (11 + 11 + 10, highest
-// first) and writes the lists of free places and of rows that fill them.
-// evict_move_kernel moves rows: a workgroup has one sequence, head, K or V
-// (or the sums) and a slice of the row, and goes through the moves in order,
-// a chunk at a time: read, barrier, write.  No write of a chunk meets a read
-// of a later one: free places lie below cut and every source at or above
-// it, and the newest rows, after all of those, move down in ascending order.
+// evict_plan_kernel (one workgroup per sequence and head) holds up to 32768
+// sums in registers (longer ones are read again), finds the cut-th largest by
+// three histogram passes over its bits (11 + 11 + 10, highest first; four
+// copies of a histogram, since most sums share few exponents) and writes the
+// lists of free places and of the rows that fill them.
+//
+// The rows are moved by two kernels.  The free places lie below cut and every
+// source at or above it, so evict_fill_kernel moves those rows in any order.
+// evict_shift_kernel then moves the newest ones (and the sums).  Where they
+// move by less than their number, places and sources overlap, and one
+// workgroup goes through a slice of all rows in ascending order, a chunk at
+// a time: read, barrier, write; a chunk's writes lie below every later
+// chunk's reads.  With many sequences and heads that kernel does both, and
+// one launch is saved: the free places come first in its list.
 struct EvictArgs {
     KvView c;
     KvTable t;
@@ -132,11 +138,13 @@ struct EvictArgs {
     int32_t* dst;          // [sequences][hk][m]
     int32_t* src;
     int64_t m;
-    int slices, units;     // slices of a row, 16-byte units of a slice
-    int holes_done;        // the free places are filled by an earlier launch
+    int slices, ushift;    // slices of a row, of 1 << ushift 16-byte units
+    int blocks;            // workgroups along the rows, where the order is free
+    int filled;            // the free places are filled by an earlier launch
 };
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kBins = 2048, kCopies = 4;
+constexpr int kHeld = 32, kHeldSums = kHeld * kPlanThreads;  // sums in a thread's registers, in a workgroup's
 
 // Order of the sums: NaN lowest, then by value (-0 as 0).
 __device__ __forceinline__ uint32_t sum_key(float w) {
@@ -145,26 +153,26 @@ __device__ __forceinline__ uint32_t sum_key(float w) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ int wave_incl_scan(int v) {
+__device__ __forceinline__ uint32_t wave_incl_scan(uint32_t v) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o);
+        const uint32_t u = __shfl_up(v, o);
         if (lane >= o) v += u;
     }
     return v;
 }
 
 // Exclusive prefix of v over the workgroup's threads and its total.
-__device__ __forceinline__ int block_excl_scan(int v, int* total, int* sh) {
+__device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* total, uint32_t* sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int inc = wave_incl_scan(v);
+    const uint32_t inc = wave_incl_scan(v);
     __syncthreads();  // (sh may still be read from a previous scan)
     if (lane == 63) sh[wave] = inc;
     __syncthreads();
-    int before = 0, sum = 0;
+    uint32_t before = 0, sum = 0;
     for (int i = 0; i < kPlanWaves; i++) {
-        const int s = sh[i];
+        const uint32_t s = sh[i];
         if (i < wave) before += s;
         sum += s;
     }
@@ -173,9 +181,10 @@ __device__ __forceinline__ int block_excl_scan(int v, int* total, int* sh) {
 }
 
 __global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(EvictArgs a) {
-    __shared__ int hist[kCopies][kBins];
-    __shared__ int sh[kPlanWaves];
-    __shared__ int found[4];
+    __shared__ uint32_t hist[kCopies][kBins];
+    __shared__ uint32_t cnt[kHeld * kPlanWaves];  // of a run of 64 sums: entry (round, wave)
+    __shared__ uint32_t sh[kPlanWaves];
+    __shared__ uint32_t found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = blockIdx.x, b = a.b0 + int(blockIdx.y), row = int(blockIdx.y) * a.c.hk + h;
     const int n = a.t.lens[b];
@@ -201,162 +210,227 @@ __global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(EvictArgs a) {
         if (tid == 0) a.count[row] = 0;
         return;
     }
+    uint32_t k[kHeld];  // sum i0 + r * 1024 + tid
+    auto hold = [&](int i0) {
+#pragma unroll
+        for (int r = 0; r < kHeld; r++) {
+            const int i = i0 + r * kPlanThreads + tid;
+            k[r] = i < old ? sum_key(w[i]) : 0;
+        }
+    };
+    hold(0);
+    const bool all = old <= kHeldSums;
     // the cut-th largest key (1 <= cut < old)
-    uint32_t prefix = 0;
-    int want = cut, shift = 32;
-    int equal = 0;
+    uint32_t prefix = 0, want = uint32_t(cut), equal = 0;
+    int shift = 32;
     for (int pass = 0; pass < 3; pass++) {
         const int bits = pass < 2 ? 11 : 10;
+        __syncthreads();
         for (int i = tid; i < kCopies * kBins; i += kPlanThreads) (&hist[0][0])[i] = 0;
         __syncthreads();
         shift -= bits;
-        for (int i = tid; i < old; i += kPlanThreads) {
-            const uint32_t k = sum_key(w[i]);
-            const bool in = pass == 0 || (k >> (shift + bits)) == prefix;
-            if (in) atomicAdd(&hist[lane % kCopies][(k >> shift) & ((1u << bits) - 1)], 1);
+        for (int i0 = 0; i0 < old; i0 += kHeldSums) {
+            if (!all) hold(i0);
+#pragma unroll
+            for (int r = 0; r < kHeld; r++) {
+                if (i0 + r * kPlanThreads >= old) break;
+                const bool in = pass == 0 || (k[r] >> (shift + bits)) == prefix;
+                if (in && i0 + r * kPlanThreads + tid < old)
+                    atomicAdd(&hist[lane % kCopies][(k[r] >> shift) & ((1u << bits) - 1)], 1u);
+            }
         }
         __syncthreads();
         const int hi = kBins - 1 - 2 * tid, lo = hi - 1;
-        int nh = 0, nl = 0;
+        uint32_t nh = 0, nl = 0;
 #pragma unroll
         for (int c = 0; c < kCopies; c++) {
             nh += hist[c][hi];
             nl += hist[c][lo];
         }
-        int total;
-        const int before = block_excl_scan(nh + nl, &total, sh);
+        uint32_t total;
+        const uint32_t before = block_excl_scan(nh + nl, &total, sh);
         if (before < want && want <= before + nh + nl) {
             const bool first = want <= before + nh;
-            found[0] = first ? hi : lo;
+            found[0] = uint32_t(first ? hi : lo);
             found[1] = want - before - (first ? 0 : nh);
             found[2] = first ? nh : nl;
         }
         __syncthreads();
-        prefix = (prefix << bits) | uint32_t(found[0]);
+        prefix = (prefix << bits) | found[0];
         want = found[1];
         equal = found[2];
     }
-    // keys above `prefix` stay, of the equal ones the first `want`.  Every wave
-    // has a run of slots, 64 at a time in order.
-    const int seg = ((old + kPlanWaves - 1) / kPlanWaves + 63) / 64 * 64;
-    const int s0 = min(wave * seg, old), s1 = min(s0 + seg, old);
-    int eq_before = 0;
-    if (equal > want) {
-        int mine = 0;
-        for (int i = s0 + lane; i < s1; i += 64) mine += sum_key(w[i]) == prefix;
-        for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
-        __syncthreads();
-        if (lane == 0) sh[wave] = mine;
-        __syncthreads();
-        for (int i = 0; i < wave; i++) eq_before += sh[i];
-        __syncthreads();
-    }
+    // Keys above `prefix` stay, of the equal ones the first `want`.  In slot
+    // order (round, wave, lane) the ranks come from the ballots of the runs
+    // of 64 and a scan over the runs.
     const uint64_t below = lane ? (~uint64_t(0) >> (64 - lane)) : 0;
+    const bool ties = equal > want;
     int32_t* dst = a.dst + row * a.m;
     int32_t* src = a.src + row * a.m;
-    int holes = 0, highs = 0;  // of the waves before, then running
-    for (int pass = 0; pass < 2; pass++) {
-        int nhole = 0, nhigh = 0, eq = eq_before;
-        for (int i0 = s0; i0 < s1; i0 += 64) {
-            const int i = i0 + lane;
-            const uint32_t k = i < s1 ? sum_key(w[i]) : 0;
-            const bool same = i < s1 && k == prefix;
-            const uint64_t eqm = __ballot(same);
-            const bool keep = i < s1 && (k > prefix || (same && eq + __popcll(eqm & below) < want));
-            eq += __popcll(eqm);
-            const bool hole = i < s1 && !keep && i < cut, high = keep && i >= cut;
-            const uint64_t hm = __ballot(hole), gm = __ballot(high);
-            if (pass == 1) {
-                if (hole) dst[holes + nhole + __popcll(hm & below)] = i;
-                if (high) src[highs + nhigh + __popcll(gm & below)] = i;
-            }
-            nhole += __popcll(hm);
-            nhigh += __popcll(gm);
-        }
-        if (pass == 0) {
-            if (lane == 0) {
-                hist[0][wave] = nhole;
-                hist[1][wave] = nhigh;
+    uint32_t eqs = 0, holes = 0, highs = 0;  // of the sums before i0
+    for (int i0 = 0; i0 < old; i0 += kHeldSums) {
+        if (!all) hold(i0);
+        uint32_t total;
+        uint32_t keep = 0;  // bit r: the sum of round r stays
+        __syncthreads();
+        if (ties) {
+            if (tid < kHeld * kPlanWaves) cnt[tid] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < kHeld; r++) {
+                if (i0 + r * kPlanThreads >= old) break;
+                const uint64_t eq = __ballot(k[r] == prefix && i0 + r * kPlanThreads + tid < old);
+                if (lane == 0) cnt[r * kPlanWaves + wave] = uint32_t(__popcll(eq));
             }
             __syncthreads();
-            int all = 0;
-            for (int i = 0; i < kPlanWaves; i++) {
-                if (i < wave) {
-                    holes += hist[0][i];
-                    highs += hist[1][i];
-                }
-                all += hist[0][i];
-            }
-            if (tid == 0) a.count[row] = all;
+            const uint32_t c = tid < kHeld * kPlanWaves ? cnt[tid] : 0;
+            const uint32_t before = block_excl_scan(c, &total, sh);
+            if (tid < kHeld * kPlanWaves) cnt[tid] = eqs + before;
+            eqs += total;
+            __syncthreads();
         }
+#pragma unroll
+        for (int r = 0; r < kHeld; r++) {
+            const int i = i0 + r * kPlanThreads + tid;
+            bool stay = i < old && k[r] >= prefix;
+            if (ties) {
+                const bool same = i < old && k[r] == prefix;
+                const uint64_t eq = __ballot(same);
+                if (same) stay = cnt[r * kPlanWaves + wave] + uint32_t(__popcll(eq & below)) < want;
+            }
+            keep |= uint32_t(stay) << r;
+        }
+        __syncthreads();
+        if (tid < kHeld * kPlanWaves) cnt[tid] = 0;
+        __syncthreads();
+        // (at most 32768 of either: two counts in a word)
+#pragma unroll
+        for (int r = 0; r < kHeld; r++) {
+            const int i = i0 + r * kPlanThreads + tid;
+            if (i0 + r * kPlanThreads >= old) break;
+            const bool stay = keep >> r & 1;
+            const uint64_t hm = __ballot(i < cut && !stay), gm = __ballot(i >= cut && stay);
+            if (lane == 0) cnt[r * kPlanWaves + wave] = uint32_t(__popcll(hm)) | uint32_t(__popcll(gm)) << 16;
+        }
+        __syncthreads();
+        const uint32_t c = tid < kHeld * kPlanWaves ? cnt[tid] : 0;
+        const uint32_t before = block_excl_scan(c, &total, sh);
+        if (tid < kHeld * kPlanWaves) cnt[tid] = before;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kHeld; r++) {
+            const int i = i0 + r * kPlanThreads + tid;
+            if (i0 + r * kPlanThreads >= old) break;
+            const bool stay = keep >> r & 1;
+            const bool hole = i < cut && !stay, high = i >= cut && stay;
+            const uint64_t hm = __ballot(hole), gm = __ballot(high);
+            const uint32_t at = cnt[r * kPlanWaves + wave];
+            if (hole) dst[holes + (at & 0xffffu) + uint32_t(__popcll(hm & below))] = i;
+            if (high) src[highs + (at >> 16) + uint32_t(__popcll(gm & below))] = i;
+        }
+        holes += total & 0xffffu;
+        highs += total >> 16;
     }
+    if (tid == 0) a.count[row] = int32_t(holes);
 }
 
 // Byte offset of (token t of sequence b, head h) in either pool (page ids
 // were checked by the plan).
 __device__ __forceinline__ int64_t kv_offset(const KvView& c, const KvTable& t, int b, int h, int tok) {
-    const int p = tok / c.ps;
-    return 2 * (t.table[b * t.ld + p] * c.pstr + int64_t(tok - p * c.ps) * c.sstr + h * c.hstr);
+    const uint32_t p = page_of(uint32_t(tok), c.div);
+    return 2 * (t.table[b * t.ld + p] * c.pstr + int64_t(uint32_t(tok) - p * uint32_t(c.ps)) * c.sstr + h * c.hstr);
 }
 
 constexpr int kMoveThreads = 256, kMoveUnroll = 8;
 
-// grid: x = (K, V) x slices of a row, then one for the sums; y = head; z =
-// sequence.
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
+// Moves rows [m0, m1) of a list, a slice's 16-byte units of each from `u0` on: a
+// chunk of 8 units a thread is read, then (after a barrier, if the order
+// counts) written.
+template <bool ORDERED, class From, class To>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b, int h, int64_t m0, int64_t m1, int u0,
+                                          From from, To to) {
+    const int rows = kMoveThreads >> a.ushift, r0 = int(threadIdx.x) >> a.ushift;
+    const int u = u0 + (int(threadIdx.x) & ((1 << a.ushift) - 1));
+    const bool in = u < a.c.d / 8;
+    for (; m0 < m1; m0 += rows * kMoveUnroll) {
+        u32x4_t x[kMoveUnroll];
+#pragma unroll
+        for (int r = 0; r < kMoveUnroll; r++) {
+            const int64_t m = m0 + r * rows + r0;
+            if (in && m < m1)
+                x[r] = *reinterpret_cast<const u32x4_t*>(pool + kv_offset(a.c, a.t, b, h, from(int(m))) + u * 16);
+        }
+        if (ORDERED) {
+            __builtin_amdgcn_s_waitcnt(0);  // (the values are here before another wave writes)
+            __syncthreads();
+        }
+#pragma unroll
+        for (int r = 0; r < kMoveUnroll; r++) {
+            const int64_t m = m0 + r * rows + r0;
+            if (in && m < m1)
+                *reinterpret_cast<u32x4_t*>(pool + kv_offset(a.c, a.t, b, h, to(int(m))) + u * 16) = x[r];
+        }
+    }
+}
+
+// grid: x = (K, V) x slices x blocks of rows; y = head; z = sequence
+__global__ __launch_bounds__(kMoveThreads, 2) void evict_fill_kernel(EvictArgs a) {
+    const int h = blockIdx.y, b = a.b0 + int(blockIdx.z), row = int(blockIdx.z) * a.c.hk + h;
+    const int holes = a.count[row];
+    const int block = int(blockIdx.x) / (2 * a.slices), sl = int(blockIdx.x) % (2 * a.slices);
+    const int per = (kMoveThreads >> a.ushift) * kMoveUnroll;
+    const int64_t m0 = int64_t(block) * per;
+    if (m0 >= holes) return;
+    const int32_t* dst = a.dst + row * a.m;
+    const int32_t* src = a.src + row * a.m;
+    char* pool = const_cast<char*>(sl < a.slices ? a.c.k : a.c.v);
+    move_rows<false>(a, pool, b, h, m0, min(int64_t(holes), m0 + per), (sl % a.slices) << a.ushift,
+                     [&](int i) { return src[i]; }, [&](int i) { return dst[i]; });
+}
+
+// grid: x = (K, V) x slices x blocks of rows, then one for the sums; y = head;
+// z = sequence
+__global__ __launch_bounds__(kMoveThreads, 2) void evict_shift_kernel(EvictArgs a) {
     const int h = blockIdx.y, b = a.b0 + int(blockIdx.z), row = int(blockIdx.z) * a.c.hk + h;
     const int holes = a.count[row];
     if (holes < 0) return;
     const int n = a.t.lens[b], recent = int(a.recent), cut = int(a.budget) - recent, tid = threadIdx.x;
     const int32_t* dst = a.dst + row * a.m;
     const int32_t* src = a.src + row * a.m;
-    const int first = a.holes_done ? holes : 0;
     auto from = [&](int i) { return i < holes ? src[i] : n - recent + (i - holes); };
     auto to = [&](int i) { return i < holes ? dst[i] : cut + (i - holes); };
-    if (int(blockIdx.x) == 2 * a.slices) {
+    const int64_t moves = int64_t(holes) + recent;
+    if (int(blockIdx.x) == 2 * a.slices * a.blocks) {
         float* w = a.w + (int64_t(b) * a.c.hk + h) * a.wld;
-        for (int m0 = 0; m0 < holes + recent; m0 += kMoveThreads * kMoveUnroll) {
+        for (int64_t m0 = 0; m0 < moves; m0 += kMoveThreads * kMoveUnroll) {
             float x[kMoveUnroll];
 #pragma unroll
             for (int r = 0; r < kMoveUnroll; r++) {
-                const int i = m0 + r * kMoveThreads + tid;
-                x[r] = i < holes + recent ? w[from(i)] : 0.0f;
+                const int64_t i = m0 + r * kMoveThreads + tid;
+                x[r] = i < moves ? w[from(int(i))] : 0.0f;
             }
-            __builtin_amdgcn_s_waitcnt(0);  // (the values are here before another wave writes)
+            __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
 #pragma unroll
             for (int r = 0; r < kMoveUnroll; r++) {
-                const int i = m0 + r * kMoveThreads + tid;
-                if (i < holes + recent) w[to(i)] = x[r];
+                const int64_t i = m0 + r * kMoveThreads + tid;
+                if (i < moves) w[to(int(i))] = x[r];
             }
         }
         __syncthreads();
         for (int i = int(a.budget) + tid; i < n; i += kMoveThreads) w[i] = 0.0f;
         return;
     }
-    char* pool = const_cast<char*>(int(blockIdx.x) < a.slices ? a.c.k : a.c.v);
-    const int u0 = int(blockIdx.x) % a.slices * a.units, nu = min(a.units, a.c.d / 8 - u0);
-    const int64_t total = int64_t(holes + recent) * nu;
-    for (int64_t m0 = int64_t(first) * nu; m0 < total; m0 += kMoveThreads * kMoveUnroll) {
-        u32x4_t x[kMoveUnroll];
-#pragma unroll
-        for (int r = 0; r < kMoveUnroll; r++) {
-            const int64_t i = m0 + r * kMoveThreads + tid;
-            if (i < total) {
-                const int m = int(i / nu), u = int(i % nu);
-                x[r] = *reinterpret_cast<const u32x4_t*>(pool + kv_offset(a.c, a.t, b, h, from(m)) + (u0 + u) * 16);
-            }
-        }
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kMoveUnroll; r++) {
-            const int64_t i = m0 + r * kMoveThreads + tid;
-            if (i < total) {
-                const int m = int(i / nu), u = int(i % nu);
-                *reinterpret_cast<u32x4_t*>(pool + kv_offset(a.c, a.t, b, h, to(m)) + (u0 + u) * 16) = x[r];
-            }
-        }
+    const int block = int(blockIdx.x) / (2 * a.slices), sl = int(blockIdx.x) % (2 * a.slices);
+    char* pool = const_cast<char*>(sl < a.slices ? a.c.k : a.c.v);
+    const int u0 = (sl % a.slices) << a.ushift;
+    const int per = (kMoveThreads >> a.ushift) * kMoveUnroll;
+    if (a.filled && n - a.budget >= recent) {
+        // the newest rows' places and sources do not meet: any order
+        for (int64_t m0 = holes + int64_t(block) * per; m0 < moves; m0 += int64_t(a.blocks) * per)
+            move_rows<false>(a, pool, b, h, m0, min(moves, m0 + per), u0, from, to);
+    } else if (block == 0) {
+        move_rows<true>(a, pool, b, h, a.filled ? holes : 0, moves, u0, from, to);
     }
 }
 
@@ -426,16 +500,29 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
     a.count = reinterpret_cast<int32_t*>(ws->partials);
     a.dst = a.count + int64_t(step) * a.c.hk;
     a.src = a.dst + int64_t(step) * a.c.hk * m;
+    // a workgroup's slice of the rows: 64 bytes, so that an ordered move has
+    // as many workgroups as a row's length allows
     const int row_units = a.c.d / 8;
-    a.units = row_units;
-    a.slices = 1;
+    a.ushift = row_units >= 4 ? 2 : (row_units >= 2 ? 1 : 0);
+    a.slices = (row_units + (1 << a.ushift) - 1) >> a.ushift;
+    const int64_t per = (iq::kMoveThreads >> a.ushift) * iq::kMoveUnroll;
     for (a.b0 = 0; a.b0 < B; a.b0 += step) {
         const int nb = std::min(step, B - a.b0);
-        iq::evict_plan_kernel<<<dim3(unsigned(a.c.hk), unsigned(nb)), iq::kPlanThreads, 0, s>>>(a);
+        const unsigned hk = unsigned(a.c.hk), nz = unsigned(nb);
+        iq::evict_plan_kernel<<<dim3(hk, nz), iq::kPlanThreads, 0, s>>>(a);
         // (a cache that cannot hold more than the budget has nothing to move)
-        if (a.t.cap > budget)
-            iq::evict_move_kernel<<<dim3(unsigned(2 * a.slices + 1), unsigned(a.c.hk), unsigned(nb)),
-                                    iq::kMoveThreads, 0, s>>>(a);
+        if (a.t.cap <= budget) continue;
+        // fewer than two workgroups a CU in an ordered move: spread over blocks of rows
+        const int64_t wgs = int64_t(2) * a.slices * a.c.hk * nb;
+        a.filled = wgs < 2 * iq::device_cu_count() && m > per;
+        a.blocks = 1;
+        if (a.filled) {
+            a.blocks = int(std::min<int64_t>((m + per - 1) / per, 65536));
+            iq::evict_fill_kernel<<<dim3(2 * unsigned(a.slices * a.blocks), hk, nz), iq::kMoveThreads, 0, s>>>(a);
+            a.blocks = int(std::min<int64_t>((recent + per - 1) / per, 64));
+            a.blocks = std::max(a.blocks, 1);
+        }
+        iq::evict_shift_kernel<<<dim3(2 * unsigned(a.slices * a.blocks) + 1, hk, nz), iq::kMoveThreads, 0, s>>>(a);
     }
     return int(hipGetLastError());
 }
