@@ -59,24 +59,6 @@ struct AttnArgs {
     float* fin;       // [B][hq][2]: maximum and sum of every head, for the weights
 };
 
-// --------------------------------------------------- sums over a wave (DPP)
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
-    return v + uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROW_MASK, 0xf, true));
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    v = dpp_add<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8: within 16 lanes
-    v = dpp_add<0x112, 0xf>(v);
-    v = dpp_add<0x114, 0xf>(v);
-    v = dpp_add<0x118, 0xf>(v);
-    v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-    v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-    return v;
-}
-__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
-    return uint32_t(__builtin_amdgcn_readlane(int(v), lane));
-}
-
 struct Item {
     int b, n;            // sequence and its length (as given)
     uint32_t j, c, chunks, first;  // chunk, tiles of a chunk, chunks of the sequence, its first partial
@@ -204,12 +186,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
         const int32_t id = table[p];
         const bool ok = id >= 0 && id < a.c.pages;
         poison |= !ok;
-        return ok ? id * a.c.pstr + int64_t(s) * a.c.sstr : 0;
+        return ok ? kv_element(a.c, uint32_t(id), s, 0) : 0;
     };
     // chunks past the row's end repeat its first one (q is 0 there, and the
     // sums of those columns are not written)
     const int ch = lane % CH, chsrc = ch * 8 < d ? ch : 0;
-    const int64_t lane_off = j * a.c.hstr + chsrc * 8;
+    const int64_t lane_off = int64_t(uint64_t(j) * a.c.hstr) + chsrc * 8;
     const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.c.k) + lane_off;
     const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.c.v) + lane_off;
     u32x4_t kr[NI], vr[NI];

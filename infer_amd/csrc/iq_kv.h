@@ -10,10 +10,12 @@
 
 namespace iq {
 
-// Kernel-argument copy of iq_kv, strides in elements of 2 bytes.
+// Kernel-argument copy of iq_kv, strides in elements of 2 bytes (at most
+// 2^30, so that a product with an index is one 32 x 32 bit multiplication).
 struct KvView {
     int32_t type, hk, d, ps;
-    int64_t pages, pstr, sstr, hstr;
+    int64_t pages;
+    uint32_t pstr, sstr, hstr;
     const char* k;
     const char* v;
     PageDiv div;  // by ps
@@ -30,6 +32,11 @@ struct KvTable {
 
 constexpr int kMaxSeqs = 1024;
 
+// Element offset of (page id, slot, head) in either pool, id in [0, pages).
+__device__ __forceinline__ int64_t kv_element(const KvView& c, uint32_t id, uint32_t slot, uint32_t head) {
+    return int64_t(uint64_t(id) * c.pstr + uint64_t(slot) * c.sstr + uint64_t(head) * c.hstr);
+}
+
 // Element of a 16-bit cache as fp32, and back (to nearest even).
 template <int TYPE>
 __device__ __forceinline__ float kv_to_f32(uint16_t u) {
@@ -40,6 +47,24 @@ template <int TYPE>
 __device__ __forceinline__ uint16_t f32_to_kv(float f) {
     if constexpr (TYPE == IQ_KV_BF16) return f32_to_bf16(f);
     else return __builtin_bit_cast(uint16_t, _Float16(f));
+}
+
+// Inclusive prefix sum over a wave's lanes (DPP: no LDS).
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+    return v + uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROW_MASK, 0xf, true));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = dpp_add<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8: within 16 lanes
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+    return uint32_t(__builtin_amdgcn_readlane(int(v), lane));
 }
 
 inline bool ranges_overlap(const void* a, int64_t abytes, const void* b, int64_t bbytes) {
@@ -69,9 +94,9 @@ inline int check_kv(const iq_kv* kv, KvView* out) {
     out->d = kv->head_dim;
     out->ps = kv->page_size;
     out->pages = kv->pages;
-    out->pstr = stride[0];
-    out->sstr = stride[1];
-    out->hstr = stride[2];
+    out->pstr = uint32_t(stride[0]);
+    out->sstr = uint32_t(stride[1]);
+    out->hstr = uint32_t(stride[2]);
     out->k = static_cast<const char*>(kv->k);
     out->v = static_cast<const char*>(kv->v);
     out->div = page_div(uint32_t(kv->page_size));

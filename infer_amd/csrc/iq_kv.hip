@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const int64_t slot = a.slots[t];
     const bool live = slot >= 0 && slot < a.c.pages * a.c.ps;
     const int64_t page = live ? slot / a.c.ps : 0;
-    const int64_t base = page * a.c.pstr + (live ? slot % a.c.ps : 0) * a.c.sstr;
+    const int64_t base = kv_element(a.c, uint32_t(page), live ? uint32_t(slot - page * a.c.ps) : 0, 0);
     const int per = d / 8;  // 4-pair units of a head
     const int h0 = blockIdx.y * kAppendHeads, h1 = min(h0 + kAppendHeads, heads);
     for (int u = threadIdx.x; u < (h1 - h0) * per; u += 256) {
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
                 dst[e1 + r] = y1[r];
             }
         } else {
-            uint16_t* dst = reinterpret_cast<uint16_t*>(const_cast<char*>(is_k ? a.c.k : a.c.v)) + base + j * a.c.hstr;
+            uint16_t* dst = reinterpret_cast<uint16_t*>(const_cast<char*>(is_k ? a.c.k : a.c.v)) + base + uint64_t(j) * a.c.hstr;
             store_kv4<TYPE>(dst + e0, y0);
             store_kv4<TYPE>(dst + e1, y1);
         }
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 // would move everything behind the first evicted one.
 //
 // evict_plan_kernel (one workgroup per sequence and head) holds up to 32768
-// sums in registers (longer ones are read again), finds the cut-th largest by
+// sums in registers (longer rows are read again), finds the cut-th largest by
 // three histogram passes over its bits (11 + 11 + 10, highest first; four
 // copies of a histogram, since most sums share few exponents) and writes the
 // lists of free places and of the rows that fill them.
@@ -143,8 +143,7 @@ struct EvictArgs {
     int filled;            // the free places are filled by an earlier launch
 };
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kBins = 2048, kCopies = 4;
-constexpr int kHeld = 32, kHeldSums = kHeld * kPlanThreads;  // sums in a thread's registers, in a workgroup's
+constexpr int kBins = 2048, kCopies = 4;
 
 // Order of the sums: NaN lowest, then by value (-0 as 0).
 __device__ __forceinline__ uint32_t sum_key(float w) {
@@ -153,25 +152,17 @@ __device__ __forceinline__ uint32_t sum_key(float w) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ uint32_t wave_incl_scan(uint32_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
-    return v;
-}
-
-// Exclusive prefix of v over the workgroup's threads and its total.
+// Exclusive prefix of v over the workgroup's W waves of threads and its total.
+template <int W>
 __device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* total, uint32_t* sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t inc = wave_incl_scan(v);
+    const uint32_t inc = wave_scan(v);
     __syncthreads();  // (sh may still be read from a previous scan)
     if (lane == 63) sh[wave] = inc;
     __syncthreads();
     uint32_t before = 0, sum = 0;
-    for (int i = 0; i < kPlanWaves; i++) {
+#pragma unroll
+    for (int i = 0; i < W; i++) {
         const uint32_t s = sh[i];
         if (i < wave) before += s;
         sum += s;
@@ -180,153 +171,179 @@ __device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* total,
     return before + inc - v;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(EvictArgs a) {
-    __shared__ uint32_t hist[kCopies][kBins];
-    __shared__ uint32_t cnt[kHeld * kPlanWaves];  // of a run of 64 sums: entry (round, wave)
-    __shared__ uint32_t sh[kPlanWaves];
+// The lanes of the 64 slots from i on that lie below `end`.
+__device__ __forceinline__ uint64_t lanes_below(int i, int end) {
+    const int c = end - i;
+    return c >= 64 ? ~uint64_t(0) : (c <= 0 ? 0 : (uint64_t(1) << c) - 1);
+}
+
+__device__ __forceinline__ uint32_t lanes_before(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
+}
+
+// A wave holds a run of up to HELD x 64 sums in slot order, 64 in a round, so
+// that ranks are a scan over the waves and counts of ballots, which the scalar
+// unit makes (the places below cut and past the end are masks of it too).
+template <int W, int HELD>
+__global__ __launch_bounds__(64 * W) void evict_plan_kernel(EvictArgs a) {
+    constexpr int TH = 64 * W, BLOCK = TH * HELD, PER = kBins / TH;
+    __shared__ __align__(16) uint32_t hist[kCopies][kBins + 16];  // (the copies on different banks)
+    __shared__ uint32_t sh[W];
     __shared__ uint32_t found[3];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x, b = a.b0 + int(blockIdx.y), row = int(blockIdx.y) * a.c.hk + h;
     const int n = a.t.lens[b];
-    bool bad = n < 0 || n > a.t.cap;
-    if (!bad) {
-        const int np = (n + a.c.ps - 1) / a.c.ps;
+    const bool fits = n >= 0 && n <= a.t.cap, over = fits && n > a.budget;
+    const int old = n - int(a.recent), cut = int(a.budget - a.recent);
+    const float* w = a.w + (int64_t(b) * a.c.hk + h) * a.wld;
+    // this block of sums: rounds of a wave, its first slot; keys of places
+    // past the end are 0
+    uint32_t k[HELD];
+    int rounds = 0, w0 = 0;
+    auto hold = [&](int i0) {
+        rounds = (min(old - i0, BLOCK) + TH - 1) / TH;
+        w0 = i0 + wave * rounds * 64;
+        float x[HELD];
+#pragma unroll
+        for (int r = 0; r < HELD; r++) {
+            if (r >= rounds) break;
+            x[r] = w[min(w0 + r * 64 + lane, old - 1)];
+        }
+#pragma unroll
+        for (int r = 0; r < HELD; r++) {
+            if (r >= rounds) break;
+            k[r] = w0 + r * 64 + lane < old ? sum_key(x[r]) : 0;
+        }
+    };
+    if (over && cut) hold(0);
+    bool bad = !fits;
+    if (over) {
+        const int np = int(page_of(uint32_t(n - 1), a.c.div)) + 1;
         bool mine = false;
-        for (int i = tid; i < np; i += kPlanThreads) {
+        for (int i = tid; i < np; i += TH) {
             const int p = a.t.table[b * a.t.ld + i];
             mine |= p < 0 || p >= a.c.pages;
         }
         bad = __syncthreads_or(mine);
     }
-    const bool idle = bad || n <= a.budget;
+    const bool idle = bad || !over;
     if (h == 0 && tid == 0) a.new_lens[b] = idle ? n : int(a.budget);
-    if (idle) {
-        if (tid == 0) a.count[row] = -1;
+    if (idle || cut == 0) {
+        if (tid == 0) a.count[row] = idle ? -1 : 0;
         return;
     }
-    const int old = n - int(a.recent), cut = int(a.budget - a.recent);
-    const float* w = a.w + (int64_t(b) * a.c.hk + h) * a.wld;
-    if (cut == 0) {
-        if (tid == 0) a.count[row] = 0;
-        return;
-    }
-    uint32_t k[kHeld];  // sum i0 + r * 1024 + tid
-    auto hold = [&](int i0) {
-#pragma unroll
-        for (int r = 0; r < kHeld; r++) {
-            const int i = i0 + r * kPlanThreads + tid;
-            k[r] = i < old ? sum_key(w[i]) : 0;
-        }
-    };
-    hold(0);
-    const bool all = old <= kHeldSums;
-    // the cut-th largest key (1 <= cut < old)
+    const bool all = old <= BLOCK;
+    // the cut-th largest key (1 <= cut < old): its upper bits, until the
+    // keys that share them are all wanted (mostly after two passes)
     uint32_t prefix = 0, want = uint32_t(cut), equal = 0;
     int shift = 32;
     for (int pass = 0; pass < 3; pass++) {
         const int bits = pass < 2 ? 11 : 10;
-        __syncthreads();
-        for (int i = tid; i < kCopies * kBins; i += kPlanThreads) (&hist[0][0])[i] = 0;
+        for (int i = tid; i < kCopies * (kBins + 16) / 4; i += TH)
+            reinterpret_cast<uint4*>(&hist[0][0])[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         shift -= bits;
-        for (int i0 = 0; i0 < old; i0 += kHeldSums) {
+        uint32_t* mine = hist[lane % kCopies];
+        uint32_t past = 0;  // keys 0 of places past the end
+        for (int i0 = 0; i0 < old; i0 += BLOCK) {
             if (!all) hold(i0);
+            past += uint32_t(rounds * TH - min(old - i0, BLOCK));
 #pragma unroll
-            for (int r = 0; r < kHeld; r++) {
-                if (i0 + r * kPlanThreads >= old) break;
-                const bool in = pass == 0 || (k[r] >> (shift + bits)) == prefix;
-                if (in && i0 + r * kPlanThreads + tid < old)
-                    atomicAdd(&hist[lane % kCopies][(k[r] >> shift) & ((1u << bits) - 1)], 1u);
+            for (int r = 0; r < HELD; r++) {
+                if (r >= rounds) break;
+                if (pass == 0) {
+                    atomicAdd(&mine[k[r] >> 21], 1u);
+                } else if ((k[r] >> (shift + bits)) == prefix) {
+                    atomicAdd(&mine[(k[r] >> shift) & ((1u << bits) - 1)], 1u);
+                }
             }
         }
         __syncthreads();
-        const int hi = kBins - 1 - 2 * tid, lo = hi - 1;
-        uint32_t nh = 0, nl = 0;
+        // bins from the highest down, PER a thread
+        uint32_t nb[PER], sum = 0;
 #pragma unroll
-        for (int c = 0; c < kCopies; c++) {
-            nh += hist[c][hi];
-            nl += hist[c][lo];
+        for (int i = 0; i < PER; i++) {
+            nb[i] = 0;
+            const int bin = kBins - 1 - PER * tid - i;
+#pragma unroll
+            for (int c = 0; c < kCopies; c++) nb[i] += hist[c][bin];
+            if (bin == 0 && prefix == 0) nb[i] -= past;
+            sum += nb[i];
         }
-        uint32_t total;
-        const uint32_t before = block_excl_scan(nh + nl, &total, sh);
-        if (before < want && want <= before + nh + nl) {
-            const bool first = want <= before + nh;
-            found[0] = uint32_t(first ? hi : lo);
-            found[1] = want - before - (first ? 0 : nh);
-            found[2] = first ? nh : nl;
+        uint32_t total, before = block_excl_scan<W>(sum, &total, sh);
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            if (before < want && want <= before + nb[i]) {
+                found[0] = uint32_t(kBins - 1 - PER * tid - i);
+                found[1] = want - before;
+                found[2] = nb[i];
+            }
+            before += nb[i];
         }
         __syncthreads();
         prefix = (prefix << bits) | found[0];
         want = found[1];
         equal = found[2];
+        if (equal == want) break;
     }
-    // Keys above `prefix` stay, of the equal ones the first `want`.  In slot
-    // order (round, wave, lane) the ranks come from the ballots of the runs
-    // of 64 and a scan over the runs.
-    const uint64_t below = lane ? (~uint64_t(0) >> (64 - lane)) : 0;
+    // Keys from `least` on stay; with ties (all 32 bits are known then), of
+    // the keys equal to it the first `want`.
+    const uint32_t least = prefix << shift;
     const bool ties = equal > want;
     int32_t* dst = a.dst + row * a.m;
     int32_t* src = a.src + row * a.m;
-    uint32_t eqs = 0, holes = 0, highs = 0;  // of the sums before i0
-    for (int i0 = 0; i0 < old; i0 += kHeldSums) {
+    uint32_t eqs = 0, holes = 0, highs = 0;  // of the blocks before
+    for (int i0 = 0; i0 < old; i0 += BLOCK) {
         if (!all) hold(i0);
-        uint32_t total;
-        uint32_t keep = 0;  // bit r: the sum of round r stays
-        __syncthreads();
+        uint32_t total, eq = 0;
         if (ties) {
-            if (tid < kHeld * kPlanWaves) cnt[tid] = 0;
-            __syncthreads();
 #pragma unroll
-            for (int r = 0; r < kHeld; r++) {
-                if (i0 + r * kPlanThreads >= old) break;
-                const uint64_t eq = __ballot(k[r] == prefix && i0 + r * kPlanThreads + tid < old);
-                if (lane == 0) cnt[r * kPlanWaves + wave] = uint32_t(__popcll(eq));
+            for (int r = 0; r < HELD; r++) {
+                if (r >= rounds) break;
+                eq += uint32_t(__popcll(__ballot(k[r] == least) & lanes_below(w0 + r * 64, old)));
             }
-            __syncthreads();
-            const uint32_t c = tid < kHeld * kPlanWaves ? cnt[tid] : 0;
-            const uint32_t before = block_excl_scan(c, &total, sh);
-            if (tid < kHeld * kPlanWaves) cnt[tid] = eqs + before;
+            eq = eqs + block_excl_scan<W>(lane == 0 ? eq : 0, &total, sh);
+            eq = uint32_t(__builtin_amdgcn_readfirstlane(int(eq)));
             eqs += total;
-            __syncthreads();
         }
+        // the lanes whose sum stays (eq: equal ones before)
+        auto stays = [&](int r, uint32_t& eq_now) -> uint64_t {
+            const uint64_t in = lanes_below(w0 + r * 64, old);
+            if (!ties) return __ballot(k[r] >= least) & in;
+            const uint64_t same = __ballot(k[r] == least) & in;
+            const uint64_t more = __ballot(k[r] > least) & in;
+            const uint64_t first = __ballot(eq_now + lanes_before(same) < want) & same;
+            eq_now += uint32_t(__popcll(same));
+            return more | first;
+        };
+        // (a block has at most 32768 of either: two counts in a word)
+        uint32_t count = 0, e = eq;
 #pragma unroll
-        for (int r = 0; r < kHeld; r++) {
-            const int i = i0 + r * kPlanThreads + tid;
-            bool stay = i < old && k[r] >= prefix;
-            if (ties) {
-                const bool same = i < old && k[r] == prefix;
-                const uint64_t eq = __ballot(same);
-                if (same) stay = cnt[r * kPlanWaves + wave] + uint32_t(__popcll(eq & below)) < want;
+        for (int r = 0; r < HELD; r++) {
+            if (r >= rounds) break;
+            const uint64_t stay = stays(r, e), low = lanes_below(w0 + r * 64, cut);
+            const uint64_t in = lanes_below(w0 + r * 64, old);
+            count += uint32_t(__popcll(low & in & ~stay)) + (uint32_t(__popcll(stay & ~low)) << 16);
+        }
+        uint32_t at = block_excl_scan<W>(lane == 0 ? count : 0, &total, sh);
+        at = uint32_t(__builtin_amdgcn_readfirstlane(int(at)));
+        int32_t* hole = dst + holes + (at & 0xffffu);
+        int32_t* high = src + highs + (at >> 16);
+        e = eq;
+#pragma unroll
+        for (int r = 0; r < HELD; r++) {
+            if (r >= rounds) break;
+            const int i = w0 + r * 64;
+            const uint64_t stay = stays(r, e), low = lanes_below(i, cut);
+            const uint64_t to = low & lanes_below(i, old) & ~stay, from = stay & ~low;
+            if (to) {
+                if (to >> lane & 1) hole[lanes_before(to)] = i + lane;
+                hole += __popcll(to);
             }
-            keep |= uint32_t(stay) << r;
-        }
-        __syncthreads();
-        if (tid < kHeld * kPlanWaves) cnt[tid] = 0;
-        __syncthreads();
-        // (at most 32768 of either: two counts in a word)
-#pragma unroll
-        for (int r = 0; r < kHeld; r++) {
-            const int i = i0 + r * kPlanThreads + tid;
-            if (i0 + r * kPlanThreads >= old) break;
-            const bool stay = keep >> r & 1;
-            const uint64_t hm = __ballot(i < cut && !stay), gm = __ballot(i >= cut && stay);
-            if (lane == 0) cnt[r * kPlanWaves + wave] = uint32_t(__popcll(hm)) | uint32_t(__popcll(gm)) << 16;
-        }
-        __syncthreads();
-        const uint32_t c = tid < kHeld * kPlanWaves ? cnt[tid] : 0;
-        const uint32_t before = block_excl_scan(c, &total, sh);
-        if (tid < kHeld * kPlanWaves) cnt[tid] = before;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kHeld; r++) {
-            const int i = i0 + r * kPlanThreads + tid;
-            if (i0 + r * kPlanThreads >= old) break;
-            const bool stay = keep >> r & 1;
-            const bool hole = i < cut && !stay, high = i >= cut && stay;
-            const uint64_t hm = __ballot(hole), gm = __ballot(high);
-            const uint32_t at = cnt[r * kPlanWaves + wave];
-            if (hole) dst[holes + (at & 0xffffu) + uint32_t(__popcll(hm & below))] = i;
-            if (high) src[highs + (at >> 16) + uint32_t(__popcll(gm & below))] = i;
+            if (from) {
+                if (from >> lane & 1) high[lanes_before(from)] = i + lane;
+                high += __popcll(from);
+            }
         }
         holes += total & 0xffffu;
         highs += total >> 16;
@@ -338,59 +355,60 @@ __global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(EvictArgs a) {
 // were checked by the plan).
 __device__ __forceinline__ int64_t kv_offset(const KvView& c, const KvTable& t, int b, int h, int tok) {
     const uint32_t p = page_of(uint32_t(tok), c.div);
-    return 2 * (t.table[b * t.ld + p] * c.pstr + int64_t(uint32_t(tok) - p * uint32_t(c.ps)) * c.sstr + h * c.hstr);
+    return 2 * kv_element(c, uint32_t(t.table[b * t.ld + p]), uint32_t(tok) - p * uint32_t(c.ps), uint32_t(h));
 }
 
-constexpr int kMoveThreads = 256, kMoveUnroll = 8;
+constexpr int kMoveThreads = 256, kMoveUnroll = 4;
 
-// Moves rows [m0, m1) of a list, a slice's 16-byte units of each from `u0` on: a
-// chunk of 8 units a thread is read, then (after a barrier, if the order
-// counts) written.
+// Moves rows [m0, m1) of a list (m1 - m0 at most 2^31 less a chunk), a
+// slice's 16-byte units of each from `u0` on: a chunk of 4 units a thread is
+// read, then (after a barrier, if the order counts) written.
 template <bool ORDERED, class From, class To>
-__device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b, int h, int64_t m0, int64_t m1, int u0,
-                                          From from, To to) {
+__device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b, int h, int m0, int m1, int u0, From from,
+                                          To to) {
     const int rows = kMoveThreads >> a.ushift, r0 = int(threadIdx.x) >> a.ushift;
     const int u = u0 + (int(threadIdx.x) & ((1 << a.ushift) - 1));
-    const bool in = u < a.c.d / 8;
+    const int left = u < a.c.d / 8 ? m1 - r0 : 0;  // rows from m on are this thread's while m < left
+    pool += u * 16;
     for (; m0 < m1; m0 += rows * kMoveUnroll) {
         u32x4_t x[kMoveUnroll];
+        int64_t go[kMoveUnroll];
 #pragma unroll
         for (int r = 0; r < kMoveUnroll; r++) {
-            const int64_t m = m0 + r * rows + r0;
-            if (in && m < m1)
-                x[r] = *reinterpret_cast<const u32x4_t*>(pool + kv_offset(a.c, a.t, b, h, from(int(m))) + u * 16);
+            const int m = m0 + r * rows;
+            if (m < left) {
+                x[r] = *reinterpret_cast<const u32x4_t*>(pool + kv_offset(a.c, a.t, b, h, from(m + r0)));
+                go[r] = kv_offset(a.c, a.t, b, h, to(m + r0));
+            }
         }
         if (ORDERED) {
             __builtin_amdgcn_s_waitcnt(0);  // (the values are here before another wave writes)
             __syncthreads();
         }
 #pragma unroll
-        for (int r = 0; r < kMoveUnroll; r++) {
-            const int64_t m = m0 + r * rows + r0;
-            if (in && m < m1)
-                *reinterpret_cast<u32x4_t*>(pool + kv_offset(a.c, a.t, b, h, to(int(m))) + u * 16) = x[r];
-        }
+        for (int r = 0; r < kMoveUnroll; r++)
+            if (m0 + r * rows < left) *reinterpret_cast<u32x4_t*>(pool + go[r]) = x[r];
     }
 }
 
 // grid: x = (K, V) x slices x blocks of rows; y = head; z = sequence
-__global__ __launch_bounds__(kMoveThreads, 2) void evict_fill_kernel(EvictArgs a) {
+__global__ __launch_bounds__(kMoveThreads, 4) void evict_fill_kernel(EvictArgs a) {
     const int h = blockIdx.y, b = a.b0 + int(blockIdx.z), row = int(blockIdx.z) * a.c.hk + h;
     const int holes = a.count[row];
     const int block = int(blockIdx.x) / (2 * a.slices), sl = int(blockIdx.x) % (2 * a.slices);
     const int per = (kMoveThreads >> a.ushift) * kMoveUnroll;
-    const int64_t m0 = int64_t(block) * per;
+    const int m0 = block * per;
     if (m0 >= holes) return;
     const int32_t* dst = a.dst + row * a.m;
     const int32_t* src = a.src + row * a.m;
     char* pool = const_cast<char*>(sl < a.slices ? a.c.k : a.c.v);
-    move_rows<false>(a, pool, b, h, m0, min(int64_t(holes), m0 + per), (sl % a.slices) << a.ushift,
+    move_rows<false>(a, pool, b, h, m0, min(holes, m0 + per), (sl % a.slices) << a.ushift,
                      [&](int i) { return src[i]; }, [&](int i) { return dst[i]; });
 }
 
 // grid: x = (K, V) x slices x blocks of rows, then one for the sums; y = head;
 // z = sequence
-__global__ __launch_bounds__(kMoveThreads, 2) void evict_shift_kernel(EvictArgs a) {
+__global__ __launch_bounds__(kMoveThreads, 4) void evict_shift_kernel(EvictArgs a) {
     const int h = blockIdx.y, b = a.b0 + int(blockIdx.z), row = int(blockIdx.z) * a.c.hk + h;
     const int holes = a.count[row];
     if (holes < 0) return;
@@ -399,22 +417,22 @@ __global__ __launch_bounds__(kMoveThreads, 2) void evict_shift_kernel(EvictArgs 
     const int32_t* src = a.src + row * a.m;
     auto from = [&](int i) { return i < holes ? src[i] : n - recent + (i - holes); };
     auto to = [&](int i) { return i < holes ? dst[i] : cut + (i - holes); };
-    const int64_t moves = int64_t(holes) + recent;
+    const int moves = holes + recent;  // (at most the budget)
     if (int(blockIdx.x) == 2 * a.slices * a.blocks) {
         float* w = a.w + (int64_t(b) * a.c.hk + h) * a.wld;
-        for (int64_t m0 = 0; m0 < moves; m0 += kMoveThreads * kMoveUnroll) {
+        for (int m0 = 0; m0 < moves; m0 += kMoveThreads * kMoveUnroll) {
             float x[kMoveUnroll];
 #pragma unroll
             for (int r = 0; r < kMoveUnroll; r++) {
-                const int64_t i = m0 + r * kMoveThreads + tid;
-                x[r] = i < moves ? w[from(int(i))] : 0.0f;
+                const int i = m0 + r * kMoveThreads + tid;
+                x[r] = i < moves ? w[from(i)] : 0.0f;
             }
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
 #pragma unroll
             for (int r = 0; r < kMoveUnroll; r++) {
-                const int64_t i = m0 + r * kMoveThreads + tid;
-                if (i < moves) w[to(int(i))] = x[r];
+                const int i = m0 + r * kMoveThreads + tid;
+                if (i < moves) w[to(i)] = x[r];
             }
         }
         __syncthreads();
@@ -427,7 +445,7 @@ __global__ __launch_bounds__(kMoveThreads, 2) void evict_shift_kernel(EvictArgs 
     const int per = (kMoveThreads >> a.ushift) * kMoveUnroll;
     if (a.filled && n - a.budget >= recent) {
         // the newest rows' places and sources do not meet: any order
-        for (int64_t m0 = holes + int64_t(block) * per; m0 < moves; m0 += int64_t(a.blocks) * per)
+        for (int m0 = holes + block * per; m0 < moves; m0 += a.blocks * per)
             move_rows<false>(a, pool, b, h, m0, min(moves, m0 + per), u0, from, to);
     } else if (block == 0) {
         move_rows<true>(a, pool, b, h, a.filled ? holes : 0, moves, u0, from, to);
@@ -509,7 +527,7 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
     for (a.b0 = 0; a.b0 < B; a.b0 += step) {
         const int nb = std::min(step, B - a.b0);
         const unsigned hk = unsigned(a.c.hk), nz = unsigned(nb);
-        iq::evict_plan_kernel<<<dim3(hk, nz), iq::kPlanThreads, 0, s>>>(a);
+        iq::evict_plan_kernel<16, 32><<<dim3(hk, nz), 1024, 0, s>>>(a);
         // (a cache that cannot hold more than the budget has nothing to move)
         if (a.t.cap <= budget) continue;
         // fewer than two workgroups a CU in an ordered move: spread over blocks of rows
