@@ -148,8 +148,8 @@ constexpr int kBins = 2048, kCopies = 4;
 // Order of the sums: NaN lowest, then by value (-0 as 0).
 __device__ __forceinline__ uint32_t sum_key(float w) {
     const uint32_t u = __float_as_uint(w + 0.0f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return 0;
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    const uint32_t k = u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
+    return w != w ? 0 : k;
 }
 
 // Exclusive prefix of v over the workgroup's W waves of threads and its total.
@@ -212,7 +212,12 @@ __global__ __launch_bounds__(64 * W) void evict_plan_kernel(EvictArgs a) {
 #pragma unroll
         for (int r = 0; r < HELD; r++) {
             if (r >= rounds) break;
-            k[r] = w0 + r * 64 + lane < old ? sum_key(x[r]) : 0;
+            k[r] = sum_key(x[r]);
+        }
+        if (w0 + rounds * 64 > old) {
+#pragma unroll
+            for (int r = 0; r < HELD; r++)
+                if (w0 + r * 64 + lane >= old) k[r] = 0;
         }
     };
     if (over && cut) hold(0);
@@ -316,33 +321,58 @@ __global__ __launch_bounds__(64 * W) void evict_plan_kernel(EvictArgs a) {
             eq_now += uint32_t(__popcll(same));
             return more | first;
         };
+        // a run that lies on one side of cut, with no ties: one ballot a round
+        const int run = w0 + rounds * 64;
+        const bool plain = !ties && run <= old && (run <= cut || w0 >= cut);
         // (a block has at most 32768 of either: two counts in a word)
         uint32_t count = 0, e = eq;
+        if (plain) {
 #pragma unroll
-        for (int r = 0; r < HELD; r++) {
-            if (r >= rounds) break;
-            const uint64_t stay = stays(r, e), low = lanes_below(w0 + r * 64, cut);
-            const uint64_t in = lanes_below(w0 + r * 64, old);
-            count += uint32_t(__popcll(low & in & ~stay)) + (uint32_t(__popcll(stay & ~low)) << 16);
+            for (int r = 0; r < HELD; r++) {
+                if (r >= rounds) break;
+                count += uint32_t(__popcll(__ballot(k[r] >= least)));
+            }
+            count = run <= cut ? uint32_t(rounds) * 64 - count : count << 16;
+        } else {
+#pragma unroll
+            for (int r = 0; r < HELD; r++) {
+                if (r >= rounds) break;
+                const uint64_t stay = stays(r, e), low = lanes_below(w0 + r * 64, cut);
+                const uint64_t in = lanes_below(w0 + r * 64, old);
+                count += uint32_t(__popcll(low & in & ~stay)) + (uint32_t(__popcll(stay & ~low)) << 16);
+            }
         }
         uint32_t at = block_excl_scan<W>(lane == 0 ? count : 0, &total, sh);
         at = uint32_t(__builtin_amdgcn_readfirstlane(int(at)));
         int32_t* hole = dst + holes + (at & 0xffffu);
         int32_t* high = src + highs + (at >> 16);
         e = eq;
+        if (plain) {
+            int32_t* list = run <= cut ? hole : high;
+            const bool holes_here = run <= cut;
 #pragma unroll
-        for (int r = 0; r < HELD; r++) {
-            if (r >= rounds) break;
-            const int i = w0 + r * 64;
-            const uint64_t stay = stays(r, e), low = lanes_below(i, cut);
-            const uint64_t to = low & lanes_below(i, old) & ~stay, from = stay & ~low;
-            if (to) {
-                if (to >> lane & 1) hole[lanes_before(to)] = i + lane;
-                hole += __popcll(to);
+            for (int r = 0; r < HELD; r++) {
+                if (r >= rounds) break;
+                const bool mine = (k[r] >= least) != holes_here;
+                const uint64_t m = __ballot(mine);
+                if (mine) list[lanes_before(m)] = w0 + r * 64 + lane;
+                list += __popcll(m);
             }
-            if (from) {
-                if (from >> lane & 1) high[lanes_before(from)] = i + lane;
-                high += __popcll(from);
+        } else {
+#pragma unroll
+            for (int r = 0; r < HELD; r++) {
+                if (r >= rounds) break;
+                const int i = w0 + r * 64;
+                const uint64_t stay = stays(r, e), low = lanes_below(i, cut);
+                const uint64_t to = low & lanes_below(i, old) & ~stay, from = stay & ~low;
+                if (to) {
+                    if (to >> lane & 1) hole[lanes_before(to)] = i + lane;
+                    hole += __popcll(to);
+                }
+                if (from) {
+                    if (from >> lane & 1) high[lanes_before(from)] = i + lane;
+                    high += __popcll(from);
+                }
             }
         }
         holes += total & 0xffffu;
@@ -391,16 +421,25 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b,
     }
 }
 
-// grid: x = (K, V) x slices x blocks of rows; y = head; z = sequence
+constexpr int kSumBlocks = 4;
+
+// grid: x = (K, V) x slices x blocks of rows, then kSumBlocks for the sums; y =
+// head; z = sequence
 __global__ __launch_bounds__(kMoveThreads, 4) void evict_fill_kernel(EvictArgs a) {
     const int h = blockIdx.y, b = a.b0 + int(blockIdx.z), row = int(blockIdx.z) * a.c.hk + h;
     const int holes = a.count[row];
-    const int block = int(blockIdx.x) / (2 * a.slices), sl = int(blockIdx.x) % (2 * a.slices);
     const int per = (kMoveThreads >> a.ushift) * kMoveUnroll;
-    const int m0 = block * per;
-    if (m0 >= holes) return;
     const int32_t* dst = a.dst + row * a.m;
     const int32_t* src = a.src + row * a.m;
+    const int sums = int(blockIdx.x) - 2 * a.slices * a.blocks;
+    if (sums >= 0) {
+        float* w = a.w + (int64_t(b) * a.c.hk + h) * a.wld;
+        for (int i = sums * kMoveThreads + int(threadIdx.x); i < holes; i += kSumBlocks * kMoveThreads) w[dst[i]] = w[src[i]];
+        return;
+    }
+    const int block = int(blockIdx.x) / (2 * a.slices), sl = int(blockIdx.x) % (2 * a.slices);
+    const int m0 = block * per;
+    if (m0 >= holes) return;
     char* pool = const_cast<char*>(sl < a.slices ? a.c.k : a.c.v);
     move_rows<false>(a, pool, b, h, m0, min(holes, m0 + per), (sl % a.slices) << a.ushift,
                      [&](int i) { return src[i]; }, [&](int i) { return dst[i]; });
@@ -420,7 +459,7 @@ __global__ __launch_bounds__(kMoveThreads, 4) void evict_shift_kernel(EvictArgs 
     const int moves = holes + recent;  // (at most the budget)
     if (int(blockIdx.x) == 2 * a.slices * a.blocks) {
         float* w = a.w + (int64_t(b) * a.c.hk + h) * a.wld;
-        for (int m0 = 0; m0 < moves; m0 += kMoveThreads * kMoveUnroll) {
+        for (int m0 = a.filled ? holes : 0; m0 < moves; m0 += kMoveThreads * kMoveUnroll) {
             float x[kMoveUnroll];
 #pragma unroll
             for (int r = 0; r < kMoveUnroll; r++) {
@@ -536,7 +575,7 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
         a.blocks = 1;
         if (a.filled) {
             a.blocks = int(std::min<int64_t>((m + per - 1) / per, 65536));
-            iq::evict_fill_kernel<<<dim3(2 * unsigned(a.slices * a.blocks), hk, nz), iq::kMoveThreads, 0, s>>>(a);
+            iq::evict_fill_kernel<<<dim3(2 * unsigned(a.slices * a.blocks) + iq::kSumBlocks, hk, nz), iq::kMoveThreads, 0, s>>>(a);
             a.blocks = int(std::min<int64_t>((recent + per - 1) / per, 64));
             a.blocks = std::max(a.blocks, 1);
         }
