@@ -71,9 +71,18 @@ __device__ bool find_item(const AttnArgs& a, uint32_t w, Item* it) {
     auto length = [&](int b) { return b < a.B ? a.t.lens[b] : 0; };
     auto tiles_of = [&](int n) { return n < 0 || n > a.t.cap ? 0u : attn_tiles(n); };
     int n = length(lane);
+    const int n0 = n;
     uint32_t total = lane_of(wave_scan(tiles_of(n)), 63);
     for (int b0 = 64; b0 < a.B; b0 += 64) total += lane_of(wave_scan(tiles_of(length(b0 + lane))), 63);
-    const uint32_t c = attn_chunk_tiles(total, a.nh, a.target);
+    const uint32_t least = attn_chunk_tiles(total, a.nh, a.target);
+    uint32_t c = least;
+    for (int i = 0; i < kAttnTries && uint32_t(a.B) * a.nh <= a.target; i++) {
+        uint32_t items = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64)
+            items += lane_of(wave_scan(b0 + lane < a.B ? attn_chunks(tiles_of(b0 ? length(b0 + lane) : n0), c) : 0), 63);
+        if (items * a.nh <= a.target) break;
+        c = attn_more_tiles(c, least);
+    }
     uint32_t before = 0, first = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         if (b0) n = length(b0 + lane);
@@ -212,6 +221,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     char* kl = lds[wave];
     char* vl = lds[wave] + KVB;
 
+    // The chain of loads that nothing shortens is length, page id, rows: q,
+    // needed last, is requested behind the first page ids and cut while the
+    // first rows come.
+    const int64_t off0 = row_offset(wave);
     // q: column = head, 8 values of each 32-value step a lane
     s16x8_t qt[KC][T::N];
     float mul = a.mul;
@@ -222,10 +235,16 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const int e = c * 32 + g * 8;
-            const bool in = col < gh && e < d;
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[c][i] = q[(e < d ? e : 0) + i];
+        }
+        if (wave < ntiles) load(off0);
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            const bool in = col < gh && c * 32 + g * 8 < d;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[c][i] = in ? q[e + i] : 0.0f;
+                x[c][i] = in ? x[c][i] : 0.0f;
                 big = fmaxf(big, fabsf(x[c][i]));
             }
         }
@@ -251,7 +270,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     float m = -INFINITY, l = 0.0f;
     float* sc = a.sc ? a.sc + ((int64_t(b) * a.c.hk + j) * a.t.cap) * a.group + h0 + col : nullptr;
 
-    if (wave < ntiles) load(row_offset(wave));
     int64_t off_next = wave + kAttnWaves < ntiles ? row_offset(wave + kAttnWaves) : 0;
     for (int tile = wave; tile < ntiles; tile += kAttnWaves) {
         const int tk = t0 + tile * kAttnTile;  // first token
@@ -384,71 +402,114 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     }
 }
 
-// One workgroup per (head, sequence): the chunks' sums, each times 2^(its
-// maximum - the largest), in chunk order within 256 / (d / 4 rounded to a
-// power of two) runs that are then added in order.
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+// Chunk i's maximum and sum of a head, of the sequence whose plan is pl.
+__device__ __forceinline__ float2 chunk_ml(const AttnArgs& a, uint2 pl, int head, uint32_t i) {
+    const int hg = head % a.group;
+    const int64_t slot = (int64_t(pl.y) + i) * a.nh + head / a.group * a.ht + hg / 16;
+    return reinterpret_cast<const float2*>(a.ml)[slot * 16 + hg % 16];
+}
+
+// One workgroup per (head, sequence): the chunks' rows, each times 2^(its
+// maximum - the largest so far), in chunk order within 256 / (d / 4 rounded
+// to a power of two) runs that are then added in order.
+__device__ __forceinline__ void join_head(const AttnArgs& a, int b, int head) {
     __shared__ float4_t xs[256];
-    __shared__ float ls[256];
-    const int b = blockIdx.y, head = blockIdx.x, d = a.c.d, tid = threadIdx.x;
-    if (a.t.lens[b] <= 0 || a.t.lens[b] > a.t.cap) return;
+    __shared__ float2 ms[256];
+    const int d = a.c.d, tid = threadIdx.x;
     const uint2 pl = a.plan[b];
     if (pl.x < 2) return;
     const int j = head / a.group, hg = head % a.group, hidx = j * a.ht + hg / 16, h = hg % 16;
-    const int64_t s0 = int64_t(pl.y) * a.nh + hidx;
-    auto ml = [&](int i) { return reinterpret_cast<const float2*>(a.ml)[(s0 + int64_t(i) * a.nh) * 16 + h]; };
-    const int n = int(pl.x);
-    float M = -INFINITY;
-    for (int i = tid & 63; i < n; i += 64) M = fmaxf(M, ml(i).x);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    const float* part = a.part + (int64_t(pl.y) * a.nh + hidx) * 16 * d + h * d;
     int w = 2;  // 16-byte pieces of a row, to a power of two
     while (w * 4 < d) w *= 2;
-    const int e = tid % w * 4, run = tid / w, runs = 256 / w;
-    float L = 0.0f;
+    const int e = tid % w * 4, run = tid / w, runs = 256 / w, n = int(pl.x);
+    float M = -INFINITY, L = 0.0f;
     float4_t x = {0, 0, 0, 0};
+    auto add = [&](float2 v, float4_t y) {
+        const float mn = fmaxf(M, v.x), f = __builtin_amdgcn_exp2f(M - mn), k = __builtin_amdgcn_exp2f(v.x - mn);
+        M = mn;
+        L = L * f + v.y * k;
+        x = x * f + y * k;
+    };
     if (e < d) {
-#pragma unroll 4
-        for (int i = run; i < n; i += runs) {
-            const float2 v = ml(i);
-            const float f = __builtin_amdgcn_exp2f(v.x - M);
-            L += v.y * f;
-            x += *reinterpret_cast<const float4_t*>(a.part + (s0 + int64_t(i) * a.nh) * 16 * d + h * d + e) * f;
+        int i = run;
+        for (; i + 3 * runs < n; i += 4 * runs) {
+            float2 v[4];
+            float4_t y[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                v[r] = chunk_ml(a, pl, head, uint32_t(i + r * runs));
+                y[r] = *reinterpret_cast<const float4_t*>(part + int64_t(i + r * runs) * a.nh * 16 * d + e);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) add(v[r], y[r]);
         }
+        for (; i < n; i += runs)
+            add(chunk_ml(a, pl, head, uint32_t(i)), *reinterpret_cast<const float4_t*>(part + int64_t(i) * a.nh * 16 * d + e));
     }
     xs[tid] = x;
-    ls[tid] = L;
+    ms[tid] = make_float2(M, L);
     __syncthreads();
     if (run == 0 && e < d) {
-        for (int r = 1; r < runs; r++) {
-            x += xs[r * w + tid];
-            L += ls[r * w + tid];
-        }
+        for (int r = 1; r < min(runs, n); r++) add(ms[r * w + tid], xs[r * w + tid]);
         const float inv = 1.0f / L;
         float* out = a.out + (int64_t(b) * a.hq + head) * d + e;
 #pragma unroll
         for (int r = 0; r < 4; r++) out[r] = x[r] * inv;
-        if (e == 0) {
-            float* f = a.fin + (int64_t(b) * a.hq + head) * 2;
-            f[0] = M;
-            f[1] = L;
-        }
     }
 }
 
-// weights[b][j][t] += sum over the group's heads, in order, of 2^(score -
-// maximum) / sum.
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) { join_head(a, blockIdx.y, blockIdx.x); }
+
+// The same with further workgroups that add the weights: for 256 tokens of a
+// key/value head, weights[b][j][t] += sum over the group's heads, in order,
+// of 2^(score - maximum) / sum.  The heads' maxima and sums over the chunks
+// are made here again, 16 heads x 16 runs of chunks at a time.
 __global__ __launch_bounds__(256) void attn_weights_kernel(AttnArgs a, float* weights, int64_t wld, float up) {
-    const int b = blockIdx.z, j = blockIdx.y, n = a.t.lens[b];
-    if (n > a.t.cap) return;
-    const int64_t row = int64_t(b) * a.c.hk + j;
-    for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < n; t += int64_t(gridDim.x) * 256) {
-        const float* s = a.sc + (row * a.t.cap + t) * a.group;
-        const float* f = a.fin + (int64_t(b) * a.hq + j * a.group) * 2;
-        float sum = 0.0f;
-        for (int h = 0; h < a.group; h++) sum += __builtin_amdgcn_exp2f(s[h] - (f[2 * h] - up)) / f[2 * h + 1];
-        weights[row * wld + t] += sum;
+    __shared__ float2 run_ml[16][17];
+    __shared__ float2 head_ml[16];  // maximum less `up`, 1 / sum
+    const int b = blockIdx.y, tid = threadIdx.x;
+    if (int(blockIdx.x) < a.hq) {
+        join_head(a, b, blockIdx.x);
+        return;
     }
+    const int n = a.t.lens[b];
+    const uint32_t w = blockIdx.x - uint32_t(a.hq);
+    const int j = int(w % uint32_t(a.c.hk)), t0 = int(w / uint32_t(a.c.hk)) * 256, t = t0 + tid;
+    if (n > a.t.cap || t0 >= n) return;
+    const uint2 pl = a.plan[b];
+    const int64_t row = int64_t(b) * a.c.hk + j;
+    const float* s = a.sc + (row * a.t.cap + min(t, n - 1)) * a.group;
+    float sum = 0.0f;
+    for (int h0 = 0; h0 < a.group; h0 += 16) {
+        const int gh = min(16, a.group - h0), h = tid & 15, run = tid >> 4;
+        float M = -INFINITY, L = 0.0f;
+        auto add = [&](float2 v) {
+            const float mn = fmaxf(M, v.x);
+            L = L * __builtin_amdgcn_exp2f(M - mn) + v.y * __builtin_amdgcn_exp2f(v.x - mn);
+            M = mn;
+        };
+        if (h < gh) {
+            if (pl.x < 2) {
+                if (run == 0) add(reinterpret_cast<const float2*>(a.fin)[int64_t(b) * a.hq + j * a.group + h0 + h]);
+            } else {
+                for (uint32_t i = uint32_t(run); i < pl.x; i += 16) add(chunk_ml(a, pl, j * a.group + h0 + h, i));
+            }
+        }
+        __syncthreads();
+        run_ml[h][run] = make_float2(M, L);
+        __syncthreads();
+        if (tid < gh) {
+            const int runs = pl.x < 2 ? 1 : int(min(pl.x, 16u));
+            M = run_ml[tid][0].x;
+            L = run_ml[tid][0].y;
+            for (int r = 1; r < runs; r++) add(run_ml[tid][r]);
+            head_ml[tid] = make_float2(M - up, 1.0f / L);
+        }
+        __syncthreads();
+        for (int i = 0; i < gh; i++) sum += __builtin_amdgcn_exp2f(s[h0 + i] - head_ml[i].x) * head_ml[i].y;
+    }
+    if (t < n) weights[row * wld + t] += sum;
 }
 
 template <int TYPE>
@@ -486,8 +547,11 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
     a.ht = (a.group + 15) / 16;
     a.nh = uint32_t(a.c.hk * a.ht);
     a.mul = scale * 1.44269504088896340736f;
-    // two workgroups a CU (what the LDS of d <= 128 holds)
-    a.target = uint32_t(2 * iq::device_cu_count());
+    // as many work items as run at once: 4, 3, 2 or 1 workgroups a CU by the
+    // registers (d <= 64) and the LDS of an instance.  Measured for d = 128 on
+    // 131072 tokens / 32 sequences of up to 8192: 1 a CU 64.7 / 29.2 us, 2 63.7
+    // / 26.7, 3 71.3 / 30.6, 4 70.1 / 31.1.
+    a.target = uint32_t((a.c.d <= 32 ? 4 : a.c.d <= 64 ? 3 : a.c.d <= 128 ? 2 : 1) * iq::device_cu_count());
     const int64_t capt = iq::attn_tiles(a.t.cap);
     // the workspace's partial sums: plan | final (maximum, sum) | chunks' | rows;
     // its GEMM operand area: the scores that the weights are made of
@@ -511,12 +575,12 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
         const int64_t grid = iq::attn_max_items(a.B, a.nh, a.t.cap, a.target);
         if (kv->type == IQ_KV_BF16) iq::launch_attn<IQ_KV_BF16>(a, unsigned(grid), s);
         else iq::launch_attn<IQ_KV_F16>(a, unsigned(grid), s);
-        if (capt > iq::kAttnWaves)  // (else no sequence has two chunks)
-            iq::attn_join_kernel<<<dim3(unsigned(q_heads), unsigned(a.B)), 256, 0, s>>>(a);
         if (weights) {
-            const int64_t blocks = std::min<int64_t>((a.t.cap + 255) / 256, 1024);
-            iq::attn_weights_kernel<<<dim3(unsigned(blocks), unsigned(a.c.hk), unsigned(a.B)), 256, 0, s>>>(
+            const int64_t blocks = q_heads + (a.t.cap + 255) / 256 * int64_t(a.c.hk);
+            iq::attn_weights_kernel<<<dim3(unsigned(blocks), unsigned(a.B)), 256, 0, s>>>(
                 a, weights + int64_t(b0) * a.c.hk * weights_ld, weights_ld, kv->type == IQ_KV_F16 ? 12.0f : 0.0f);
+        } else if (capt > iq::kAttnWaves) {  // (else no sequence has two chunks)
+            iq::attn_join_kernel<<<dim3(unsigned(q_heads), unsigned(a.B)), 256, 0, s>>>(a);
         }
     }
     return int(hipGetLastError());

@@ -4,11 +4,12 @@
 // on its own).
 //
 // Lengths are known on the device only.  Every sequence is cut into chunks
-// of the same number of 32-token tiles, C, chosen from the batch's total so
-// that all chunks of all key/value head tiles are about `target` work items:
-// a long sequence beside short ones gets as many workgroups as its share of
-// the tokens.  A sequence always has one chunk at least (an empty one's
-// writes its zeros).
+// of the same number of 32-token tiles, C: the least share of the batch's
+// total, or up to 7/4 of it, with which all chunks of all key/value head tiles
+// are at most `target` work items, so that a long sequence beside short ones
+// gets as many workgroups as its share of the tokens and all of them run at
+// once.  A sequence always has one chunk at least (an empty one's writes its
+// zeros), so many sequences may still be more than `target` items.
 #pragma once
 
 #include <algorithm>
@@ -42,12 +43,14 @@ constexpr int kAttnWaves = 4;   // waves of a workgroup: a chunk's tiles are dea
 
 IQ_HD uint32_t attn_tiles(int32_t len) { return (uint32_t(len) + kAttnTile - 1) / kAttnTile; }
 
-// Tiles of a chunk: `total` tiles of all sequences, `heads` head tiles each
-// (total * heads < 2^31), in whole rounds of the workgroup's waves.
+// Tiles of a chunk, `total` tiles of all sequences with `heads` head tiles
+// each (total * heads < 2^31): the least, and the next one to try.
+constexpr int kAttnTries = 6;
 IQ_HD uint32_t attn_chunk_tiles(uint32_t total, uint32_t heads, uint32_t target) {
     const uint32_t c = (total * heads + target - 1) / target;
-    return c <= kAttnWaves ? uint32_t(kAttnWaves) : (c + kAttnWaves - 1) / kAttnWaves * kAttnWaves;
+    return c < uint32_t(kAttnWaves) ? uint32_t(kAttnWaves) : c;
 }
+IQ_HD uint32_t attn_more_tiles(uint32_t c, uint32_t least) { return c + (least + 7) / 8; }
 
 IQ_HD uint32_t attn_chunks(uint32_t tiles, uint32_t c) { return tiles <= c ? 1 : (tiles + c - 1) / c; }
 

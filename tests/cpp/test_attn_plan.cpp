@@ -14,8 +14,15 @@ static long failures = 0;
 static void check_batch(const std::vector<int32_t>& lens, uint32_t heads, int64_t cap, uint32_t target) {
     uint32_t total = 0;
     for (const int32_t n : lens) total += iq::attn_tiles(n);
-    const uint32_t c = iq::attn_chunk_tiles(total, heads, target);
-    CHECK(c >= uint32_t(iq::kAttnWaves) && c % iq::kAttnWaves == 0);
+    const uint32_t least = iq::attn_chunk_tiles(total, heads, target);
+    uint32_t c = least;
+    for (int i = 0; i < iq::kAttnTries; i++) {
+        uint64_t all = 0;
+        for (const int32_t n : lens) all += iq::attn_chunks(iq::attn_tiles(n), c);
+        if (all * heads <= target) break;
+        c = iq::attn_more_tiles(c, least);
+    }
+    CHECK(c >= uint32_t(iq::kAttnWaves));
     int64_t items = 0, partials = 0;
     for (const int32_t n : lens) {
         const uint32_t tiles = iq::attn_tiles(n), k = iq::attn_chunks(tiles, c);
