@@ -35,7 +35,7 @@ struct LogprobArgs {
     float* tlp;
     uint32_t chunks, size;  // parts of a row, logits of a part (whole batches)
     float4* stat;           // [rows][chunks]: m, s, u
-    uint2* list;            // [rows][chunks][top]: key, id
+    uint64_t* list;         // [rows][chunks][top]
 };
 
 // Order of the logits: by value (-0 as 0), NaN largest.  0 is below every
@@ -79,62 +79,63 @@ struct Stat {
     }
 };
 
-// Whether (k, i) ranks before (l, j): key descending, id ascending.
-__device__ __forceinline__ bool before(uint32_t k, uint32_t i, uint32_t l, uint32_t j) {
-    return k > l || (k == l && i < j);
+// A logit's place in the ranking: key descending, then id ascending; 0: none.
+__device__ __forceinline__ uint64_t entry(uint32_t key, uint32_t id) { return uint64_t(key) << 32 | uint32_t(~id); }
+__device__ __forceinline__ uint64_t lane_of64(uint64_t v, int lane) {
+    return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32 |
+           uint32_t(__builtin_amdgcn_readlane(int(v), lane));
 }
 
-// The wave's largest logits by (key descending, id ascending), entry i in
-// lane i; key 0: none.
+// The wave's largest logits in order, entry i in lane i.
 struct List {
-    uint32_t key, id;    // this lane's entry
-    uint32_t last, lid;  // entry top - 1, uniform
-    __device__ __forceinline__ void clear() {
-        key = last = 0;
-        id = lid = 0xffffffffu;
-    }
+    uint64_t e;      // this lane's entry
+    uint64_t floor;  // an entry that `top` others of the row reach
+    uint64_t last;   // entry top - 1 or the floor: what a candidate has to pass; uniform
+    __device__ __forceinline__ void clear() { e = floor = last = 0; }
     __device__ __forceinline__ void find_last(int top) {
-        last = uint32_t(__builtin_amdgcn_readlane(int(key), top - 1));
-        lid = uint32_t(__builtin_amdgcn_readlane(int(id), top - 1));
+        const uint64_t l = lane_of64(e, top - 1);
+        last = l > floor ? l : floor;
     }
-    // The lanes' candidates (k, i), one after the other; k == 0: none.
-    __device__ __forceinline__ void add(uint32_t k, uint32_t i, int top) {
+    __device__ __forceinline__ uint32_t last_key() const { return uint32_t(last >> 32); }
+    // The lanes' candidates, one after the other (0: none).
+    __device__ __forceinline__ void add(uint64_t c, int top) {
         const int lane = threadIdx.x & 63;
-        uint64_t more = __ballot(k != 0 && before(k, i, last, lid));
+        uint64_t more = __ballot(c > last);
         while (more) {
-            const int from = __builtin_ctzll(more);
-            const uint32_t nk = uint32_t(__builtin_amdgcn_readlane(int(k), from));
-            const uint32_t ni = uint32_t(__builtin_amdgcn_readlane(int(i), from));
+            const uint64_t n = lane_of64(c, __builtin_ctzll(more));
             // entries before the new one stay, the others move up a lane
-            const uint32_t pk = uint32_t(__builtin_amdgcn_update_dpp(0, int(key), 0x138, 0xf, 0xf, false));  // wave_shr:1
-            const uint32_t pi = uint32_t(__builtin_amdgcn_update_dpp(0, int(id), 0x138, 0xf, 0xf, false));
-            const int at = __builtin_popcountll(__ballot(before(key, id, nk, ni)));
-            key = lane < at ? key : (lane == at ? nk : pk);
-            id = lane < at ? id : (lane == at ? ni : pi);
+            const uint32_t ph = uint32_t(__builtin_amdgcn_update_dpp(0, int(e >> 32), 0x138, 0xf, 0xf, false));  // wave_shr:1
+            const uint32_t pl = uint32_t(__builtin_amdgcn_update_dpp(0, int(e), 0x138, 0xf, 0xf, false));
+            const int at = __builtin_popcountll(__ballot(e > n));
+            e = lane < at ? e : (lane == at ? n : uint64_t(ph) << 32 | pl);
             find_last(top);
             more &= more - 1;
-            more &= __ballot(before(k, i, last, lid));
+            more &= __ballot(c > last);
         }
     }
-    // The first batch, 16 candidates a lane, into the empty list.  Inserting
-    // them one by one would take some 5 top steps; instead a bound that at
-    // least `top` of them reach is found by bisection, first over the lanes'
-    // largest (counted by one ballot a step), then, while more than a wave's
-    // lanes reach it, over all; those that do go to a lane each (through
-    // `room`, the wave's own 64 places in LDS) and to the place that the
-    // number of greater ones says.
+    // A wave's first batch, 16 candidates a lane, into the empty list (where
+    // first_batch below cannot): a bound that at least `top` of them reach is
+    // found by bisection, first over the lanes' largest (counted by one
+    // ballot a step, until no more than 24 lanes reach it), then, while more
+    // than a wave's lanes do, over all; those that do go to a lane each
+    // (through `room`, the wave's own 64 places in LDS) and from there to the
+    // place that the number of greater ones says.
     template <class Id>
-    __device__ __forceinline__ void fill(const uint32_t (&k)[16], Id id_of, int top, uint2* room) {
+    __device__ __forceinline__ void fill(const uint32_t (&k)[16], Id id_of, int top, uint64_t* room) {
         const int lane = threadIdx.x & 63;
+        room[lane] = 0;
         uint32_t lm = k[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) lm = max(lm, k[i]);
         uint32_t lo = 0;
+        const int few = max(top, 24);
         for (int bit = 31; bit >= 0; bit--) {
             const uint32_t to = lo | (1u << bit);
             const int n = __builtin_popcountll(__ballot(lm >= to));
-            if (n >= top) lo = to;
-            if (n == top) break;
+            if (n >= top) {
+                lo = to;
+                if (n <= few) break;
+            }
         }
         lo = max(lo, 1u);
         auto count = [&](uint32_t to) {
@@ -157,92 +158,186 @@ struct List {
         }
         if (c > 64) {  // (many equal ones)
 #pragma unroll
-            for (int i = 0; i < 16; i++) add(k[i] >= lo ? k[i] : 0, id_of(i), top);
+            for (int i = 0; i < 16; i++) add(k[i] >= lo ? entry(k[i], id_of(i)) : 0, top);
             return;
         }
-        const uint64_t below = lane ? (~uint64_t(0) >> (64 - lane)) : 0;
         int at = 0;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const uint64_t in = __ballot(k[i] >= lo);
-            if (k[i] >= lo) room[at + __builtin_popcountll(in & below)] = make_uint2(k[i], id_of(i));
+            if (k[i] >= lo)
+                room[at + __builtin_amdgcn_mbcnt_hi(uint32_t(in >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(in), 0))] =
+                    entry(k[i], id_of(i));
             at += __builtin_popcountll(in);
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
-        uint2 e = make_uint2(0, 0xffffffffu);
-        if (lane < c) e = room[lane];
+        const uint64_t mine = room[lane];
         int rank = 0;
-        for (int i = 0; i < c; i++)
-            rank += before(uint32_t(__builtin_amdgcn_readlane(int(e.x), i)), uint32_t(__builtin_amdgcn_readlane(int(e.y), i)), e.x, e.y);
-        if (lane >= c) rank = lane;
-        key = uint32_t(__builtin_amdgcn_ds_permute(rank * 4, int(e.x)));
-        id = uint32_t(__builtin_amdgcn_ds_permute(rank * 4, int(e.y)));
+        for (int i = 0; i < c; i += 8)
+#pragma unroll
+            for (int r = 0; r < 8; r++) rank += room[i + r] > mine;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        if (lane < c) room[rank] = mine;  // (the places from c on stay 0)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        e = room[lane];
         find_last(top);
     }
-    // Up to 16 candidates a lane into the list; `nan`: some may be NaN.
+    // Up to 16 candidates a lane into the list, `most` their largest key;
+    // `nan`: some may be NaN, which does not show in it.
     template <class Key, class Id>
-    __device__ __forceinline__ void batch(Key key_of, Id id_of, uint32_t most, bool nan, int top, uint2* room) {
-        if (!__any(most >= last || nan)) return;
+    __device__ __forceinline__ void batch(Key key_of, Id id_of, uint32_t most, bool nan, int top, uint64_t* room) {
+        if (!__any(most >= last_key() || nan)) return;
         uint32_t k[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) k[i] = key_of(i);
-        if (last == 0 && lane_key0() == 0) {
+        if (last == 0 && lane_of64(e, 0) == 0) {
             fill(k, id_of, top, room);
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; i++) add(k[i], id_of(i), top);
+            for (int i = 0; i < 16; i++) add(k[i] ? entry(k[i], id_of(i)) : 0, top);
         }
     }
-    __device__ __forceinline__ uint32_t lane_key0() const { return uint32_t(__builtin_amdgcn_readfirstlane(int(key))); }
 };
 
+// Maximum and sum over a wave's lanes, in every lane (DPP: row_shr 1, 2, 4,
+// 8, then the rows' last lanes into the next rows; lane 63 has the result).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float from_lane(float v, float none) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+template <class Op>
+__device__ __forceinline__ float wave_reduce(float v, float none, Op op) {
+    v = op(v, from_lane<0x111, 0xf>(v, none));
+    v = op(v, from_lane<0x112, 0xf>(v, none));
+    v = op(v, from_lane<0x114, 0xf>(v, none));
+    v = op(v, from_lane<0x118, 0xf>(v, none));
+    v = op(v, from_lane<0x142, 0xa>(v, none));
+    v = op(v, from_lane<0x143, 0xc>(v, none));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
 __device__ __forceinline__ Stat wave_join(Stat st) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        Stat p;
-        p.m = __shfl_xor(st.m, o);
-        p.s = __shfl_xor(st.s, o);
-        p.u = __shfl_xor(st.u, o);
-        st.join(p);
-    }
+    st.raise(wave_reduce(st.m, -FLT_MAX, [](float x, float y) { return fmaxf(x, y); }));
+    st.s = wave_reduce(st.s, 0.0f, [](float x, float y) { return x + y; });
+    st.u = wave_reduce(st.u, 0.0f, [](float x, float y) { return x + y; });
     return st;
 }
 
-// Shared memory of a workgroup: a wave's room, then its list.
+// Shared memory of a workgroup: first_batch's, then a wave's room, then its list.
 struct Shared {
     Stat st[kWaves];
-    uint2 room[kWaves][kMaxTop];
-    uint2 out[kMaxTop];
+    uint32_t most[64 * kWaves];  // the lanes' largest keys
+    uint64_t room[kWaves][kMaxTop];
+    uint64_t out[kMaxTop];
+    uint32_t nan[kWaves];
+    uint32_t lo, count;
 };
+
+// The workgroup's first batch, 16 candidates a lane of all its waves.
+// Inserting them one by one would take some 5 top steps a wave (32 rows of
+// 152064, top 20: 53 us a launch; a bound and a sorted list for every wave,
+// 15).  Instead wave 0 bisects for a bound that `top` of the 256 lanes'
+// largest keys reach (at most 24, if top allows), the few candidates that
+// reach it (`reach(i, bound)`) are collected in LDS, and each goes to the
+// place that the number of greater ones says: wave 0's list, and the floor of
+// the other waves'.  False, with nothing changed, where more than 256 reach
+// it (many equal ones, or a large `top`) or there may be NaN: the waves then
+// fill lists of their own.
+template <class Reach, class Entry>
+__device__ __forceinline__ bool first_batch(List& li, uint32_t most, bool nan, int top, Shared& sh, Reach reach,
+                                            Entry entry_of) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint64_t* found = &sh.room[0][0];
+    sh.most[tid] = most;
+    found[tid] = 0;
+    if (wave == 0) sh.out[lane] = 0;
+    const bool any = __any(nan);
+    if (lane == 0) sh.nan[wave] = any;
+    __syncthreads();
+    if (wave == 0) {
+        uint32_t k[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) k[w] = sh.most[w * 64 + lane];
+        uint32_t lo = 0;
+        const int few = max(top, 24);
+        for (int bit = 31; bit >= 0; bit--) {
+            const uint32_t to = lo | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) n += __builtin_popcountll(__ballot(k[w] >= to));
+            if (n >= top) {
+                lo = to;
+                if (n <= few) break;
+            }
+        }
+        if (lane == 0) {
+            sh.lo = max(lo, 1u);
+            sh.count = 0;
+        }
+    }
+    __syncthreads();
+    const uint32_t lo = sh.lo;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        if (reach(i, lo)) {
+            const uint32_t at = atomicAdd(&sh.count, 1u);
+            if (at < 64 * kWaves) found[at] = entry_of(i);
+        }
+    }
+    __syncthreads();
+    const int c = int(sh.count);
+    if (c > 64 * kWaves || sh.nan[0] | sh.nan[1] | sh.nan[2] | sh.nan[3]) {
+        __syncthreads();  // (the rooms become the waves' own)
+        return false;
+    }
+    const uint64_t mine = found[tid];
+    if (tid < c) {
+        int rank = 0;
+        for (int i = 0; i < c; i += 8)
+#pragma unroll
+            for (int r = 0; r < 8; r++) rank += found[i + r] > mine;
+        if (rank < kMaxTop) sh.out[rank] = mine;
+    }
+    __syncthreads();
+    if (wave == 0) li.e = sh.out[lane];
+    li.floor = sh.out[top - 1];
+    li.find_last(top);
+    __syncthreads();
+    return true;
+}
+static_assert(kWaves == 4, "first_batch ors four flags");
 
 // The workgroup's waves joined, in wave order; the list is wave 0's.  Of the
 // waves' sorted lists an entry's place is its own index and the number of
-// entries of the other lists that rank before it.
+// entries of the other lists that rank before it.  `done`: it is wave 0's already.
 template <bool TOP>
-__device__ __forceinline__ void block_join(Stat& st, List& li, int top, Shared& sh) {
+__device__ __forceinline__ void block_join(Stat& st, List& li, int top, Shared& sh, bool done) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     st = wave_join(st);
     if (lane == 0) sh.st[wave] = st;
-    if (TOP) {
-        sh.room[wave][lane] = make_uint2(li.key, li.id);
-        if (wave == 0) sh.out[lane] = make_uint2(0, 0xffffffffu);
+    if (TOP && !done) {
+        sh.room[wave][lane] = lane < top ? li.e : 0;
+        if (wave == 0) sh.out[lane] = 0;
     }
     __syncthreads();
     st = sh.st[0];
 #pragma unroll
     for (int w = 1; w < kWaves; w++) st.join(sh.st[w]);
-    if (TOP) {
+    if (TOP && !done) {
         int at = lane;
+        const uint64_t mine = li.e;
 #pragma unroll
         for (int o = 1; o < kWaves; o++) {
-            const uint2* l = sh.room[(wave + o) % kWaves];
-            for (int i = 0; i < top; i++) at += before(l[i].x, l[i].y, li.key, li.id);
+            const uint64_t* l = sh.room[(wave + o) % kWaves];
+            for (int i = 0; i < top; i += 4)
+#pragma unroll
+                for (int r = 0; r < 4; r++) at += l[i + r] > mine;
         }
-        if (lane < top && at < top && li.key) sh.out[at] = make_uint2(li.key, li.id);
+        if (lane < top && at < top && mine) sh.out[at] = mine;
         __syncthreads();
-        li.key = sh.out[lane].x;
-        li.id = sh.out[lane].y;
+        li.e = sh.out[lane];
     }
 }
 
@@ -261,13 +356,16 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int64_t t, const St
         if (a.ent) a.ent[t] = lz - st.u / st.s;
     }
     if (TOP && lane < a.top) {
-        a.ids[t * a.top + lane] = li.id;
-        a.tlp[t * a.top + lane] = (key_logit(li.key) - st.m) - lz;
+        a.ids[t * a.top + lane] = uint32_t(~li.e);
+        a.tlp[t * a.top + lane] = (key_logit(uint32_t(li.e >> 32)) - st.m) - lz;
     }
 }
 
+// Workgroups a CU that a call is split into (and that its registers allow for).
+constexpr int kPerCu = 4, kPerCuTop = 5;
+
 template <bool TOP>
-__global__ __launch_bounds__(64 * kWaves) void logprob_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 5) void logprob_kernel(LogprobArgs a) {
     __shared__ Shared sh;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t t = blockIdx.x / a.chunks;
@@ -278,10 +376,11 @@ __global__ __launch_bounds__(64 * kWaves) void logprob_kernel(LogprobArgs a) {
     List li;
     st.clear();
     li.clear();
-    for (uint32_t b = chunk * a.size + wave * kBatch; b < end; b += kWaves * kBatch) {
-        float v[16];
-        const bool whole = b + kBatch <= end;
-        if (whole) {
+    const uint32_t b0 = chunk * a.size;
+    bool done = false;
+    for (uint32_t b = b0 + wave * kBatch; b < end || b < b0 + kWaves * kBatch; b += kWaves * kBatch) {
+        float v[16];  // past the end: -inf
+        if (b + kBatch <= end) {
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -306,19 +405,32 @@ __global__ __launch_bounds__(64 * kWaves) void logprob_kernel(LogprobArgs a) {
             st.u = fmaf(e, fmaxf(d, -200.0f), st.u);
         }
         if constexpr (TOP) {
-            // (a NaN does not show in the maximum, but in the sum)
+            // (a NaN shows in the sum)
             auto id_of = [&](int i) { return b + i / 4 * 256 + lane * 4 + i % 4; };
+            if (b < b0 + kWaves * kBatch) {
+                // (the bound as a logit: keys up to -inf's are all logits)
+                done = first_batch(
+                    li, b + lane * 4 < end ? logit_key(mx) : 0, !(st.s >= 0.0f), a.top, sh,
+                    [&](int i, uint32_t lo) {
+                        return v[i] >= (lo <= 0x007fffffu ? -INFINITY : key_logit(lo)) && id_of(i) < end;
+                    },
+                    [&](int i) { return entry(logit_key(v[i]), id_of(i)); });
+                if (done) continue;
+            } else {
+                done = false;
+            }
             li.batch([&](int i) { return id_of(i) < end ? logit_key(v[i]) : 0u; }, id_of, logit_key(mx), !(st.s >= 0.0f),
                      a.top, sh.room[wave]);
         }
     }
-    block_join<TOP>(st, li, a.top, sh);
+    done = done && end - b0 <= kWaves * kBatch;
+    block_join<TOP>(st, li, a.top, sh, done);
     if (a.chunks == 1) {
         finish<TOP>(a, t, st, li);
         return;
     }
     if (threadIdx.x == 0) a.stat[blockIdx.x] = make_float4(st.m, st.s, st.u, 0.0f);
-    if (TOP && wave == 0 && lane < a.top) a.list[int64_t(blockIdx.x) * a.top + lane] = make_uint2(li.key, li.id);
+    if (TOP && wave == 0 && lane < a.top) a.list[int64_t(blockIdx.x) * a.top + lane] = li.e;
 }
 
 template <bool TOP>
@@ -334,22 +446,29 @@ __global__ __launch_bounds__(64 * kWaves) void logprob_join_kernel(LogprobArgs a
         const float4 f = a.stat[t * a.chunks + c];
         st.join(Stat{f.x, f.y, f.z});
     }
+    bool done = false;
     if constexpr (TOP) {
         const uint32_t n = a.chunks * a.top;
-        const uint2* l = a.list + t * n;
-        for (uint32_t b = wave * kBatch; b < n; b += kWaves * kBatch) {
-            uint2 e[16];
+        const uint64_t* l = a.list + t * n;
+        for (uint32_t b = wave * kBatch; b < n || b < kWaves * kBatch; b += kWaves * kBatch) {
+            uint64_t e[16];
             uint32_t most = 0;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const uint32_t at = b + i * 64 + lane;
-                e[i] = at < n ? l[at] : make_uint2(0, 0);
-                most = max(most, e[i].x);
+                e[i] = at < n ? l[at] : 0;
+                most = max(most, uint32_t(e[i] >> 32));
             }
-            li.batch([&](int i) { return e[i].x; }, [&](int i) { return e[i].y; }, most, false, a.top, sh.room[wave]);
+            if (b < kWaves * kBatch) {
+                done = first_batch(li, most, false, a.top, sh,
+                                   [&](int i, uint32_t lo) { return uint32_t(e[i] >> 32) >= lo; }, [&](int i) { return e[i]; });
+                if (done) continue;
+            }
+            li.batch([&](int i) { return uint32_t(e[i] >> 32); }, [&](int i) { return uint32_t(~e[i]); }, most, false, a.top,
+                     sh.room[wave]);
         }
     }
-    block_join<TOP>(st, li, a.top, sh);
+    block_join<TOP>(st, li, a.top, sh, done && a.chunks * a.top <= kWaves * kBatch);
     finish<TOP>(a, t, st, li);
 }
 
@@ -365,11 +484,16 @@ int iq_logprobs(const float* logits, int64_t ld, int64_t T, int64_t V, const int
     if (!logprob && !entropy && !top) return IQ_ENULL;
     if (V > 0x7fffffff - 65536 || T > 0x7fffffff) return IQ_ETOOLARGE;
     iq::LogprobArgs a{logits, ld, uint32_t(V), tokens, top, logprob, entropy, top_ids, top_logprobs};
-    // about eight workgroups a CU, parts of four batches at least
+    // workgroups for every CU, parts of four batches at least (32 rows of 152064,
+    // top 20, in 8 / 19 / 38 / 75 parts: 26.5 / 21.5 / 20.3 / 27.2 us; 999 rows,
+    // no list, in 1 / 2 / 4: 139.8 / 143.5 / 145.3)
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t target = 8 * int64_t(iq::device_cu_count());
-    int64_t chunks = std::max<int64_t>(1, std::min((target + T - 1) / T, (V + 4095) / 4096));
-    const int64_t size = ((V + chunks - 1) / chunks + iq::kBatch - 1) / iq::kBatch * iq::kBatch;
+    const int64_t target = (top ? iq::kPerCuTop : iq::kPerCu) * int64_t(iq::device_cu_count());
+    int64_t chunks = std::max<int64_t>(1, std::min(target / T, (V + 4095) / 4096));
+    // whole steps of a workgroup where they are few, of a wave where many
+    int64_t size = (V + chunks - 1) / chunks;
+    const int64_t whole = size > 16 * iq::kBatch ? iq::kBatch : iq::kWaves * iq::kBatch;
+    size = (size + whole - 1) / whole * whole;
     chunks = (V + size - 1) / size;
     a.chunks = uint32_t(chunks);
     a.size = uint32_t(size);
@@ -379,7 +503,7 @@ int iq_logprobs(const float* logits, int64_t ld, int64_t T, int64_t V, const int
         if (e != hipSuccess) return e == hipErrorOutOfMemory ? IQ_ENOMEM : int(e);
         if (T * chunks * (4 + 2 * int64_t(top)) > ws->part_floats) return IQ_ETOOLARGE;
         a.stat = reinterpret_cast<float4*>(ws->partials);
-        a.list = reinterpret_cast<uint2*>(ws->partials + T * chunks * 4);
+        a.list = reinterpret_cast<uint64_t*>(ws->partials + T * chunks * 4);
     }
     const unsigned grid = unsigned(T * chunks);
     if (top) iq::logprob_kernel<true><<<grid, 64 * iq::kWaves, 0, s>>>(a);
