@@ -168,3 +168,108 @@ class DecodeStep:
         for Lw in self.model["layers"]:
             n += sum(Lw[k].nbytes() for k in ("q", "k", "v", "o", "gate", "up", "down"))
         return n + self.model["head"].nbytes()
+
+
+class CachedDecodeStep:
+    """One decode step of B sequences over paged key/value caches, one
+    ops.KvCache a layer: every sequence's next token, at the position and
+    cache length that `positions` and `lens` hold, through all layers to
+    logits.  `model` as for DecodeStep, with cfg["theta"] (rotary base).
+
+    table: int32 [B, pages], the pages of every sequence (the same ids in all
+    layers); enough of them have to be there before the step that fills them.
+    weights: keep the attention weight every cached token has received, per
+    layer [B, kv_heads, pages * page_size], for evict().
+
+    Device state, which the caller may set between steps: lens (int32 [B],
+    tokens in the cache), positions (int64 [B], of the next token; they part
+    from lens after an eviction).  step() issues only device work, so it can
+    be captured into a graph (after ops.init on the capturing stream)."""
+
+    def __init__(self, model, caches, table, weights=False, device="cuda"):
+        c = model["cfg"]
+        H, I, V = c["hidden"], c["inter"], c["vocab"]
+        nh, nkv, hd, L = c["heads"], c["kv_heads"], c["head_dim"], c["layers"]
+        if len(caches) != L or any((k.kv_heads, k.head_dim) != (nkv, hd) for k in caches):
+            raise ValueError("CachedDecodeStep: one cache a layer, of the model's key/value heads and head size")
+        if len({k.page_size for k in caches}) != 1:
+            raise ValueError("CachedDecodeStep: caches of one page size")
+        B = self.rows = table.shape[0]
+        self.model, self.caches, self.table = model, list(caches), table
+        self.page = caches[0].page_size
+        self.capacity = table.shape[1] * self.page
+        qo, kvo = nh * hd, nkv * hd
+        sizes = [H] + [qo, kvo, kvo, qo, qo, H, I, H] * L + [V]
+        self.arena = Arena([B * n for n in sizes], device)
+        vs = iter(self.arena.views)
+        self.h0 = next(vs)
+        self.ids = torch.zeros(B, dtype=torch.int64, device=device)
+        self.lens = torch.zeros(B, dtype=torch.int32, device=device)
+        self.positions = torch.zeros(B, dtype=torch.int64, device=device)
+        self.slots = torch.full((B,), -1, dtype=torch.int64, device=device)
+        self.freqs = ops.rope_freqs(hd, c["theta"], device)
+        self.weights = [torch.zeros(B, nkv, self.capacity, device=device) for _ in range(L)] if weights else None
+        self._new_lens = torch.zeros(B, dtype=torch.int32, device=device)
+        self.per_layer, self.chains = [], []
+        h, stages = self.h0, []
+        for li in range(L):
+            Lw = model["layers"][li]
+            q, k, v, q_rot, attn, h1, act, h2 = (next(vs) for _ in range(8))
+            stages.append(Stage([Lw["q"], Lw["k"], Lw["v"]], h, [q, k, v], IN_RMSNORM, OUT_STORE,
+                                biases=[Lw.get("q_b"), Lw.get("k_b"), Lw.get("v_b")], norm=Lw["input_ln"],
+                                eps=c["eps"], rows=B))
+            self.chains.append(Chain(stages))
+            stages = [Stage([Lw["o"]], attn, [h1], IN_PLAIN, OUT_RESIDUAL, residual=h, rows=B),
+                      Stage([Lw["gate"], Lw["up"]], h1, [act], IN_RMSNORM, OUT_SWIGLU, norm=Lw["post_ln"],
+                            eps=c["eps"], rows=B),
+                      Stage([Lw["down"]], act, [h2], IN_PLAIN, OUT_RESIDUAL, residual=h1, rows=B)]
+            self.per_layer.append(dict(h=h, q=q, k=k, v=v, q_rot=q_rot, attn=attn, h1=h1, act=act, h2=h2))
+            h = h2
+        self.logits = next(vs).view(B, V)
+        stages.append(Stage([model["head"]], h, [self.logits], IN_RMSNORM, OUT_STORE, norm=model["final_norm"],
+                            eps=c["eps"], rows=B))
+        self.chains.append(Chain(stages))
+        self.h_last = h
+
+    def step(self, token_id=None, stream=None):
+        """The tokens `token_id` (an int for every row, or a sequence of B ints;
+        None: the ids already in self.ids) are added to the caches, attend to
+        them and leave their logits; lens and positions move on by one.  A
+        sequence whose pages are full, or whose next page id is negative, keeps
+        its cache; a full one's logits are NaN."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.step(token_id)
+        if token_id is not None:
+            if isinstance(token_id, int):
+                self.ids.fill_(int(token_id))
+            else:
+                self.ids.copy_(torch.tensor([int(t) for t in token_id], dtype=torch.int64))
+        at = self.lens.clamp(max=self.capacity - 1)
+        page = self.table.gather(1, (at // self.page).long()[:, None])[:, 0]
+        slot = page.long() * self.page + at % self.page
+        self.slots.copy_(torch.where((self.lens < self.capacity) & (page >= 0), slot, torch.full_like(slot, -1)))
+        self.lens.add_(1)
+        ops.launch_embedding_q(self.model["embed"], self.ids, self.rows, self.model["cfg"]["hidden"], self.h0)
+        self.chains[0].run()
+        for li, b in enumerate(self.per_layer):
+            ops.kv_append(b["q"], b["k"], b["v"], self.positions, self.slots, self.freqs, self.caches[li],
+                          q_out=b["q_rot"])
+            ops.attn_decode(b["q_rot"], self.caches[li], self.table, self.lens, out=b["attn"],
+                            weights=self.weights[li] if self.weights else None)
+            self.chains[li + 1].run()
+        self.positions.add_(1)
+
+    def evict(self, budget, recent):
+        """Every layer's caches cut to `budget` tokens a sequence by the weights
+        they have received (ops.kv_evict); the pages past them are free."""
+        if not self.weights:
+            raise ValueError("CachedDecodeStep.evict: made without weights")
+        for cache, w in zip(self.caches, self.weights):
+            ops.kv_evict(cache, self.table, self.lens, w, budget, recent, new_lens=self._new_lens)
+        self.lens.copy_(self._new_lens)
+
+    def logprobs(self, tokens=None, top=0, out=None):
+        """Log probabilities, entropy and top alternatives of the last step's
+        logits (ops.logprobs)."""
+        return ops.logprobs(self.logits, tokens, top, out)
