@@ -113,10 +113,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 // would move everything behind the first evicted one.
 //
 // evict_plan_kernel (one workgroup per sequence and head) holds up to 32768
-// sums in registers (longer rows are read again), finds the cut-th largest by
-// three histogram passes over its bits (11 + 11 + 10, highest first; four
-// copies of a histogram, since most sums share few exponents) and writes the
-// lists of free places and of the rows that fill them.
+// sums in LDS (longer rows are read again), finds the cut-th largest by
+// histograms of its bits (12 + 12 + 8, highest first; few share the upper 24,
+// and are ranked by counting) and writes the lists of free places and of the
+// rows that fill them.
 //
 // The rows are moved by two kernels.  The free places lie below cut and every
 // source at or above it, so evict_fill_kernel moves those rows in any order.
@@ -143,7 +143,9 @@ struct EvictArgs {
     int filled;            // the free places are filled by an earlier launch
 };
 
-constexpr int kBins = 2048, kCopies = 4;
+constexpr int kPlanWaves = 16, kPlanThreads = 64 * kPlanWaves;
+constexpr int kBinBits = 12, kBins = 1 << kBinBits, kFew = 64;
+constexpr int kHeldSums = 32768;  // keys that a workgroup holds (128 KiB of LDS)
 
 // Order of the sums: NaN lowest, then by value (-0 as 0).
 __device__ __forceinline__ uint32_t sum_key(float w) {
@@ -181,51 +183,47 @@ __device__ __forceinline__ uint32_t lanes_before(uint64_t mask) {
     return __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
 }
 
-// A wave holds a run of up to HELD x 64 sums in slot order, 64 in a round, so
-// that ranks are a scan over the waves and counts of ballots, which the scalar
-// unit makes (the places below cut and past the end are masks of it too).
-template <int W, int HELD>
-__global__ __launch_bounds__(64 * W) void evict_plan_kernel(EvictArgs a) {
-    constexpr int TH = 64 * W, BLOCK = TH * HELD, PER = kBins / TH;
-    __shared__ __align__(16) uint32_t hist[kCopies][kBins + 16];  // (the copies on different banks)
-    __shared__ uint32_t sh[W];
-    __shared__ uint32_t found[3];
+// The keys lie in LDS.  A wave goes through a run of them in slot order, 64 in
+// a round, so that ranks are a scan over the waves and counts of ballots.  The
+// loops are kept short on purpose: with the keys in
+// registers they have to be unrolled, and instructions that are executed once
+// cost more to fetch than they take (32768 sums: 28 us with 32 keys a lane, 22.5
+// so; 2112 sums: 8.8 and 7.8).
+__global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(EvictArgs a) {
+    extern __shared__ __align__(16) uint32_t lds[];
+    uint32_t* hist = lds;
+    uint32_t* keys = lds + kBins;
+    __shared__ uint64_t cand[kFew];
+    __shared__ uint32_t sh[kPlanWaves];
+    __shared__ uint32_t found[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x, b = a.b0 + int(blockIdx.y), row = int(blockIdx.y) * a.c.hk + h;
     const int n = a.t.lens[b];
     const bool fits = n >= 0 && n <= a.t.cap, over = fits && n > a.budget;
     const int old = n - int(a.recent), cut = int(a.budget - a.recent);
     const float* w = a.w + (int64_t(b) * a.c.hk + h) * a.wld;
-    // this block of sums: rounds of a wave, its first slot; keys of places
-    // past the end are 0
-    uint32_t k[HELD];
+    // this block of sums from slot i0 on: rounds of a wave, its first slot
     int rounds = 0, w0 = 0;
+    const uint32_t* own = nullptr;  // its keys
     auto hold = [&](int i0) {
-        rounds = (min(old - i0, BLOCK) + TH - 1) / TH;
+        const int count = min(old - i0, kHeldSums);
+        rounds = (count + kPlanThreads - 1) / kPlanThreads;
         w0 = i0 + wave * rounds * 64;
-        float x[HELD];
-#pragma unroll
-        for (int r = 0; r < HELD; r++) {
-            if (r >= rounds) break;
-            x[r] = w[min(w0 + r * 64 + lane, old - 1)];
+        own = keys + wave * rounds * 64 + lane;
+        __syncthreads();  // (the block before is done with)
+#pragma unroll 8
+        for (int r = 0; r < rounds; r++) {
+            const int i = r * kPlanThreads + tid;
+            keys[i] = sum_key(w[i0 + min(i, count - 1)]);  // (past the end: not counted)
         }
-#pragma unroll
-        for (int r = 0; r < HELD; r++) {
-            if (r >= rounds) break;
-            k[r] = sum_key(x[r]);
-        }
-        if (w0 + rounds * 64 > old) {
-#pragma unroll
-            for (int r = 0; r < HELD; r++)
-                if (w0 + r * 64 + lane >= old) k[r] = 0;
-        }
+        __syncthreads();
     };
     if (over && cut) hold(0);
     bool bad = !fits;
     if (over) {
         const int np = int(page_of(uint32_t(n - 1), a.c.div)) + 1;
         bool mine = false;
-        for (int i = tid; i < np; i += TH) {
+        for (int i = tid; i < np; i += kPlanThreads) {
             const int p = a.t.table[b * a.t.ld + i];
             mine |= p < 0 || p >= a.c.pages;
         }
@@ -237,49 +235,39 @@ __global__ __launch_bounds__(64 * W) void evict_plan_kernel(EvictArgs a) {
         if (tid == 0) a.count[row] = idle ? -1 : 0;
         return;
     }
-    const bool all = old <= BLOCK;
-    // the cut-th largest key (1 <= cut < old): its upper bits, until the
-    // keys that share them are all wanted (mostly after two passes)
+    const bool all = old <= kHeldSums;
+    // The cut-th largest key (1 <= cut < old): its upper bits, 12 + 12 + 8,
+    // until the keys that share them are all wanted or few.
     uint32_t prefix = 0, want = uint32_t(cut), equal = 0;
     int shift = 32;
     for (int pass = 0; pass < 3; pass++) {
-        const int bits = pass < 2 ? 11 : 10;
-        for (int i = tid; i < kCopies * (kBins + 16) / 4; i += TH)
-            reinterpret_cast<uint4*>(&hist[0][0])[i] = make_uint4(0, 0, 0, 0);
+        const int bits = pass < 2 ? kBinBits : 32 - 2 * kBinBits;
+        reinterpret_cast<uint4*>(hist)[tid] = make_uint4(0, 0, 0, 0);
+        if (tid == 0) found[3] = 0;
         __syncthreads();
         shift -= bits;
-        uint32_t* mine = hist[lane % kCopies];
-        uint32_t past = 0;  // keys 0 of places past the end
-        for (int i0 = 0; i0 < old; i0 += BLOCK) {
+        for (int i0 = 0; i0 < old; i0 += kHeldSums) {
             if (!all) hold(i0);
-            past += uint32_t(rounds * TH - min(old - i0, BLOCK));
-#pragma unroll
-            for (int r = 0; r < HELD; r++) {
-                if (r >= rounds) break;
+#pragma unroll 4
+            for (int r = 0; r < rounds; r++) {
+                const uint32_t k = own[r * 64];
                 if (pass == 0) {
-                    atomicAdd(&mine[k[r] >> 21], 1u);
-                } else if ((k[r] >> (shift + bits)) == prefix) {
-                    atomicAdd(&mine[(k[r] >> shift) & ((1u << bits) - 1)], 1u);
+                    if (w0 + r * 64 + lane < old) atomicAdd(&hist[k >> (32 - kBinBits)], 1u);
+                } else if ((k >> (shift + bits)) == prefix && w0 + r * 64 + lane < old) {
+                    atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
                 }
             }
         }
         __syncthreads();
-        // bins from the highest down, PER a thread
-        uint32_t nb[PER], sum = 0;
+        // bins from the highest down, four a thread
+        const int b0 = kBins - 4 * (tid + 1);
+        const uint4 q = *reinterpret_cast<const uint4*>(&hist[b0]);
+        uint32_t total, before = block_excl_scan<kPlanWaves>(q.x + q.y + q.z + q.w, &total, sh);
+        const uint32_t nb[4] = {q.w, q.z, q.y, q.x};
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            nb[i] = 0;
-            const int bin = kBins - 1 - PER * tid - i;
-#pragma unroll
-            for (int c = 0; c < kCopies; c++) nb[i] += hist[c][bin];
-            if (bin == 0 && prefix == 0) nb[i] -= past;
-            sum += nb[i];
-        }
-        uint32_t total, before = block_excl_scan<W>(sum, &total, sh);
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
+        for (int i = 0; i < 4; i++) {
             if (before < want && want <= before + nb[i]) {
-                found[0] = uint32_t(kBins - 1 - PER * tid - i);
+                found[0] = uint32_t(b0 + 3 - i);
                 found[1] = want - before;
                 found[2] = nb[i];
             }
@@ -289,90 +277,97 @@ __global__ __launch_bounds__(64 * W) void evict_plan_kernel(EvictArgs a) {
         prefix = (prefix << bits) | found[0];
         want = found[1];
         equal = found[2];
-        if (equal == want) break;
+        if (equal == want || equal <= kFew) break;
     }
-    // Keys from `least` on stay; with ties (all 32 bits are known then), of
-    // the keys equal to it the first `want`.
-    const uint32_t least = prefix << shift;
-    const bool ties = equal > want;
-    int32_t* dst = a.dst + row * a.m;
-    int32_t* src = a.src + row * a.m;
-    uint32_t eqs = 0, holes = 0, highs = 0;  // of the blocks before
-    for (int i0 = 0; i0 < old; i0 += BLOCK) {
-        if (!all) hold(i0);
-        uint32_t total, eq = 0;
-        if (ties) {
-#pragma unroll
-            for (int r = 0; r < HELD; r++) {
-                if (r >= rounds) break;
-                eq += uint32_t(__popcll(__ballot(k[r] == least) & lanes_below(w0 + r * 64, old)));
+    // Which sums stay: keys above `least`, and of those equal to it the ones
+    // up to slot `upto`.
+    uint32_t least = prefix << shift;
+    int upto = 0x7fffffff;
+    if (equal > want && equal <= kFew) {
+        // few keys share the bits: each one's rank among them (key descending,
+        // slot ascending) is the number of greater ones
+        for (int i0 = 0; i0 < old; i0 += kHeldSums) {
+            if (!all) hold(i0);
+#pragma unroll 4
+            for (int r = 0; r < rounds; r++) {
+                const uint32_t k = own[r * 64];
+                const int i = w0 + r * 64 + lane;
+                if ((k >> shift) == prefix && i < old) cand[atomicAdd(&found[3], 1u)] = uint64_t(k) << 32 | uint32_t(~i);
             }
-            eq = eqs + block_excl_scan<W>(lane == 0 ? eq : 0, &total, sh);
-            eq = uint32_t(__builtin_amdgcn_readfirstlane(int(eq)));
+        }
+        __syncthreads();
+        if (tid < int(equal)) {
+            const uint64_t mine = cand[tid];
+            uint32_t rank = 0;
+            for (int i = 0; i < int(equal); i++) rank += cand[i] > mine;
+            if (rank == want - 1) {
+                found[0] = uint32_t(mine >> 32);
+                found[1] = uint32_t(~mine);
+            }
+        }
+        __syncthreads();
+        least = found[0];
+        upto = int(found[1]);
+    } else if (equal > want) {
+        // many equal ones (all 32 bits are known): the slot of the want-th
+        uint32_t eqs = 0;  // in the blocks before
+        for (int i0 = 0; i0 < old; i0 += kHeldSums) {
+            if (!all) hold(i0);
+            uint32_t total, eq = 0;
+            for (int r = 0; r < rounds; r++)
+                eq += uint32_t(__popcll(__ballot(own[r * 64] == least) & lanes_below(w0 + r * 64, old)));
+            eq = block_excl_scan<kPlanWaves>(lane == 0 ? eq : 0, &total, sh);
+            eq = eqs + uint32_t(__builtin_amdgcn_readfirstlane(int(eq)));
+            for (int r = 0; r < rounds; r++) {
+                const uint64_t same = __ballot(own[r * 64] == least) & lanes_below(w0 + r * 64, old);
+                if ((same >> lane & 1) && eq + lanes_before(same) == want - 1) found[1] = uint32_t(w0 + r * 64 + lane);
+                eq += uint32_t(__popcll(same));
+            }
             eqs += total;
         }
-        // the lanes whose sum stays (eq: equal ones before)
-        auto stays = [&](int r, uint32_t& eq_now) -> uint64_t {
-            const uint64_t in = lanes_below(w0 + r * 64, old);
-            if (!ties) return __ballot(k[r] >= least) & in;
-            const uint64_t same = __ballot(k[r] == least) & in;
-            const uint64_t more = __ballot(k[r] > least) & in;
-            const uint64_t first = __ballot(eq_now + lanes_before(same) < want) & same;
-            eq_now += uint32_t(__popcll(same));
-            return more | first;
+        __syncthreads();
+        upto = int(found[1]);
+    }
+    int32_t* dst = a.dst + row * a.m;
+    int32_t* src = a.src + row * a.m;
+    uint32_t holes = 0, highs = 0;  // of the blocks before
+    for (int i0 = 0; i0 < old; i0 += kHeldSums) {
+        if (!all) hold(i0);
+        // the lanes of round r whose place becomes free, and whose row has to
+        // move (few instructions: the CU's one scalar unit, and its vector
+        // units together, start one a cycle for all sixteen waves)
+        const uint64_t bound = uint64_t(least) << 32 | uint32_t(~upto);
+        auto masks = [&](int r, uint64_t& to, uint64_t& from) {
+            const int i = w0 + r * 64 + lane;
+            const uint64_t stay = __ballot((uint64_t(own[r * 64]) << 32 | uint32_t(~i)) >= bound && i < old);
+            const uint64_t low = __ballot(i < cut);
+            to = low & ~stay;
+            from = stay & ~low;
         };
-        // a run that lies on one side of cut, with no ties: one ballot a round
-        const int run = w0 + rounds * 64;
-        const bool plain = !ties && run <= old && (run <= cut || w0 >= cut);
         // (a block has at most 32768 of either: two counts in a word)
-        uint32_t count = 0, e = eq;
-        if (plain) {
-#pragma unroll
-            for (int r = 0; r < HELD; r++) {
-                if (r >= rounds) break;
-                count += uint32_t(__popcll(__ballot(k[r] >= least)));
-            }
-            count = run <= cut ? uint32_t(rounds) * 64 - count : count << 16;
-        } else {
-#pragma unroll
-            for (int r = 0; r < HELD; r++) {
-                if (r >= rounds) break;
-                const uint64_t stay = stays(r, e), low = lanes_below(w0 + r * 64, cut);
-                const uint64_t in = lanes_below(w0 + r * 64, old);
-                count += uint32_t(__popcll(low & in & ~stay)) + (uint32_t(__popcll(stay & ~low)) << 16);
-            }
+        uint32_t total, count = 0;
+#pragma unroll 4
+        for (int r = 0; r < rounds; r++) {
+            uint64_t to, from;
+            masks(r, to, from);
+            count += uint32_t(__popcll(to)) + (uint32_t(__popcll(from)) << 16);
         }
-        uint32_t at = block_excl_scan<W>(lane == 0 ? count : 0, &total, sh);
+        uint32_t at = block_excl_scan<kPlanWaves>(lane == 0 ? count : 0, &total, sh);
         at = uint32_t(__builtin_amdgcn_readfirstlane(int(at)));
         int32_t* hole = dst + holes + (at & 0xffffu);
         int32_t* high = src + highs + (at >> 16);
-        e = eq;
-        if (plain) {
-            int32_t* list = run <= cut ? hole : high;
-            const bool holes_here = run <= cut;
-#pragma unroll
-            for (int r = 0; r < HELD; r++) {
-                if (r >= rounds) break;
-                const bool mine = (k[r] >= least) != holes_here;
-                const uint64_t m = __ballot(mine);
-                if (mine) list[lanes_before(m)] = w0 + r * 64 + lane;
-                list += __popcll(m);
+#pragma unroll 2
+        for (int r = 0; r < rounds; r++) {
+            const int i = w0 + r * 64 + lane;
+            uint64_t to, from;
+            masks(r, to, from);
+            if (to) {
+                if (to >> lane & 1) hole[lanes_before(to)] = i;
+                hole += __popcll(to);
             }
-        } else {
-#pragma unroll
-            for (int r = 0; r < HELD; r++) {
-                if (r >= rounds) break;
-                const int i = w0 + r * 64;
-                const uint64_t stay = stays(r, e), low = lanes_below(i, cut);
-                const uint64_t to = low & lanes_below(i, old) & ~stay, from = stay & ~low;
-                if (to) {
-                    if (to >> lane & 1) hole[lanes_before(to)] = i + lane;
-                    hole += __popcll(to);
-                }
-                if (from) {
-                    if (from >> lane & 1) high[lanes_before(from)] = i + lane;
-                    high += __popcll(from);
-                }
+            if (from) {
+                if (from >> lane & 1) high[lanes_before(from)] = i;
+                high += __popcll(from);
             }
         }
         holes += total & 0xffffu;
@@ -563,10 +558,12 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
     a.ushift = row_units >= 4 ? 2 : (row_units >= 2 ? 1 : 0);
     a.slices = (row_units + (1 << a.ushift) - 1) >> a.ushift;
     const int64_t per = (iq::kMoveThreads >> a.ushift) * iq::kMoveUnroll;
+    iq::allow_big_lds<iq::evict_plan_kernel>();
     for (a.b0 = 0; a.b0 < B; a.b0 += step) {
         const int nb = std::min(step, B - a.b0);
         const unsigned hk = unsigned(a.c.hk), nz = unsigned(nb);
-        iq::evict_plan_kernel<16, 32><<<dim3(hk, nz), 1024, 0, s>>>(a);
+        const size_t held = size_t(std::min<int64_t>((a.t.cap + 1023) / 1024 * 1024, iq::kHeldSums));
+        iq::evict_plan_kernel<<<dim3(hk, nz), iq::kPlanThreads, (iq::kBins + held) * 4, s>>>(a);
         // (a cache that cannot hold more than the budget has nothing to move)
         if (a.t.cap <= budget) continue;
         // fewer than two workgroups a CU in an ordered move: spread over blocks of rows
