@@ -28,7 +28,9 @@
  * allocates, frees or synchronises, so any call can be graph-captured the
  * first time it is made.  A stream under graph capture cannot allocate: a
  * call on a capturing stream that has no workspace yet (no iq_init_stream
- * before the capture) returns an error and enqueues nothing.
+ * before the capture) returns an error and enqueues nothing.  A captured
+ * graph uses the workspace of the stream it was captured on: its replays have
+ * to be ordered with that stream's calls and with other graphs captured on it.
  */
 #ifndef IQ_H
 #define IQ_H
@@ -263,14 +265,17 @@ int iq_kv_append(const float* q, const float* k, const float* v, const int64_t* 
  * [B][table_ld] of which the first max_pages entries of a row may be used
  * (entries past a sequence's last page are not read), lens int32 [B], 1 <= B
  * <= 1024.  Scores, softmax and sums are fp32; the 16-bit keys and values
- * are exact.  Keys and values past a sequence's length have no influence,
+ * are taken as they are.  Keys and values past a sequence's length have no influence,
  * whatever they hold.
  * weights (may be NULL): fp32 [B][kv_heads][weights_ld], weights_ld >=
  * max_pages * page_size; weights[b][j][t] += sum over the heads h of key/value
- * head j of p[b,h,t], for t < lens[b]; the rest is left as it was.
+ * head j of p[b,h,t], for t < lens[b]; the rest is left as it was.  A
+ * sequence's scores lie in the workspace: max_pages * page_size * q_heads may
+ * be at most 20971520 with weights (IQ_ETOOLARGE).
  * A sequence of length 0 gives zeros.  A length below 0 or above max_pages *
- * page_size gives NaN (its weights are left as they were), as does a page id
- * outside [0, pages) or a non-finite q, key or value that is attended to. */
+ * page_size gives NaN, its weights left as they were.  A page id outside [0,
+ * pages) among the sequence's pages, or a non-finite q, key or value, gives
+ * NaN to the heads that read it and to the weights made of them. */
 int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t max_pages,
                    const int32_t* lens, int B, int q_heads, float scale, float* out, float* weights,
                    int64_t weights_ld, void* stream);
@@ -285,7 +290,10 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
  * weights move along, and weights[b][h][t] = 0 for budget <= t < n, so that a
  * slot appended later starts at 0.  new_lens[b] = min(lens[b], budget) for
  * every head alike (the pages past it are free); it must not overlap lens.
- * Pages must not be shared between the sequences of a call.  A sequence whose
+ * Pages must not be shared between the sequences of a call nor appear twice in
+ * one.  The lists of what moves lie in the workspace: min(budget - recent,
+ * max_pages * page_size - budget) * kv_heads may be at most 8 million
+ * (IQ_ETOOLARGE).  A sequence whose
  * length is below 0 or above max_pages * page_size, or any of whose first
  * ceil(n / page_size) page ids lies outside [0, pages), is left as it is and
  * its new length is its old one.  1 <= B <= 1024, budget >= 1; table, lens and
@@ -295,7 +303,7 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
                 void* stream);
 
 /* Log probabilities over rows of logits, fp32 [T][V] with `ld` >= V floats
- * from row to row (V < 2^31):
+ * from row to row (V < 2^31 - 65536):
  *   logprob[t]  log softmax(row t)[tokens[t]]; NaN for a token outside [0, V)
  *   entropy[t]  -sum p log p
  *   top_ids[t][i], top_logprobs[t][i], i < top <= 64: the `top` largest, by

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
         for (int i = threadIdx.x; i < gh * d; i += 64 * kAttnWaves) out[i] = x;
         return;
     }
-    const int t0 = int(it.j * it.c) * kAttnTile, t1 = min(n, t0 + int(it.c) * kAttnTile);
+    const int t0 = int(it.j * it.c) * kAttnTile, t1 = t0 + min(n - t0, int(it.c) * kAttnTile);
     const int ntiles = (t1 - t0 + kAttnTile - 1) / kAttnTile;
 
     // row r of a tile: element offset of its (page, slot), 0 where there is none
@@ -534,7 +534,8 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
     rc = iq::check_table(a.c, table, table_ld, max_pages, lens, B, &a.t);
     if (rc) return rc;
     if (!q || !out) return IQ_ENULL;
-    if (q_heads < 1 || q_heads > 16384 || q_heads % a.c.hk || !std::isfinite(scale)) return IQ_ESHAPE;
+    a.mul = scale * 1.44269504088896340736f;
+    if (q_heads < 1 || q_heads > 16384 || q_heads % a.c.hk || !std::isfinite(a.mul)) return IQ_ESHAPE;
     if (weights && weights_ld < a.t.cap) return IQ_ESHAPE;
     const int64_t row = int64_t(q_heads) * a.c.d;
     if (iq::ranges_overlap(q, B * row * 4, out, B * row * 4)) return IQ_EALIAS;
@@ -546,7 +547,6 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
     a.group = q_heads / a.c.hk;
     a.ht = (a.group + 15) / 16;
     a.nh = uint32_t(a.c.hk * a.ht);
-    a.mul = scale * 1.44269504088896340736f;
     // as many work items as run at once: 4, 3, 2 or 1 workgroups a CU by the
     // registers (d <= 64) and the LDS of an instance.  Measured for d = 128 on
     // 131072 tokens / 32 sequences of up to 8192: 1 a CU 64.7 / 29.2 us, 2 63.7

@@ -59,7 +59,7 @@ def test_attention():
     def call(q=P, c=None, table=P, ld=8, pages=8, lens=P, B=4, hq=4, scale=0.1, out=2 * P, w=None, wld=0):
         return L.iq_attn_decode(q, c or kv(), table, ld, pages, lens, B, hq, scale, out, w, wld, None)
     for bad in (dict(B=0), dict(B=1025), dict(hq=0), dict(hq=3), dict(hq=-2), dict(hq=16386), dict(pages=0), dict(ld=7),
-                dict(scale=float("nan")), dict(scale=float("inf")), dict(w=P, wld=127)):
+                dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(w=P, wld=127)):
         assert call(**bad) == SHAPE, bad
     for bad in (dict(q=None), dict(table=None), dict(lens=None), dict(out=None)):
         assert call(**bad) == NULL, bad

@@ -203,3 +203,18 @@ def test_pool_past_32_bits():
     k[-n:], v[-n:] = pg.cache.k, pg.cache.v
     out = ops.attn_decode(q, ops.KvCache(k, v), pg.table + (big - n), pg.lens_t)
     assert torch.equal(out, ref)
+
+
+def test_longest_sequence():
+    """2^31 - 65536 tokens, the most that a table can hold, in one page of
+    65536 slots that every table entry names: the softmax over equal runs is
+    the softmax over one of them.  Every lane adds up to 2^31 / (512 * 4 * 32) *
+    8 = 2^18 rounded terms, each off by at most half a step of the sum."""
+    rng = np.random.default_rng(12)
+    n, runs = 65536, 32767
+    k, v = (torch.from_numpy(rng.standard_normal((1, n, 1, 8)).astype(np.float32)).to(BF).cuda() for _ in range(2))
+    q = torch.from_numpy(rng.standard_normal((1, 2, 8)).astype(np.float32)).cuda()
+    table = torch.zeros(1, runs, dtype=torch.int32, device="cuda")
+    out = ops.attn_decode(q, ops.KvCache(k, v), table, torch.tensor([runs * n], dtype=torch.int32, device="cuda"))
+    ref, _, ck, cv = attn_f64(q[0].cpu().double().numpy(), k[0].cpu().double().numpy(), v[0].cpu().double().numpy(), 8 ** -0.5)
+    assert np.all(np.abs(out[0].cpu().numpy() - ref) <= (attn_rel(8, ck)[:, None] + 2 ** 18 * EPS32) * cv)

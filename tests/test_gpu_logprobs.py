@@ -121,6 +121,16 @@ def test_peaked_and_flat():
     check(x, [77, 0, 1, 2], 20)
 
 
+def test_long_rows_with_many_alternatives():
+    """More parts of a row than one step of the join holds."""
+    rng = np.random.default_rng(9)
+    x = (rng.standard_normal((2, 700001)) * 2).astype(np.float32)
+    x[1] = np.round(x[1] * 4) / 4
+    check(x, [5, 700000], 64)
+    x[0, 300000] = np.nan
+    check(x, [5, 700000], 64)
+
+
 def test_more_elements_than_32_bits():
     """Rows past 2^31 floats from the first."""
     V, T = 160, 3
