@@ -410,11 +410,14 @@ __device__ __forceinline__ float2 chunk_ml(const AttnArgs& a, uint2 pl, int head
 }
 
 // One workgroup per (head, sequence): the chunks' rows, each times 2^(its
-// maximum - the largest so far), in chunk order within 256 / (d / 4 rounded
-// to a power of two) runs that are then added in order.
+// maximum - the largest so far), in chunk order within TH / (d / 4 rounded to
+// a power of two) runs that are then added in order.  TH: 1024 threads for
+// few sequences with many chunks each (one of 20000 tokens, 2 key/value heads:
+// 17.4 us with 256, 15.6 so; their runs are added in pairs down to 8), else 256.
+template <int TH>
 __device__ __forceinline__ void join_head(const AttnArgs& a, int b, int head) {
-    __shared__ float4_t xs[256];
-    __shared__ float2 ms[256];
+    __shared__ float4_t xs[TH];
+    __shared__ float2 ms[TH];
     const int d = a.c.d, tid = threadIdx.x;
     const uint2 pl = a.plan[b];
     if (pl.x < 2) return;
@@ -422,8 +425,8 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, int b, int head) {
     const float* part = a.part + (int64_t(pl.y) * a.nh + hidx) * 16 * d + h * d;
     int w = 2;  // 16-byte pieces of a row, to a power of two
     while (w * 4 < d) w *= 2;
-    const int e = tid % w * 4, run = tid / w, runs = 256 / w, n = int(pl.x);
-    float M = -INFINITY, L = 0.0f;
+    const int e = tid % w * 4, run = tid / w, runs = TH / w, n = int(pl.x);
+    float M = -3.4e38f, L = 0.0f;  // (finite: a run may be without chunks)
     float4_t x = {0, 0, 0, 0};
     auto add = [&](float2 v, float4_t y) {
         const float mn = fmaxf(M, v.x), f = __builtin_amdgcn_exp2f(M - mn), k = __builtin_amdgcn_exp2f(v.x - mn);
@@ -450,8 +453,18 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, int b, int head) {
     xs[tid] = x;
     ms[tid] = make_float2(M, L);
     __syncthreads();
+    if constexpr (TH > 256) {
+        for (int s = runs / 2; s > 4; s /= 2) {
+            if (run < s) {
+                add(ms[tid + s * w], xs[tid + s * w]);
+                xs[tid] = x;
+                ms[tid] = make_float2(M, L);
+            }
+            __syncthreads();
+        }
+    }
     if (run == 0 && e < d) {
-        for (int r = 1; r < min(runs, n); r++) add(ms[r * w + tid], xs[r * w + tid]);
+        for (int r = 1; r < min(TH > 256 ? min(runs, 8) : runs, n); r++) add(ms[r * w + tid], xs[r * w + tid]);
         const float inv = 1.0f / L;
         float* out = a.out + (int64_t(b) * a.hq + head) * d + e;
 #pragma unroll
@@ -459,23 +472,28 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, int b, int head) {
     }
 }
 
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) { join_head(a, blockIdx.y, blockIdx.x); }
+template <int TH>
+__global__ __launch_bounds__(TH) void attn_join_kernel(AttnArgs a) {
+    join_head<TH>(a, blockIdx.y, blockIdx.x);
+}
 
-// The same with further workgroups that add the weights: for 256 tokens of a
+// The same with further workgroups that add the weights: for TH tokens of a
 // key/value head, weights[b][j][t] += sum over the group's heads, in order,
 // of 2^(score - maximum) / sum.  The heads' maxima and sums over the chunks
-// are made here again, 16 heads x 16 runs of chunks at a time.
-__global__ __launch_bounds__(256) void attn_weights_kernel(AttnArgs a, float* weights, int64_t wld, float up) {
-    __shared__ float2 run_ml[16][17];
+// are made here again, 16 heads x TH / 16 runs of chunks at a time.
+template <int TH>
+__global__ __launch_bounds__(TH) void attn_weights_kernel(AttnArgs a, float* weights, int64_t wld, float up) {
+    constexpr int RUNS = TH / 16;
+    __shared__ float2 run_ml[16][RUNS + 1];
     __shared__ float2 head_ml[16];  // maximum less `up`, 1 / sum
     const int b = blockIdx.y, tid = threadIdx.x;
     if (int(blockIdx.x) < a.hq) {
-        join_head(a, b, blockIdx.x);
+        join_head<TH>(a, b, blockIdx.x);
         return;
     }
     const int n = a.t.lens[b];
     const uint32_t w = blockIdx.x - uint32_t(a.hq);
-    const int j = int(w % uint32_t(a.c.hk)), t0 = int(w / uint32_t(a.c.hk)) * 256, t = t0 + tid;
+    const int j = int(w % uint32_t(a.c.hk)), t0 = int(w / uint32_t(a.c.hk)) * TH, t = t0 + tid;
     if (n > a.t.cap || t0 >= n) return;
     const uint2 pl = a.plan[b];
     const int64_t row = int64_t(b) * a.c.hk + j;
@@ -493,14 +511,14 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(AttnArgs a, float* we
             if (pl.x < 2) {
                 if (run == 0) add(reinterpret_cast<const float2*>(a.fin)[int64_t(b) * a.hq + j * a.group + h0 + h]);
             } else {
-                for (uint32_t i = uint32_t(run); i < pl.x; i += 16) add(chunk_ml(a, pl, j * a.group + h0 + h, i));
+                for (uint32_t i = uint32_t(run); i < pl.x; i += RUNS) add(chunk_ml(a, pl, j * a.group + h0 + h, i));
             }
         }
         __syncthreads();
         run_ml[h][run] = make_float2(M, L);
         __syncthreads();
         if (tid < gh) {
-            const int runs = pl.x < 2 ? 1 : int(min(pl.x, 16u));
+            const int runs = pl.x < 2 ? 1 : int(min(pl.x, uint32_t(RUNS)));
             M = run_ml[tid][0].x;
             L = run_ml[tid][0].y;
             for (int r = 1; r < runs; r++) add(run_ml[tid][r]);
@@ -575,12 +593,19 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
         const int64_t grid = iq::attn_max_items(a.B, a.nh, a.t.cap, a.target);
         if (kv->type == IQ_KV_BF16) iq::launch_attn<IQ_KV_BF16>(a, unsigned(grid), s);
         else iq::launch_attn<IQ_KV_F16>(a, unsigned(grid), s);
+        // (a sequence has at most target / nh chunks and one more)
+        const bool many = a.B <= 4 && std::min<int64_t>(capt / iq::kAttnWaves, a.target / a.nh) > 64;
+        const int th = many ? 1024 : 256;
+        const dim3 heads{unsigned(q_heads), unsigned(a.B)};
         if (weights) {
-            const int64_t blocks = q_heads + (a.t.cap + 255) / 256 * int64_t(a.c.hk);
-            iq::attn_weights_kernel<<<dim3(unsigned(blocks), unsigned(a.B)), 256, 0, s>>>(
-                a, weights + int64_t(b0) * a.c.hk * weights_ld, weights_ld, kv->type == IQ_KV_F16 ? 12.0f : 0.0f);
+            float* w = weights + int64_t(b0) * a.c.hk * weights_ld;
+            const float up = kv->type == IQ_KV_F16 ? iq::Terms<IQ_KV_F16>::kUp : iq::Terms<IQ_KV_BF16>::kUp;
+            const dim3 all{unsigned(q_heads + (int64_t(a.t.cap) + th - 1) / th * a.c.hk), unsigned(a.B)};
+            if (many) iq::attn_weights_kernel<1024><<<all, 1024, 0, s>>>(a, w, weights_ld, up);
+            else iq::attn_weights_kernel<256><<<all, 256, 0, s>>>(a, w, weights_ld, up);
         } else if (capt > iq::kAttnWaves) {  // (else no sequence has two chunks)
-            iq::attn_join_kernel<<<dim3(unsigned(q_heads), unsigned(a.B)), 256, 0, s>>>(a);
+            if (many) iq::attn_join_kernel<1024><<<heads, 1024, 0, s>>>(a);
+            else iq::attn_join_kernel<256><<<heads, 256, 0, s>>>(a);
         }
     }
     return int(hipGetLastError());
