@@ -121,10 +121,11 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 // The rows are moved by two kernels.  The free places lie below cut and every
 // source at or above it, so evict_fill_kernel moves those rows in any order.
 // evict_shift_kernel then moves the newest ones (and the sums).  Where they
-// move by less than their number, places and sources overlap, and one
-// workgroup goes through a slice of all rows in ascending order, a chunk at
-// a time: read, barrier, write; a chunk's writes lie below every later
-// chunk's reads.  With many sequences and heads that kernel does both, and
+// move by less than their number, places and sources overlap: a thread takes
+// every by-th row in ascending order, or, where `by` gives too few threads
+// work, one workgroup goes through a slice of all rows, a chunk at a time:
+// read, barrier, write; a chunk's writes lie below every later chunk's reads.
+// With many sequences and heads that kernel does both, and
 // one launch is saved: the free places come first in its list.
 struct EvictArgs {
     KvView c;
@@ -139,7 +140,7 @@ struct EvictArgs {
     int32_t* src;
     int64_t m;
     int slices, ushift;    // slices of a row, of 1 << ushift 16-byte units
-    int blocks;            // workgroups along the rows, where the order is free
+    int blocks;            // workgroups along the rows, where they are not one's
     int filled;            // the free places are filled by an earlier launch
 };
 
@@ -376,43 +377,73 @@ __global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(EvictArgs a) {
     if (tid == 0) a.count[row] = int32_t(holes);
 }
 
-// Byte offset of (token t of sequence b, head h) in either pool (page ids
-// were checked by the plan).
-__device__ __forceinline__ int64_t kv_offset(const KvView& c, const KvTable& t, int b, int h, int tok) {
-    const uint32_t p = page_of(uint32_t(tok), c.div);
-    return 2 * kv_element(c, uint32_t(t.table[b * t.ld + p]), uint32_t(tok) - p * uint32_t(c.ps), uint32_t(h));
+// Byte offsets in either pool of N tokens of sequence b, head h (page ids were
+// checked by the plan; their loads go out together).
+template <int N>
+__device__ __forceinline__ void kv_offsets(const KvView& c, const KvTable& t, int b, int h, const int (&tok)[N],
+                                           int64_t (&at)[N]) {
+    const int32_t* table = t.table + b * t.ld;
+    uint32_t p[N], id[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        p[i] = page_of(uint32_t(tok[i]), c.div);
+        id[i] = uint32_t(table[p[i]]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) at[i] = 2 * kv_element(c, id[i], uint32_t(tok[i]) - p[i] * uint32_t(c.ps), uint32_t(h));
 }
 
 constexpr int kMoveThreads = 256, kMoveUnroll = 4;
 
 // Moves rows [m0, m1) of a list (m1 - m0 at most 2^31 less a chunk), a
-// slice's 16-byte units of each from `u0` on: a chunk of 4 units a thread is
-// read, then (after a barrier, if the order counts) written.
-template <bool ORDERED, class From, class To>
+// slice's 16-byte units of each from `u0` on, a chunk of 4 units a thread at a
+// time: read, then written.  ORDERED: no thread writes a chunk before all have
+// its values; the next chunk is requested before this one is written (the
+// call on one sequence of 20027 tokens, all but 64 kept, 12889 of them the
+// newest: 145 us without that and with loads that wait for one another, 84 so).
+template <int TH, bool ORDERED, class From, class To>
 __device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b, int h, int m0, int m1, int u0, From from,
                                           To to) {
-    const int rows = kMoveThreads >> a.ushift, r0 = int(threadIdx.x) >> a.ushift;
+    const int rows = TH >> a.ushift, r0 = int(threadIdx.x) >> a.ushift;
     const int u = u0 + (int(threadIdx.x) & ((1 << a.ushift) - 1));
     const int left = u < a.c.d / 8 ? m1 - r0 : 0;  // rows from m on are this thread's while m < left
-    pool += u * 16;
-    for (; m0 < m1; m0 += rows * kMoveUnroll) {
+    struct Chunk {
         u32x4_t x[kMoveUnroll];
         int64_t go[kMoveUnroll];
+    };
+    // (past the end the last row again, not written: no branch between the
+    // loads, which would wait for one another; likewise a unit past the row)
+    if (u < a.c.d / 8) pool += u * 16;
+    auto read = [&](int m, Chunk& c) {
+        int f[kMoveUnroll], t[kMoveUnroll];
+        int64_t at[kMoveUnroll];
 #pragma unroll
         for (int r = 0; r < kMoveUnroll; r++) {
-            const int m = m0 + r * rows;
-            if (m < left) {
-                x[r] = *reinterpret_cast<const u32x4_t*>(pool + kv_offset(a.c, a.t, b, h, from(m + r0)));
-                go[r] = kv_offset(a.c, a.t, b, h, to(m + r0));
-            }
+            const int i = min(m + r * rows + r0, m1 - 1);
+            f[r] = from(i);
+            t[r] = to(i);
         }
+        kv_offsets(a.c, a.t, b, h, f, at);
+        kv_offsets(a.c, a.t, b, h, t, c.go);
+#pragma unroll
+        for (int r = 0; r < kMoveUnroll; r++) c.x[r] = *reinterpret_cast<const u32x4_t*>(pool + at[r]);
+    };
+    const int step = rows * kMoveUnroll;
+    Chunk c, next;
+    read(m0, c);
+    for (; m0 < m1; m0 += step) {
         if (ORDERED) {
-            __builtin_amdgcn_s_waitcnt(0);  // (the values are here before another wave writes)
-            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < kMoveUnroll; r++) asm volatile("" : "+v"(c.x[r]));  // (waits for the values)
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
         }
+        if (m0 + step < m1) read(m0 + step, next);
 #pragma unroll
         for (int r = 0; r < kMoveUnroll; r++)
-            if (m0 + r * rows < left) *reinterpret_cast<u32x4_t*>(pool + go[r]) = x[r];
+            if (m0 + r * rows < left) *reinterpret_cast<u32x4_t*>(pool + c.go[r]) = c.x[r];
+        c = next;
     }
 }
 
@@ -436,53 +467,88 @@ __global__ __launch_bounds__(kMoveThreads, 4) void evict_fill_kernel(EvictArgs a
     const int m0 = block * per;
     if (m0 >= holes) return;
     char* pool = const_cast<char*>(sl < a.slices ? a.c.k : a.c.v);
-    move_rows<false>(a, pool, b, h, m0, min(holes, m0 + per), (sl % a.slices) << a.ushift,
+    move_rows<kMoveThreads, false>(a, pool, b, h, m0, min(holes, m0 + per), (sl % a.slices) << a.ushift,
                      [&](int i) { return src[i]; }, [&](int i) { return dst[i]; });
 }
 
 // grid: x = (K, V) x slices x blocks of rows, then one for the sums; y = head;
 // z = sequence
-__global__ __launch_bounds__(kMoveThreads, 4) void evict_shift_kernel(EvictArgs a) {
+template <int TH>
+__global__ __launch_bounds__(TH, TH == kMoveThreads ? 4 : 1) void evict_shift_kernel(EvictArgs a) {
     const int h = blockIdx.y, b = a.b0 + int(blockIdx.z), row = int(blockIdx.z) * a.c.hk + h;
     const int holes = a.count[row];
     if (holes < 0) return;
     const int n = a.t.lens[b], recent = int(a.recent), cut = int(a.budget) - recent, tid = threadIdx.x;
     const int32_t* dst = a.dst + row * a.m;
     const int32_t* src = a.src + row * a.m;
-    auto from = [&](int i) { return i < holes ? src[i] : n - recent + (i - holes); };
-    auto to = [&](int i) { return i < holes ? dst[i] : cut + (i - holes); };
+    // (the lists have an entry at least: the load needs no branch)
+    auto from = [&](int i) {
+        const int s = src[i < holes ? i : 0];
+        return i < holes ? s : n - recent + (i - holes);
+    };
+    auto to = [&](int i) {
+        const int s = dst[i < holes ? i : 0];
+        return i < holes ? s : cut + (i - holes);
+    };
     const int moves = holes + recent;  // (at most the budget)
     if (int(blockIdx.x) == 2 * a.slices * a.blocks) {
         float* w = a.w + (int64_t(b) * a.c.hk + h) * a.wld;
-        for (int m0 = a.filled ? holes : 0; m0 < moves; m0 += kMoveThreads * kMoveUnroll) {
+        for (int m0 = a.filled ? holes : 0; m0 < moves; m0 += TH * kMoveUnroll) {
             float x[kMoveUnroll];
+            int f[kMoveUnroll], t[kMoveUnroll];
 #pragma unroll
             for (int r = 0; r < kMoveUnroll; r++) {
-                const int i = m0 + r * kMoveThreads + tid;
-                x[r] = i < moves ? w[from(i)] : 0.0f;
+                const int i = min(m0 + r * TH + tid, moves - 1);
+                f[r] = from(i);
+                t[r] = to(i);
             }
-            __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll
+            for (int r = 0; r < kMoveUnroll; r++) x[r] = w[f[r]];
+            __builtin_amdgcn_s_waitcnt(0);  // (the values are here before another wave writes)
             __syncthreads();
 #pragma unroll
-            for (int r = 0; r < kMoveUnroll; r++) {
-                const int i = m0 + r * kMoveThreads + tid;
-                if (i < moves) w[to(i)] = x[r];
-            }
+            for (int r = 0; r < kMoveUnroll; r++)
+                if (m0 + r * TH + tid < moves) w[t[r]] = x[r];
         }
         __syncthreads();
-        for (int i = int(a.budget) + tid; i < n; i += kMoveThreads) w[i] = 0.0f;
+        for (int i = int(a.budget) + tid; i < n; i += TH) w[i] = 0.0f;
         return;
     }
     const int block = int(blockIdx.x) / (2 * a.slices), sl = int(blockIdx.x) % (2 * a.slices);
     char* pool = const_cast<char*>(sl < a.slices ? a.c.k : a.c.v);
-    const int u0 = (sl % a.slices) << a.ushift;
-    const int per = (kMoveThreads >> a.ushift) * kMoveUnroll;
-    if (a.filled && n - a.budget >= recent) {
-        // the newest rows' places and sources do not meet: any order
+    const int u0 = (sl % a.slices) << a.ushift, rows = TH >> a.ushift, per = rows * kMoveUnroll;
+    const int by = n - int(a.budget);  // how far the newest rows move
+    if (a.filled && by >= recent) {
+        // their places and sources do not meet: any order
         for (int m0 = holes + block * per; m0 < moves; m0 += a.blocks * per)
-            move_rows<false>(a, pool, b, h, m0, min(moves, m0 + per), u0, from, to);
+            move_rows<TH, false>(a, pool, b, h, m0, min(moves, m0 + per), u0, from, to);
+    } else if (a.filled && by >= rows) {
+        // row i goes where row i - by was read: the rows of one remainder
+        // modulo `by` are a thread's, in ascending order, reads first
+        const int u = u0 + (tid & ((1 << a.ushift) - 1));
+        if (u >= a.c.d / 8) return;
+        pool += u * 16;
+        for (int c = block * rows + (tid >> a.ushift); c < by; c += a.blocks * rows)
+            for (int64_t i = c; i < recent; i += int64_t(by) * kMoveUnroll) {
+                u32x4_t x[kMoveUnroll];
+                int f[kMoveUnroll], t[kMoveUnroll];
+                int64_t at[kMoveUnroll], go[kMoveUnroll];
+#pragma unroll
+                for (int r = 0; r < kMoveUnroll; r++) {
+                    const int m = int(min(i + int64_t(r) * by, int64_t(recent) - 1));
+                    f[r] = n - recent + m;
+                    t[r] = cut + m;
+                }
+                kv_offsets(a.c, a.t, b, h, f, at);
+                kv_offsets(a.c, a.t, b, h, t, go);
+#pragma unroll
+                for (int r = 0; r < kMoveUnroll; r++) x[r] = *reinterpret_cast<const u32x4_t*>(pool + at[r]);
+#pragma unroll
+                for (int r = 0; r < kMoveUnroll; r++)
+                    if (i + int64_t(r) * by < recent) *reinterpret_cast<u32x4_t*>(pool + go[r]) = x[r];
+            }
     } else if (block == 0) {
-        move_rows<true>(a, pool, b, h, a.filled ? holes : 0, moves, u0, from, to);
+        move_rows<TH, true>(a, pool, b, h, a.filled ? holes : 0, moves, u0, from, to);
     }
 }
 
@@ -573,10 +639,12 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
         if (a.filled) {
             a.blocks = int(std::min<int64_t>((m + per - 1) / per, 65536));
             iq::evict_fill_kernel<<<dim3(2 * unsigned(a.slices * a.blocks) + iq::kSumBlocks, hk, nz), iq::kMoveThreads, 0, s>>>(a);
-            a.blocks = int(std::min<int64_t>((recent + per - 1) / per, 64));
-            a.blocks = std::max(a.blocks, 1);
+            // (four times the threads: an ordered move has few workgroups)
+            a.blocks = int(std::max<int64_t>(1, std::min<int64_t>((recent + 4 * per - 1) / (4 * per), 64)));
+            iq::evict_shift_kernel<1024><<<dim3(2 * unsigned(a.slices * a.blocks) + 1, hk, nz), 1024, 0, s>>>(a);
+        } else {
+            iq::evict_shift_kernel<iq::kMoveThreads><<<dim3(2 * unsigned(a.slices) + 1, hk, nz), iq::kMoveThreads, 0, s>>>(a);
         }
-        iq::evict_shift_kernel<<<dim3(2 * unsigned(a.slices * a.blocks) + 1, hk, nz), iq::kMoveThreads, 0, s>>>(a);
     }
     return int(hipGetLastError());
 }

@@ -136,7 +136,8 @@ def test_evict_layouts(hk, d, page, order):
 
 
 @pytest.mark.parametrize("n,budget,recent", [(20011, 5000, 700), (20011, 20010, 9000), (20011, 15000, 0),
-                                             (70000, 1000, 999)])
+                                             (70000, 1000, 999), (20011, 19000, 18000), (20011, 13000, 12900),
+                                             (9000, 8743, 8000), (9000, 8745, 8000)])
 def test_evict_long(n, budget, recent):
     check_evict(n + budget, BF, [n, 40], 2, 64, 16, budget, recent)
 
