@@ -5,7 +5,10 @@
 // is 7 multiply-adds for Qwen2.5-7B where HBM delivers one element per two
 // cycles and lane, too many beside the unpacking; on the matrix cores the up
 // to 16 heads of a group are the 16 columns of one product and cost nothing.
-// What bounds the operator is the read of the cache.
+// What bounds the operator is the read of the cache: 131072 tokens, 4 heads of
+// 128 in bf16 take 56.3 us (4.77 TB/s; a device copy reaches 4.74), every byte
+// read once, the matrix cores busy for 12 % of it; 32 sequences of up to 8192
+// tokens, 2 heads, 21 us (4.1 TB/s).  A join adds 4 to 5 us.
 //
 //   scores  S^T[token][head] = K[token][d] . q^T[d][head]
 //   sums    O^T[d][head]    += V^T[d][token] . P^T[token][head]

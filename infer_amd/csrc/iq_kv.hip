@@ -14,7 +14,9 @@ namespace {
 // lost its last bits in 32: 131072 rad in fp32 is known to 0.008) and its
 // sine and cosine taken in 32.  A thread then turns 4 pairs of one head
 // (two 16-byte loads, two 16- or 8-byte stores; without rotation, or past
-// rot_dim, it moves the values as they are).
+// rot_dim, it moves the values as they are).  1021 tokens of 12 + 2 x 2 heads
+// of 128: 6.6 us (2.4 TB/s); 16 tokens of 28 + 2 x 4: 3.6 us, a launch and two
+// load latencies.
 struct AppendArgs {
     const float *q, *k, *v;
     const int64_t *pos, *slots;
@@ -400,12 +402,12 @@ constexpr int kMoveThreads = 256, kMoveUnroll = 4;
 // time: read, then written.  ORDERED: no thread writes a chunk before all have
 // its values; the next chunk is requested before this one is written (the
 // call on one sequence of 20027 tokens, all but 64 kept, 12889 of them the
-// newest: 145 us without that and with loads that wait for one another, 84 so).
+// newest: 145 us without that and with loads that wait for one another).
 template <int TH, bool ORDERED, class From, class To>
-__device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b, int h, int m0, int m1, int u0, From from,
-                                          To to) {
-    const int rows = TH >> a.ushift, r0 = int(threadIdx.x) >> a.ushift;
-    const int u = u0 + (int(threadIdx.x) & ((1 << a.ushift) - 1));
+__device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b, int h, int m0, int m1, int u0,
+                                          int ushift, From from, To to) {
+    const int rows = TH >> ushift, r0 = int(threadIdx.x) >> ushift;
+    const int u = u0 + (int(threadIdx.x) & ((1 << ushift) - 1));
     const int left = u < a.c.d / 8 ? m1 - r0 : 0;  // rows from m on are this thread's while m < left
     struct Chunk {
         u32x4_t x[kMoveUnroll];
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(kMoveThreads, 4) void evict_fill_kernel(EvictArgs a
     const int m0 = block * per;
     if (m0 >= holes) return;
     char* pool = const_cast<char*>(sl < a.slices ? a.c.k : a.c.v);
-    move_rows<kMoveThreads, false>(a, pool, b, h, m0, min(holes, m0 + per), (sl % a.slices) << a.ushift,
+    move_rows<kMoveThreads, false>(a, pool, b, h, m0, min(holes, m0 + per), (sl % a.slices) << a.ushift, a.ushift,
                      [&](int i) { return src[i]; }, [&](int i) { return dst[i]; });
 }
 
@@ -521,7 +523,7 @@ __global__ __launch_bounds__(TH, TH == kMoveThreads ? 4 : 1) void evict_shift_ke
     if (a.filled && by >= recent) {
         // their places and sources do not meet: any order
         for (int m0 = holes + block * per; m0 < moves; m0 += a.blocks * per)
-            move_rows<TH, false>(a, pool, b, h, m0, min(moves, m0 + per), u0, from, to);
+            move_rows<TH, false>(a, pool, b, h, m0, min(moves, m0 + per), u0, a.ushift, from, to);
     } else if (a.filled && by >= rows) {
         // row i goes where row i - by was read: the rows of one remainder
         // modulo `by` are a thread's, in ascending order, reads first
@@ -547,8 +549,12 @@ __global__ __launch_bounds__(TH, TH == kMoveThreads ? 4 : 1) void evict_shift_ke
                 for (int r = 0; r < kMoveUnroll; r++)
                     if (i + int64_t(r) * by < recent) *reinterpret_cast<u32x4_t*>(pool + go[r]) = x[r];
             }
-    } else if (block == 0) {
-        move_rows<TH, true>(a, pool, b, h, a.filled ? holes : 0, moves, u0, from, to);
+    } else {
+        // one workgroup a slice, or two with half of it each
+        const int halves = a.blocks > 1 && a.ushift > 0;
+        if (block > halves) return;
+        const int ushift = a.ushift - halves;
+        move_rows<TH, true>(a, pool, b, h, a.filled ? holes : 0, moves, u0 + (block << ushift), ushift, from, to);
     }
 }
 
@@ -618,10 +624,11 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
     a.count = reinterpret_cast<int32_t*>(ws->partials);
     a.dst = a.count + int64_t(step) * a.c.hk;
     a.src = a.dst + int64_t(step) * a.c.hk * m;
-    // a workgroup's slice of the rows: 64 bytes, so that an ordered move has
-    // as many workgroups as a row's length allows
+    // a workgroup's slice of the rows: 128 bytes, a cache line (16 x 4 heads of
+    // 2112 tokens 16.3 us, 64 x 2 of 8000 of which 7000 move down 231; with 64
+    // bytes, which read every line twice, 19.0 and 287)
     const int row_units = a.c.d / 8;
-    a.ushift = row_units >= 4 ? 2 : (row_units >= 2 ? 1 : 0);
+    a.ushift = row_units >= 8 ? 3 : row_units >= 4 ? 2 : (row_units >= 2 ? 1 : 0);
     a.slices = (row_units + (1 << a.ushift) - 1) >> a.ushift;
     const int64_t per = (iq::kMoveThreads >> a.ushift) * iq::kMoveUnroll;
     iq::allow_big_lds<iq::evict_plan_kernel>();
@@ -632,9 +639,10 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
         iq::evict_plan_kernel<<<dim3(hk, nz), iq::kPlanThreads, (iq::kBins + held) * 4, s>>>(a);
         // (a cache that cannot hold more than the budget has nothing to move)
         if (a.t.cap <= budget) continue;
-        // fewer than two workgroups a CU in an ordered move: spread over blocks of rows
+        // fewer than two workgroups a CU in an ordered move, and more than a
+        // chunk or two of rows: spread over blocks of rows
         const int64_t wgs = int64_t(2) * a.slices * a.c.hk * nb;
-        a.filled = wgs < 2 * iq::device_cu_count() && m > per;
+        a.filled = wgs < 2 * iq::device_cu_count() && (m > per || recent > 4 * per);
         a.blocks = 1;
         if (a.filled) {
             a.blocks = int(std::min<int64_t>((m + per - 1) / per, 65536));

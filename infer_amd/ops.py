@@ -9,6 +9,9 @@ Mirrors, with the same names, argument meaning and order:
   quantize                        src/quant.h:61 (on the device here)
   upload_q                        kernels/model_gpu_internal.cuh:67-83
 
+and, without counterparts in the reference's quantised path, the operators of
+a decode step around it: KvCache, kv_append, attn_decode, kv_evict, logprobs.
+
 Every call goes through the C ABI of include/iq.h (ctypes); torch is used
 only for device memory and the current stream.  Launches are asynchronous
 on torch's current stream, like the reference's (ops.cuh:3-7).  Where the
