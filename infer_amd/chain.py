@@ -236,7 +236,7 @@ class CachedDecodeStep:
         None: the ids already in self.ids) are added to the caches, attend to
         them and leave their logits; lens and positions move on by one.  A
         sequence whose pages are full, or whose next page id is negative, keeps
-        its cache; a full one's logits are NaN."""
+        its cache, and its logits are NaN."""
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.step(token_id)

@@ -54,6 +54,7 @@ struct AttnArgs {
     int ht;           // 16-head tiles of a group
     uint32_t nh;      // hk * ht
     uint32_t target;
+    int lines;        // heads share cache lines
     float mul;        // scale * log2(e): scores in powers of two
     float* ml;        // [partials][16][2]: a chunk's maximum and sum of every head
     float* part;      // [partials][16][d]
@@ -174,8 +175,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     __shared__ float wm[kAttnWaves][16], wl[kAttnWaves][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
     Item it;
-    const uint32_t hidx = blockIdx.x % a.nh;
-    if (!find_item(a, blockIdx.x / a.nh, &it)) return;
+    // Heads that share cache lines (see the host side) go to one XCD for a
+    // chunk: workgroups are dealt to the 8 of them in turn.
+    const uint32_t turn = a.lines ? 8 : 1, round = blockIdx.x / (turn * a.nh), in = blockIdx.x % (turn * a.nh);
+    const uint32_t hidx = in / turn;
+    if (!find_item(a, round * turn + in % turn, &it)) return;
     const int b = it.b, n = it.n, d = a.c.d;
     const int j = int(hidx) / a.ht, h0 = int(hidx) % a.ht * 16, gh = min(16, a.group - h0);
     float* out = a.out + (int64_t(b) * a.hq + j * a.group + h0) * d;
@@ -573,6 +577,11 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
     // 131072 tokens / 32 sequences of up to 8192: 1 a CU 64.7 / 29.2 us, 2 63.7
     // / 26.7, 3 71.3 / 30.6, 4 70.1 / 31.1.
     a.target = uint32_t((a.c.d <= 32 ? 4 : a.c.d <= 64 ? 3 : a.c.d <= 128 ? 2 : 1) * iq::device_cu_count());
+    // Neighbouring heads' rows meet in a cache line, or several head tiles read
+    // the same rows: one XCD's L2 then serves them (8 sequences of 16384, 8 heads
+    // of 32: 49.7 -> 38.8 us; of 8192, heads of 80: 50.1 -> 44.6).  Whole lines
+    // are better spread (131072 tokens, 4 heads of 128: 61.9 and 64.0).
+    a.lines = a.nh > 1 && (a.ht > 1 || 2 * a.c.hstr % 128 != 0);
     const int64_t capt = iq::attn_tiles(a.t.cap);
     // the workspace's partial sums: plan | final (maximum, sum) | chunks' | rows;
     // its GEMM operand area: the scores that the weights are made of
@@ -593,7 +602,8 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
         a.out = out + b0 * row;
         a.t.table = table + b0 * table_ld;
         a.t.lens = lens + b0;
-        const int64_t grid = iq::attn_max_items(a.B, a.nh, a.t.cap, a.target);
+        int64_t grid = iq::attn_max_items(a.B, a.nh, a.t.cap, a.target);
+        if (a.lines) grid = (grid / a.nh + 7) / 8 * 8 * a.nh;
         if (kv->type == IQ_KV_BF16) iq::launch_attn<IQ_KV_BF16>(a, unsigned(grid), s);
         else iq::launch_attn<IQ_KV_F16>(a, unsigned(grid), s);
         // (a sequence has at most target / nh chunks and one more)

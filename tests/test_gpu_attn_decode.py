@@ -205,6 +205,40 @@ def test_pool_past_32_bits():
     assert torch.equal(out, ref)
 
 
+def test_any_alignment_and_table_stride():
+    """q, out and weights 4 bytes past a 16-byte border, table rows inside a
+    wider tensor, the cache a slice of a larger pool: the same bits."""
+    rng = np.random.default_rng(13)
+    pg = Paged(rng, [700, 45, 2100], 2, 96, 24, HF)
+    q = torch.from_numpy(rng.standard_normal((3, 10, 96)).astype(np.float32)).cuda()
+    cap = pg.width * 24
+    w = torch.rand(3, 2, cap, device="cuda")
+    w1 = torch.empty(w.numel() + 1, device="cuda")[1:].view_as(w).copy_(w)
+    ref = ops.attn_decode(q, pg.cache, pg.table, pg.lens_t, weights=w)
+    q1 = torch.empty(q.numel() + 1, device="cuda")[1:].view_as(q).copy_(q)
+    out = torch.empty(q.numel() + 3, device="cuda")[3:].view_as(q)
+    table = torch.full((3, pg.width + 9), -1, dtype=torch.int32, device="cuda")
+    table[:, 5:5 + pg.width] = pg.table + 2
+    n = pg.cache.pages
+    pool = [torch.empty(n + 5, 24, 2, 96, dtype=HF, device="cuda") for _ in range(2)]
+    pool[0][2:2 + n], pool[1][2:2 + n] = pg.cache.k, pg.cache.v
+    ops.attn_decode(q1, ops.KvCache(*pool), table[:, 5:5 + pg.width], pg.lens_t, out=out, weights=w1)
+    assert torch.equal(out, ref) and torch.equal(w1, w)
+
+
+def test_shared_pages():
+    """Two sequences with a common prefix in the same pages."""
+    rng = np.random.default_rng(14)
+    pg = Paged(rng, [640, 800], 2, 64, 16, BF)
+    table = pg.table.clone()
+    table[0, :40] = pg.table[1, :40]
+    q = torch.from_numpy(rng.standard_normal((2, 6, 64)).astype(np.float32)).cuda()
+    q[0] = q[1]
+    lens = torch.tensor([640, 640], dtype=torch.int32, device="cuda")
+    out = ops.attn_decode(q, pg.cache, table, lens)
+    assert torch.equal(out[0], out[1])
+
+
 def test_longest_sequence():
     """2^31 - 65536 tokens, the most that a table can hold, in one page of
     65536 slots that every table entry names: the softmax over equal runs is

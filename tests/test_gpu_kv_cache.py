@@ -79,6 +79,20 @@ def test_append_cache_only():
     check_append(6, HF, 9, 0, 2, 64, 64, 16, 500)
 
 
+def test_append_any_alignment_of_the_inputs():
+    rng = np.random.default_rng(9)
+    T, hq, hk, d = 37, 6, 2, 64
+    dev = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()  # noqa: E731
+    q, k, v = dev(T, hq, d), dev(T, hk, d), dev(T, hk, d)
+    pos, slots = torch.arange(T, device="cuda") * 1000, torch.randperm(64, device="cuda")[:T]
+    fr = ops.rope_freqs(d, 1e4)
+    odd = lambda t: torch.empty(t.numel() + 1, device="cuda")[1:].view_as(t).copy_(t)  # noqa: E731
+    a, b = (ops.alloc_kv(4, 16, hk, d) for _ in range(2))
+    qa = ops.kv_append(q, k, v, pos, slots, fr, a)
+    qb = ops.kv_append(odd(q), odd(k), odd(v), pos, slots, fr, b, q_out=odd(q))
+    assert torch.equal(qa, qb) and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+
+
 def test_append_rounds_and_keeps_specials():
     cache = ops.alloc_kv(1, 4, 1, 8, HF)
     x = torch.tensor([65519.0, 65520.0, float("nan"), float("-inf"), -0.0, 2.0 ** -25, 2.0 ** -24, 1 + 2.0 ** -11],
@@ -146,6 +160,26 @@ def test_evict_one_by_one():
     """A full window whose rows all move down by one."""
     check_evict(1, BF, [1025, 1025], 2, 128, 16, 1024, 1024)
     check_evict(2, BF, [1025, 1025], 2, 128, 16, 1024, 512)
+
+
+def test_evict_uses_only_the_batch_table_columns():
+    """Table rows inside a wider tensor, sums 4 bytes past a 16-byte border:
+    the same result."""
+    rng = np.random.default_rng(12)
+    pg = Paged(rng, [300, 80], 2, 64, 16, BF)
+    k0, v0 = pg.cache.k.clone(), pg.cache.v.clone()
+    w = torch.rand(2, 2, pg.width * 16, device="cuda")
+    w1 = torch.empty(w.numel() + 1, device="cuda")[1:].view_as(w).copy_(w)
+    ops.kv_evict(pg.cache, pg.table, pg.lens_t, w, 60, 13)
+    k1, v1 = pg.cache.k.clone(), pg.cache.v.clone()
+    pg.cache.k.copy_(k0)
+    pg.cache.v.copy_(v0)
+    table = torch.full((2, pg.width + 6), -1, dtype=torch.int32, device="cuda")
+    table[:, 2:2 + pg.width] = pg.table
+    ops.kv_evict(pg.cache, table[:, 2:2 + pg.width], pg.lens_t, w1, 60, 13)
+    bits = lambda t: t.view(torch.int16)  # noqa: E731
+    assert torch.equal(w, w1)
+    assert torch.equal(bits(pg.cache.k), bits(k1)) and torch.equal(bits(pg.cache.v), bits(v1))
 
 
 def test_evict_many_sequences():
