@@ -63,6 +63,10 @@ struct AttnArgs {
     float* fin;       // [B][hq][2]: maximum and sum of every head, for the weights
 };
 
+// The maximum of no scores: finite, so that scores of -inf (products past
+// fp32's range) and runs without scores count nothing instead of giving NaN.
+constexpr float kNone = -3.4e38f;
+
 struct Item {
     int b, n;            // sequence and its length (as given)
     uint32_t j, c, chunks, first;  // chunk, tiles of a chunk, chunks of the sequence, its first partial
@@ -274,7 +278,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     float4_t o[VT];
 #pragma unroll
     for (int i = 0; i < VT; i++) o[i] = float4_t{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
+    float m = kNone, l = 0.0f;
     float* sc = a.sc ? a.sc + ((int64_t(b) * a.c.hk + j) * a.t.cap) * a.group + h0 + col : nullptr;
 
     int64_t off_next = wave + kAttnWaves < ntiles ? row_offset(wave + kAttnWaves) : 0;
@@ -433,7 +437,7 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, int b, int head) {
     int w = 2;  // 16-byte pieces of a row, to a power of two
     while (w * 4 < d) w *= 2;
     const int e = tid % w * 4, run = tid / w, runs = TH / w, n = int(pl.x);
-    float M = -3.4e38f, L = 0.0f;  // (finite: a run may be without chunks)
+    float M = kNone, L = 0.0f;
     float4_t x = {0, 0, 0, 0};
     auto add = [&](float2 v, float4_t y) {
         const float mn = fmaxf(M, v.x), f = __builtin_amdgcn_exp2f(M - mn), k = __builtin_amdgcn_exp2f(v.x - mn);

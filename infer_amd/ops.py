@@ -414,6 +414,8 @@ def kv_append(q, k, v, positions, slots, freqs, cache, q_out=None, stream=None):
     _need(what, "v", v, torch.float32, T * cache.kv_heads * d)
     rot = 0
     if freqs is not None:
+        if positions is None:
+            raise ValueError(f"{what}: freqs need positions")
         _need(what, "freqs", freqs, torch.float64)
         _need(what, "positions", positions, torch.int64, T)
         rot = 2 * freqs.numel()

@@ -101,7 +101,7 @@ def cache(device="cpu", **kw):
 
 
 def test_python_checks():
-    f, i32, i64 = torch.float32, torch.int32, torch.int64
+    i32, i64 = torch.int32, torch.int64
     c = cache()
     q, k, pos = torch.zeros(3, 4, 64), torch.zeros(3, 2, 64), torch.zeros(3, dtype=i64)
     fr = ops.rope_freqs(64, 1e6, device="cpu")
@@ -118,6 +118,8 @@ def test_python_checks():
         a.update(bad)
         with pytest.raises(ValueError):
             ops.kv_append(*a.values(), c)
+    with pytest.raises(ValueError, match="positions"):
+        ops.kv_append(q, k, k, None, pos, fr, c)
     table, lens, w = torch.zeros(3, 5, dtype=i32), torch.zeros(3, dtype=i32), torch.zeros(3, 2, 80)
     with pytest.raises(ValueError, match="current CUDA device"):
         ops.attn_decode(q, c, table, lens, weights=w)
@@ -145,7 +147,6 @@ def test_python_checks():
             ops.logprobs(**a)
     with pytest.raises(TypeError):
         ops.logprobs(x, torch.zeros(4, dtype=i32), out=small)
-    assert f is torch.float32
 
 
 def test_python_caches():

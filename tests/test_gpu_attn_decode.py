@@ -116,6 +116,33 @@ def test_scales_and_large_scores(dtype):
     run_case(109, dtype, 7, 1, 128, 16, [400, 33], scale=1e-5, qsd=1e4)
 
 
+@pytest.mark.parametrize("dtype,big", [(BF, 1e10), (HF, 6e4)])
+def test_scores_below_the_range(dtype, big):
+    """Products past fp32's range: those tokens' weight is 0, whole tiles and
+    chunks of them included."""
+    rng = np.random.default_rng(15)
+    pg = Paged(rng, [3000, 700], 2, 64, 16, dtype)
+    for b, n in enumerate(pg.lens):
+        skip = np.arange(n) % 977 != 650
+        K = torch.zeros(n, 2, 64, dtype=dtype)
+        K[torch.from_numpy(skip)] = -big
+        K[torch.from_numpy(~skip)] = 0.0
+        p, s = pg.where(b, np.arange(n))
+        pg.cache.k[p.cuda(), s.cuda()] = K.cuda()
+        pg.K[b] = K
+    q = torch.full((2, 6, 64), 3e38 if dtype == HF else 1e32, device="cuda")
+    w = torch.zeros(2, 2, pg.width * 16, device="cuda")
+    out = ops.attn_decode(q, pg.cache, pg.table, pg.lens_t, weights=w)
+    for b, n in enumerate(pg.lens):
+        live = np.flatnonzero(np.arange(n) % 977 == 650)
+        V = pg.V[b].double().numpy()[live]
+        for h in range(6):
+            assert np.allclose(out[b, h].cpu().numpy(), V[:, h // 3].mean(0), rtol=0, atol=64 * EPS32 * np.abs(V).max())
+        want = np.zeros((2, n))
+        want[:, live] = 3.0 / len(live)
+        assert np.allclose(w[b, :, :n].cpu().numpy(), want, rtol=64 * EPS32, atol=0)
+
+
 def small(rng, lens=(40, 70, 100), dtype=BF):
     pg = Paged(rng, lens, 2, 64, 16, dtype)
     q = torch.from_numpy(rng.standard_normal((len(lens), 6, 64)).astype(np.float32)).cuda()
