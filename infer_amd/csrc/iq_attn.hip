@@ -345,7 +345,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
         T::cut(p, pt);
 #pragma unroll
         for (int v = 0; v < VT; v++) {
-            if (v * 16 >= d) break;
+            if (v * 16 >= d) continue;
             // rows 4g..4g+3 of either half: lane 4r + c of 16 gives row r's
             // 8-byte piece c, lane i gets the 4 rows' value of column i
             s16x8_t av;

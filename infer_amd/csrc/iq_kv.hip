@@ -349,7 +349,6 @@ __global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(EvictArgs a) {
         };
         // (a block has at most 32768 of either: two counts in a word)
         uint32_t total, count = 0;
-#pragma unroll 4
         for (int r = 0; r < rounds; r++) {
             uint64_t to, from;
             masks(r, to, from);
@@ -359,7 +358,6 @@ __global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(EvictArgs a) {
         at = uint32_t(__builtin_amdgcn_readfirstlane(int(at)));
         int32_t* hole = dst + holes + (at & 0xffffu);
         int32_t* high = src + highs + (at >> 16);
-#pragma unroll 2
         for (int r = 0; r < rounds; r++) {
             const int i = w0 + r * 64 + lane;
             uint64_t to, from;

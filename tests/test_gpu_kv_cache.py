@@ -195,6 +195,13 @@ def test_evict_ties_and_specials():
     check_evict(7, BF, [900, 333], 2, 64, 16, 700, 30, sums=lambda r, w: np.full_like(w, np.nan))
 
 
+def test_evict_ties_in_long_rows():
+    """More sums than a workgroup holds at once, most of them equal."""
+    check_evict(8, BF, [70001, 33000], 1, 8, 64, 40000, 100, sums=lambda r, w: r.integers(0, 3, w.shape) * 0.5)
+    check_evict(9, BF, [70001, 33000], 1, 8, 64, 20000, 0, sums=lambda r, w: np.zeros_like(w))
+    check_evict(10, BF, [98304], 1, 8, 64, 65536, 1, sums=lambda r, w: r.standard_normal(w.shape))
+
+
 def test_evict_refused_rows_are_left():
     rng = np.random.default_rng(8)
     pg = Paged(rng, [90, 90, 90, 90], 2, 64, 16, BF)
