@@ -578,8 +578,9 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
     a.nh = uint32_t(a.c.hk * a.ht);
     // as many work items as run at once: 4, 3, 2 or 1 workgroups a CU by the
     // registers (d <= 64) and the LDS of an instance.  Measured for d = 128 on
-    // 131072 tokens / 32 sequences of up to 8192: 1 a CU 64.7 / 29.2 us, 2 63.7
-    // / 26.7, 3 71.3 / 30.6, 4 70.1 / 31.1.
+    // 131072 tokens / 32 sequences of up to 8192: 1 a CU 69.9 / 30.4 us, 2 61.8
+    // / 24.7, 3 69.1 / 27.8, 4 66.0 / 29.4; for d = 64 (24 of up to 2047, 16
+    // heads) 18.1, 19.0, 17.2, 18.8.
     a.target = uint32_t((a.c.d <= 32 ? 4 : a.c.d <= 64 ? 3 : a.c.d <= 128 ? 2 : 1) * iq::device_cu_count());
     // Neighbouring heads' rows meet in a cache line, or several head tiles read
     // the same rows: one XCD's L2 then serves them (8 sequences of 16384, 8 heads

@@ -487,8 +487,8 @@ int iq_logprobs(const float* logits, int64_t ld, int64_t T, int64_t V, const int
     if (V > 0x7fffffff - 65536 || T > 0x7fffffff) return IQ_ETOOLARGE;
     iq::LogprobArgs a{logits, ld, uint32_t(V), tokens, top, logprob, entropy, top_ids, top_logprobs};
     // workgroups for every CU, parts of four batches at least (32 rows of 152064,
-    // top 20, in 8 / 19 / 38 / 75 parts: 26.5 / 21.5 / 20.3 / 27.2 us; 999 rows,
-    // no list, in 1 / 2 / 4: 139.8 / 143.5 / 145.3)
+    // top 20, in 4 / 8 / 19 / 38 parts: 38.6 / 27.1 / 21.8 / 19.3 us; 999 rows, no
+    // list, in 1 / 2 / 4: 138.3 / 143.5 / 145.6)
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t target = (top ? iq::kPerCuTop : iq::kPerCu) * int64_t(iq::device_cu_count());
     int64_t chunks = std::max<int64_t>(1, std::min(target / T, (V + 4095) / 4096));
