@@ -395,7 +395,8 @@ __device__ __forceinline__ void kv_offsets(const KvView& c, const KvTable& t, in
 
 constexpr int kMoveThreads = 256, kMoveUnroll = 4;
 
-// Moves rows [m0, m1) of a list (m1 - m0 at most 2^31 less a chunk), a
+// Moves rows [m0, m1) of a list (m1 - m0 at most 2^31 less a chunk; none:
+// nothing is read, a list's entries before its first are not its own), a
 // slice's 16-byte units of each from `u0` on, a chunk of 4 units a thread at a
 // time: read, then written.  ORDERED: no thread writes a chunk before all have
 // its values; the next chunk is requested before this one is written (the
@@ -404,6 +405,7 @@ constexpr int kMoveThreads = 256, kMoveUnroll = 4;
 template <int TH, bool ORDERED, class From, class To>
 __device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b, int h, int m0, int m1, int u0,
                                           int ushift, From from, To to) {
+    if (m0 >= m1) return;  // (the same for the whole workgroup: no barrier is left out by some)
     const int rows = TH >> ushift, r0 = int(threadIdx.x) >> ushift;
     const int u = u0 + (int(threadIdx.x) & ((1 << ushift) - 1));
     const int left = u < a.c.d / 8 ? m1 - r0 : 0;  // rows from m on are this thread's while m < left
@@ -481,7 +483,8 @@ __global__ __launch_bounds__(TH, TH == kMoveThreads ? 4 : 1) void evict_shift_ke
     const int n = a.t.lens[b], recent = int(a.recent), cut = int(a.budget) - recent, tid = threadIdx.x;
     const int32_t* dst = a.dst + row * a.m;
     const int32_t* src = a.src + row * a.m;
-    // (the lists have an entry at least: the load needs no branch)
+    // (past the free places entry 0 is named, which is there to be read even
+    // where no place is free; it is not used then)
     auto from = [&](int i) {
         const int s = src[i < holes ? i : 0];
         return i < holes ? s : n - recent + (i - holes);
