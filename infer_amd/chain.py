@@ -170,6 +170,17 @@ class DecodeStep:
         return n + self.model["head"].nbytes()
 
 
+def next_slots(lens, table, page_size):
+    """The cache slot (int64, page * page_size + slot) behind each sequence's
+    first lens[b] tokens; -1 where there is none: a full table, a page id below
+    0, a length below 0."""
+    capacity = table.shape[1] * page_size
+    at = lens.clamp(0, capacity - 1)  # (of any length: the index has to lie in the table)
+    page = table.gather(1, (at // page_size).long()[:, None])[:, 0]
+    slot = page.long() * page_size + at % page_size
+    return slot.masked_fill((lens != at) | (page < 0), -1)
+
+
 class CachedDecodeStep:
     """One decode step of B sequences over paged key/value caches, one
     ops.KvCache a layer: every sequence's next token, at the position and
@@ -236,7 +247,8 @@ class CachedDecodeStep:
         None: the ids already in self.ids) are added to the caches, attend to
         them and leave their logits; lens and positions move on by one.  A
         sequence whose pages are full, or whose next page id is negative, keeps
-        its cache, and its logits are NaN."""
+        its cache, and its logits are NaN; likewise an idle row, whose length is
+        below 0 and stays so."""
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.step(token_id)
@@ -245,11 +257,8 @@ class CachedDecodeStep:
                 self.ids.fill_(int(token_id))
             else:
                 self.ids.copy_(torch.tensor([int(t) for t in token_id], dtype=torch.int64))
-        at = self.lens.clamp(max=self.capacity - 1)
-        page = self.table.gather(1, (at // self.page).long()[:, None])[:, 0]
-        slot = page.long() * self.page + at % self.page
-        self.slots.copy_(torch.where((self.lens < self.capacity) & (page >= 0), slot, torch.full_like(slot, -1)))
-        self.lens.add_(1)
+        self.slots.copy_(next_slots(self.lens, self.table, self.page))
+        self.lens.add_(self.lens >= 0)
         ops.launch_embedding_q(self.model["embed"], self.ids, self.rows, self.model["cfg"]["hidden"], self.h0)
         self.chains[0].run()
         for li, b in enumerate(self.per_layer):
