@@ -170,15 +170,15 @@ class DecodeStep:
         return n + self.model["head"].nbytes()
 
 
-def next_slots(lens, table, page_size):
+def next_slots(lens, table, page_size, pages=2 ** 31):
     """The cache slot (int64, page * page_size + slot) behind each sequence's
-    first lens[b] tokens; -1 where there is none: a full table, a page id below
-    0, a length below 0."""
+    first lens[b] tokens; -1 where there is none: a full table, a page id
+    outside [0, pages), a length below 0."""
     capacity = table.shape[1] * page_size
     at = lens.clamp(0, capacity - 1)  # (of any length: the index has to lie in the table)
-    page = table.gather(1, (at // page_size).long()[:, None])[:, 0]
-    slot = page.long() * page_size + at % page_size
-    return slot.masked_fill((lens != at) | (page < 0), -1)
+    page = table.gather(1, (at // page_size).long()[:, None])[:, 0].long()
+    slot = page * page_size + at % page_size
+    return slot.masked_fill((lens != at) | (page < 0) | (page >= pages), -1)
 
 
 class CachedDecodeStep:
@@ -193,9 +193,12 @@ class CachedDecodeStep:
     layer [B, kv_heads, pages * page_size], for evict().
 
     Device state, which the caller may set between steps: lens (int32 [B],
-    tokens in the cache), positions (int64 [B], of the next token; they part
-    from lens after an eviction).  step() issues only device work, so it can
-    be captured into a graph (after ops.init on the capturing stream)."""
+    tokens of each sequence), positions (int64 [B], of the next token; they
+    part from lens after an eviction), and for a new sequence in a row its
+    weights, to 0.  held (int32 [B]) is how many of the tokens lie in the cache:
+    lens, less those that found no place (see step) since the caller or evict()
+    last set lens.  step() issues only device work, so it can be captured into
+    a graph (after ops.init on the capturing stream)."""
 
     def __init__(self, model, caches, table, weights=False, device="cuda"):
         c = model["cfg"]
@@ -208,6 +211,7 @@ class CachedDecodeStep:
         B = self.rows = table.shape[0]
         self.model, self.caches, self.table = model, list(caches), table
         self.page = caches[0].page_size
+        self.pages = min(k.pages for k in caches)
         self.capacity = table.shape[1] * self.page
         qo, kvo = nh * hd, nkv * hd
         sizes = [H] + [qo, kvo, kvo, qo, qo, H, I, H] * L + [V]
@@ -216,6 +220,9 @@ class CachedDecodeStep:
         self.h0 = next(vs)
         self.ids = torch.zeros(B, dtype=torch.int64, device=device)
         self.lens = torch.zeros(B, dtype=torch.int32, device=device)
+        self.held = torch.zeros(B, dtype=torch.int32, device=device)
+        self._left = torch.zeros(B, dtype=torch.int32, device=device)  # lens as step() or evict() left it
+        self._attend = torch.zeros(B, dtype=torch.int32, device=device)
         self.positions = torch.zeros(B, dtype=torch.int64, device=device)
         self.slots = torch.full((B,), -1, dtype=torch.int64, device=device)
         self.freqs = ops.rope_freqs(hd, c["theta"], device)
@@ -242,13 +249,20 @@ class CachedDecodeStep:
         self.chains.append(Chain(stages))
         self.h_last = h
 
+    def _held_now(self):
+        """held, or lens where the caller has set it since."""
+        return torch.where(self.lens == self._left, self.held, self.lens)
+
     def step(self, token_id=None, stream=None):
         """The tokens `token_id` (an int for every row, or a sequence of B ints;
         None: the ids already in self.ids) are added to the caches, attend to
-        them and leave their logits; lens and positions move on by one.  A
-        sequence whose pages are full, or whose next page id is negative, keeps
-        its cache, and its logits are NaN; likewise an idle row, whose length is
-        below 0 and stays so."""
+        them and leave their logits; lens, held and positions move on by one.
+        A token finds no place where its sequence's pages are full or the next
+        page id is none of the pool's: the sequence keeps its cache, its weights
+        and its position, its logits are NaN, and of the three only lens counts
+        the token.  With a page, or after evict(), the next step goes on behind
+        the tokens in the cache.  A row whose length is below 0 is idle: NaN
+        logits, and nothing of it changes."""
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.step(token_id)
@@ -257,26 +271,36 @@ class CachedDecodeStep:
                 self.ids.fill_(int(token_id))
             else:
                 self.ids.copy_(torch.tensor([int(t) for t in token_id], dtype=torch.int64))
-        self.slots.copy_(next_slots(self.lens, self.table, self.page))
+        held = self._held_now()
+        self.slots.copy_(next_slots(held, self.table, self.page, self.pages))
+        stored = self.slots >= 0
+        torch.add(held, stored, out=self.held)
+        # (a row without its token attends to nothing: no length, so that its
+        # output is NaN and its weights stay)
+        self._attend.copy_(self.held.masked_fill(~stored, -1))
         self.lens.add_(self.lens >= 0)
+        self._left.copy_(self.lens)
         ops.launch_embedding_q(self.model["embed"], self.ids, self.rows, self.model["cfg"]["hidden"], self.h0)
         self.chains[0].run()
         for li, b in enumerate(self.per_layer):
             ops.kv_append(b["q"], b["k"], b["v"], self.positions, self.slots, self.freqs, self.caches[li],
                           q_out=b["q_rot"])
-            ops.attn_decode(b["q_rot"], self.caches[li], self.table, self.lens, out=b["attn"],
+            ops.attn_decode(b["q_rot"], self.caches[li], self.table, self._attend, out=b["attn"],
                             weights=self.weights[li] if self.weights else None)
             self.chains[li + 1].run()
-        self.positions.add_(1)
+        self.positions.add_(stored)
 
     def evict(self, budget, recent):
         """Every layer's caches cut to `budget` tokens a sequence by the weights
-        they have received (ops.kv_evict); the pages past them are free."""
+        they have received (ops.kv_evict); the pages past them are free, and
+        lens and held are what is left."""
         if not self.weights:
             raise ValueError("CachedDecodeStep.evict: made without weights")
+        self.held.copy_(self._held_now())
         for cache, w in zip(self.caches, self.weights):
-            ops.kv_evict(cache, self.table, self.lens, w, budget, recent, new_lens=self._new_lens)
-        self.lens.copy_(self._new_lens)
+            ops.kv_evict(cache, self.table, self.held, w, budget, recent, new_lens=self._new_lens)
+        for t in (self.held, self.lens, self._left):
+            t.copy_(self._new_lens)
 
     def logprobs(self, tokens=None, top=0, out=None):
         """Log probabilities, entropy and top alternatives of the last step's

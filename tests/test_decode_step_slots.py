@@ -6,11 +6,11 @@ import torch
 from infer_amd.chain import next_slots
 
 
-def plain(lens, table, page):
+def plain(lens, table, page, pages=2 ** 31):
     got = []
     for b, n in enumerate(lens):
         full = n < 0 or n >= len(table[b]) * page
-        got.append(-1 if full or table[b][n // page] < 0 else table[b][n // page] * page + n % page)
+        got.append(-1 if full or not 0 <= table[b][n // page] < pages else table[b][n // page] * page + n % page)
     return got
 
 
@@ -28,3 +28,10 @@ def test_slots_in_a_part_of_a_table():
     wide = torch.arange(24, dtype=torch.int32).view(3, 8)
     lens = torch.tensor([0, 9, 31], dtype=torch.int32)
     assert next_slots(lens, wide[:, 2:5], 10).tolist() == [20, 109, -1]
+
+
+def test_pages_outside_the_pool():
+    table = [[3, 8, 9], [9, 0, 2 ** 31 - 1]]
+    for n in range(12):
+        got = next_slots(torch.tensor([n, n]), torch.tensor(table, dtype=torch.int32), 4, 9)
+        assert got.tolist() == plain([n, n], table, 4, 9), n
