@@ -338,7 +338,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            p[i] = __builtin_amdgcn_exp2f(s[i] - (m - T::kUp));
+            // (not s - (m - 12): from 2^26 on m - 12 is rounded to m - 16 and more,
+            // p becomes 2^16, past fp16's range, and the waves' scales differ)
+            const float e = s[i] - m;
+            p[i] = __builtin_amdgcn_exp2f(T::kUp != 0.0f ? e + T::kUp : e);
             l += p[i];
         }
         s16x8_t pt[T::N];
@@ -496,7 +499,7 @@ template <int TH>
 __global__ __launch_bounds__(TH) void attn_weights_kernel(AttnArgs a, float* weights, int64_t wld, float up) {
     constexpr int RUNS = TH / 16;
     __shared__ float2 run_ml[16][RUNS + 1];
-    __shared__ float2 head_ml[16];  // maximum less `up`, 1 / sum
+    __shared__ float2 head_ml[16];  // maximum, 1 / sum
     const int b = blockIdx.y, tid = threadIdx.x;
     if (int(blockIdx.x) < a.hq) {
         join_head<TH>(a, b, blockIdx.x);
@@ -533,10 +536,10 @@ __global__ __launch_bounds__(TH) void attn_weights_kernel(AttnArgs a, float* wei
             M = run_ml[tid][0].x;
             L = run_ml[tid][0].y;
             for (int r = 1; r < runs; r++) add(run_ml[tid][r]);
-            head_ml[tid] = make_float2(M - up, 1.0f / L);
+            head_ml[tid] = make_float2(M, 1.0f / L);
         }
         __syncthreads();
-        for (int i = 0; i < gh; i++) sum += __builtin_amdgcn_exp2f(s[h0 + i] - head_ml[i].x) * head_ml[i].y;
+        for (int i = 0; i < gh; i++) sum += __builtin_amdgcn_exp2f((s[h0 + i] - head_ml[i].x) + up) * head_ml[i].y;
     }
     if (t < n) weights[row * wld + t] += sum;
 }
