@@ -274,8 +274,13 @@ int iq_kv_append(const float* q, const float* k, const float* v, const int64_t* 
  * be at most 20971520 with weights (IQ_ETOOLARGE).
  * A sequence of length 0 gives zeros.  A length below 0 or above max_pages *
  * page_size gives NaN, its weights left as they were.  A page id outside [0,
- * pages) among the sequence's pages, or a non-finite q, key or value, gives
- * NaN to the heads that read it and to the weights made of them. */
+ * pages) among the sequence's pages, a q that is not finite or a key of NaN
+ * gives NaN to the heads that read it and to the weights made of them; a value
+ * that is not finite gives NaN (or its infinity) to the heads.  Scores are fp32
+ * numbers, in powers of 2: one below fp32's range (-inf) weighs nothing, and a
+ * head with no other scores gives zeros and adds nothing to the weights; one
+ * above it (+inf), or made of products past the range with both signs, is like
+ * NaN.  An infinite key gives one or the other. */
 int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t max_pages,
                    const int32_t* lens, int B, int q_heads, float scale, float* out, float* weights,
                    int64_t weights_ld, void* stream);

@@ -67,6 +67,10 @@ struct AttnArgs {
 // fp32's range) and runs without scores count nothing instead of giving NaN.
 constexpr float kNone = -3.4e38f;
 
+// 1 / a head's sum.  It is 0 only where every score is -inf: the head's values
+// are then 0 times 0 (or NaN, where a value is not finite), its weights 0.
+__device__ __forceinline__ float inv_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
 struct Item {
     int b, n;            // sequence and its length (as given)
     uint32_t j, c, chunks, first;  // chunk, tiles of a chunk, chunks of the sequence, its first partial
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
         }
         float* to;
         if (alone) {
-            const float inv = 1.0f / L;
+            const float inv = inv_sum(L);
             x *= inv;
             to = out + h * d + e;
         } else {
@@ -479,7 +483,7 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, int b, int head) {
     }
     if (run == 0 && e < d) {
         for (int r = 1; r < min(TH > 256 ? min(runs, 8) : runs, n); r++) add(ms[r * w + tid], xs[r * w + tid]);
-        const float inv = 1.0f / L;
+        const float inv = inv_sum(L);
         float* out = a.out + (int64_t(b) * a.hq + head) * d + e;
 #pragma unroll
         for (int r = 0; r < 4; r++) out[r] = x[r] * inv;
@@ -536,9 +540,11 @@ __global__ __launch_bounds__(TH) void attn_weights_kernel(AttnArgs a, float* wei
             M = run_ml[tid][0].x;
             L = run_ml[tid][0].y;
             for (int r = 1; r < runs; r++) add(run_ml[tid][r]);
-            head_ml[tid] = make_float2(M, 1.0f / L);
+            head_ml[tid] = make_float2(M, inv_sum(L));
         }
         __syncthreads();
+        // (2^(score - maximum) of a head whose sum is 0: the maximum is kNone, the
+        // scores -inf, 2^-inf = 0)
         for (int i = 0; i < gh; i++) sum += __builtin_amdgcn_exp2f((s[h0 + i] - head_ml[i].x) + up) * head_ml[i].y;
     }
     if (t < n) weights[row * wld + t] += sum;

@@ -41,3 +41,52 @@ def test_large_equal_scores(dtype, lens):
             want = np.where(live, 3.0 / live.sum(), 0.0)
             # exp and 1 / sum to a step each, three additions
             assert np.all(np.abs(w[b, 0, :m].cpu().double().numpy() - want) <= 8 * EPS32 * want), (e, b)
+
+
+@pytest.mark.parametrize("dtype,big,qbig", [(BF, 1e10, 1e32), (HF, 6e4, 3e38)])
+@pytest.mark.parametrize("lens", [[1, 33, 100, 127], [3000, 700], [20000]])
+def test_no_score_in_range(dtype, big, qbig, lens):
+    """Heads all of whose scores lie below fp32's range: zeros, and nothing
+    added to the weights, in one chunk and in several.  The third head of each
+    three has equal scores and is the mean of the values."""
+    rng = np.random.default_rng(22)
+    pg = Paged(rng, lens, 2, 64, 16, dtype)
+    for b, n in enumerate(lens):
+        set_keys(pg, b, np.full(n, -big))
+    q = torch.full((len(lens), 6, 64), qbig, device="cuda")
+    q[:, 2::3] = 0.0
+    w0 = torch.rand(len(lens), 2, pg.width * 16, device="cuda")
+    w = w0.clone()
+    for weights in (None, w):
+        out = ops.attn_decode(q, pg.cache, pg.table, pg.lens_t, weights=weights).cpu()
+        for b, n in enumerate(lens):
+            V = pg.V[b].double().numpy()
+            for h in range(6):
+                if h % 3 < 2:
+                    assert torch.all(out[b, h] == 0), (b, h, out[b, h, :3])
+                else:
+                    err = np.abs(out[b, h].double().numpy() - V[:, h // 3].mean(0))
+                    assert np.all(err <= (n + 4) * EPS32 * np.abs(V[:, h // 3]).mean(0))
+    for b, n in enumerate(lens):
+        want = w0[b, :, :n].double() + 1.0 / n
+        assert torch.all((w[b, :, :n].double() - want).abs() <= EPS32 * want + 4 * EPS32 / n)
+        assert torch.equal(w[b, :, n:], w0[b, :, n:])
+
+
+def test_no_score_in_range_keeps_nan():
+    """A page that is none still gives NaN to such a head and to its weights,
+    a value that is NaN to the head."""
+    rng = np.random.default_rng(23)
+    pg = Paged(rng, [300, 300], 1, 64, 16, BF)
+    for b in range(2):
+        set_keys(pg, b, np.full(300, -1e10))
+    q = torch.full((2, 2, 64), 1e32, device="cuda")
+    table = pg.table.clone()
+    table[1, 7] = -1
+    w = torch.zeros(2, 1, pg.width * 16, device="cuda")
+    out = ops.attn_decode(q, pg.cache, table, pg.lens_t, weights=w)
+    assert torch.all(out[0] == 0) and torch.isnan(out[1]).all()
+    assert torch.all(w[0] == 0) and torch.isnan(w[1, 0, :300]).all()
+    p, s = pg.where(0, [200])
+    pg.cache.v[p[0], s[0]] = float("nan")
+    assert torch.isnan(ops.attn_decode(q, pg.cache, pg.table, pg.lens_t)[0]).all()
