@@ -603,8 +603,10 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
     int64_t step = B;
     step = std::min<int64_t>(step, (int64_t(1) << 30) / (capt * a.nh));
     if (weights) step = std::min<int64_t>(step, int64_t(ws->gx_bytes / 4) / (int64_t(a.t.cap) * q_heads));
+    const int64_t room = ws->part_floats - 2 * iq::kMaxSeqs - slots * 16 * (2 + a.c.d) - 63;
+    step = std::min<int64_t>(step, room / (2 * q_heads));
+    if (step < 1) return IQ_ETOOLARGE;
     const int64_t fin = (step * q_heads * 2 + 63) / 64 * 64;
-    if (step < 1 || 2 * iq::kMaxSeqs + fin + slots * 16 * (2 + a.c.d) > ws->part_floats) return IQ_ETOOLARGE;
     a.plan = reinterpret_cast<uint2*>(ws->partials);
     a.fin = ws->partials + 2 * iq::kMaxSeqs;
     a.ml = a.fin + fin;

@@ -1,10 +1,13 @@
-"""iq_attn_decode where its scores are extreme."""
+"""iq_attn_decode where its scores are extreme and where its sizes are: scores
+of 2^22 to 2^33, rows none of whose scores lies in fp32's range, and more heads
+in a batch than one launch has room for."""
 import numpy as np
 import pytest
 import torch
 
 from infer_amd import ops
-from tests.kv_util import EPS32, Paged
+from tests.gpu_util import say
+from tests.kv_util import EPS32, Paged, attn_rel
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +93,33 @@ def test_no_score_in_range_keeps_nan():
     p, s = pg.where(0, [200])
     pg.cache.v[p[0], s[0]] = float("nan")
     assert torch.isnan(ops.attn_decode(q, pg.cache, pg.table, pg.lens_t)[0]).all()
+
+
+@pytest.mark.parametrize("B,hq,hk,d", [(1024, 8192, 16, 8), (900, 16384, 64, 8)])
+def test_many_heads_in_a_batch(B, hq, hk, d):
+    """More (sequence, head) pairs than one launch keeps maxima and sums of."""
+    say("attn", B, hq, hk, d)
+    gen = torch.Generator(device="cuda").manual_seed(B)
+    f = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    K, V = f(B, 16, hk, d).to(BF), f(B, 16, hk, d).to(BF)
+    q = f(B, hq, d)
+    lens = torch.randint(0, 17, (B,), generator=gen, device="cuda", dtype=torch.int32)
+    order = torch.randperm(B, generator=gen, device="cuda")
+    cache = ops.KvCache(K[order].contiguous(), V[order].contiguous())
+    table = torch.empty(B, dtype=torch.int32, device="cuda")
+    table[order] = torch.arange(B, dtype=torch.int32, device="cuda")
+    out = ops.attn_decode(q, cache, table[:, None], lens).view(B, hk, hq // hk, d)
+    step = 50
+    for b in range(0, B, step):
+        qd = q[b:b + step].view(-1, hk, hq // hk, d).double() * d ** -0.5
+        Kd, Vd = K[b:b + step].double(), V[b:b + step].double()
+        live = torch.arange(16, device="cuda")[None, :] < lens[b:b + step, None]
+        s = torch.stack([(qd * Kd[:, t, :, None]).sum(-1) for t in range(16)], -1)
+        ck = torch.stack([(qd * Kd[:, t, :, None]).abs().sum(-1) for t in range(16)], -1)
+        s = s.masked_fill(~live[:, None, None], float("-inf"))
+        p = torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e30))
+        p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+        ref = sum(p[..., t, None] * Vd[:, t, :, None] for t in range(16))
+        cv = sum(p[..., t, None] * Vd[:, t, :, None].abs() for t in range(16))
+        rel = attn_rel(d, ck.masked_fill(~live[:, None, None], 0).amax(-1))[..., None]
+        assert torch.all((out[b:b + step].double() - ref).abs() <= rel * cv), b
