@@ -156,6 +156,10 @@ inline void allow_big_lds() {
     (void)once;
 }
 
+// Workgroups of 256 threads that one launch may have along x: a grid of 2^32
+// threads or more is cut to its lower 32 bits, without an error.
+constexpr int64_t kMaxGrid256 = (int64_t(1) << 24) - 1;
+
 // Device properties used by the dispatch heuristics.
 int device_cu_count();
 

@@ -578,19 +578,23 @@ int iq_kv_append(const float* q, const float* k, const float* v, const int64_t* 
         if (q_out != q && iq::ranges_overlap(q_out, qn, q, qn)) return IQ_EALIAS;
         if (iq::ranges_overlap(q_out, qn, k, kn) || iq::ranges_overlap(q_out, qn, v, kn)) return IQ_EALIAS;
     }
-    a.q = q;
-    a.k = k;
-    a.v = v;
-    a.pos = positions;
-    a.slots = slots;
     a.freqs = freqs;
-    a.qo = q_out;
     a.hq = q_heads;
     a.rot = rot_dim;
-    const dim3 grid(static_cast<unsigned>(T), (q_heads + 2 * a.c.hk + iq::kAppendHeads - 1) / iq::kAppendHeads);
+    const int64_t qrow = int64_t(q_heads) * a.c.d, krow = int64_t(a.c.hk) * a.c.d;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (kv->type == IQ_KV_BF16) iq::append_kernel<IQ_KV_BF16><<<grid, 256, 0, s>>>(a);
-    else iq::append_kernel<IQ_KV_F16><<<grid, 256, 0, s>>>(a);
+    for (int64_t t0 = 0; t0 < T; t0 += iq::kMaxGrid256) {
+        a.q = q ? q + t0 * qrow : nullptr;
+        a.k = k + t0 * krow;
+        a.v = v + t0 * krow;
+        a.pos = positions ? positions + t0 : nullptr;
+        a.slots = slots + t0;
+        a.qo = q_out ? q_out + t0 * qrow : nullptr;
+        const dim3 grid(static_cast<unsigned>(std::min<int64_t>(T - t0, iq::kMaxGrid256)),
+                        (q_heads + 2 * a.c.hk + iq::kAppendHeads - 1) / iq::kAppendHeads);
+        if (kv->type == IQ_KV_BF16) iq::append_kernel<IQ_KV_BF16><<<grid, 256, 0, s>>>(a);
+        else iq::append_kernel<IQ_KV_F16><<<grid, 256, 0, s>>>(a);
+    }
     return int(hipGetLastError());
 }
 
