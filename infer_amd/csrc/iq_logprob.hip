@@ -507,9 +507,19 @@ int iq_logprobs(const float* logits, int64_t ld, int64_t T, int64_t V, const int
         a.stat = reinterpret_cast<float4*>(ws->partials);
         a.list = reinterpret_cast<uint64_t*>(ws->partials + T * chunks * 4);
     }
-    const unsigned grid = unsigned(T * chunks);
-    if (top) iq::logprob_kernel<true><<<grid, 64 * iq::kWaves, 0, s>>>(a);
-    else iq::logprob_kernel<false><<<grid, 64 * iq::kWaves, 0, s>>>(a);
+    // (more rows than a grid can have are more than the CUs: a part each)
+    const int64_t rows = chunks > 1 ? T : iq::kMaxGrid256;
+    for (int64_t t0 = 0; t0 < T; t0 += rows) {
+        const unsigned grid = unsigned(std::min(T - t0, rows) * chunks);
+        a.x = logits + t0 * ld;
+        a.tokens = tokens ? tokens + t0 : nullptr;
+        a.lp = logprob ? logprob + t0 : nullptr;
+        a.ent = entropy ? entropy + t0 : nullptr;
+        a.ids = top ? top_ids + t0 * top : nullptr;
+        a.tlp = top ? top_logprobs + t0 * top : nullptr;
+        if (top) iq::logprob_kernel<true><<<grid, 64 * iq::kWaves, 0, s>>>(a);
+        else iq::logprob_kernel<false><<<grid, 64 * iq::kWaves, 0, s>>>(a);
+    }
     if (chunks > 1) {
         if (top) iq::logprob_join_kernel<true><<<unsigned(T), 64 * iq::kWaves, 0, s>>>(a);
         else iq::logprob_join_kernel<false><<<unsigned(T), 64 * iq::kWaves, 0, s>>>(a);
