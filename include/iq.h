@@ -292,7 +292,12 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
  * as less than any number).  With cut = budget - recent: a kept older token
  * below cut stays where it is, the kept ones above it fill the free places
  * below cut, both in ascending order, and the newest follow in their order.
- * weights move along, and weights[b][h][t] = 0 for budget <= t < n, so that a
+ * "Newest" goes by place: the last `recent` slots.  Tokens appended one after
+ * the other lie in the order of their age; behind a call that cut the sequence
+ * only its last `recent` ones and those appended since do, so `recent` must not
+ * be more than these at the next call (a larger one keeps the tokens in the last
+ * slots, which are then not the newest; the device holds the lengths, so this
+ * is not checked).  weights move along, and weights[b][h][t] = 0 for budget <= t < n, so that a
  * slot appended later starts at 0.  new_lens[b] = min(lens[b], budget) for
  * every head alike (the pages past it are free); it must not overlap lens.
  * Pages must not be shared between the sequences of a call nor appear twice in

@@ -293,7 +293,9 @@ class CachedDecodeStep:
     def evict(self, budget, recent):
         """Every layer's caches cut to `budget` tokens a sequence by the weights
         they have received (ops.kv_evict); the pages past them are free, and
-        lens and held are what is left."""
+        lens and held are what is left.  `recent` must not be more than the
+        last evict()'s `recent` and the tokens added since: the rows before
+        those are no longer in the order of their age."""
         if not self.weights:
             raise ValueError("CachedDecodeStep.evict: made without weights")
         self.held.copy_(self._held_now())

@@ -482,7 +482,9 @@ def kv_evict(cache, table, lens, weights, budget, recent, new_lens=None, stream=
     """Cuts every sequence of more than `budget` tokens to `budget`, for each
     key/value head by itself: the newest `recent` stay and, of the others,
     those of the largest weights (fp32 [B, kv_heads, tokens], which move along;
-    entries past the budget become 0).  Returns new_lens (int32 [B]), min(lens,
+    entries past the budget become 0).  The newest are the tokens in the last
+    slots: after a call that cut a sequence, `recent` must not be more than that
+    call's `recent` and the tokens appended since.  Returns new_lens (int32 [B]), min(lens,
     budget): the pages past it are free.  include/iq.h, iq_kv_evict."""
     what = "kv_evict"
     B, pages, ld = _check_table(what, table, lens)
