@@ -170,15 +170,18 @@ class DecodeStep:
         return n + self.model["head"].nbytes()
 
 
-def next_slots(lens, table, page_size, pages=2 ** 31):
+def next_slots(lens, table, page_size, pages=2 ** 31, out=None):
     """The cache slot (int64, page * page_size + slot) behind each sequence's
-    first lens[b] tokens; -1 where there is none: a full table, a page id
-    outside [0, pages), a length below 0."""
-    capacity = table.shape[1] * page_size
-    at = lens.clamp(0, capacity - 1)  # (of any length: the index has to lie in the table)
-    page = table.gather(1, (at // page_size).long()[:, None])[:, 0].long()
-    slot = page * page_size + at % page_size
-    return slot.masked_fill((lens != at) | (page < 0) | (page >= pages), -1)
+    first lens[b] tokens, and whether there is one.  There is none where the
+    table is full, the page id outside [0, pages) or the length below 0; the
+    slot is then outside the pool.  (Few operations: a step makes them all, at
+    about 2 us each in a graph.)"""
+    at = lens.clamp(0, table.shape[1] * page_size - 1)  # (of any length: the index has to lie in the table)
+    nth = (at // page_size).long()
+    # page * page_size + at % page_size
+    slot = torch.add(at, table.gather(1, nth[:, None])[:, 0] - nth, alpha=page_size, out=out)
+    slot.masked_fill_(lens != at, -1)
+    return slot, slot == slot.clamp(0, pages * page_size - 1)
 
 
 class CachedDecodeStep:
@@ -223,6 +226,7 @@ class CachedDecodeStep:
         self.held = torch.zeros(B, dtype=torch.int32, device=device)
         self._left = torch.zeros(B, dtype=torch.int32, device=device)  # lens as step() or evict() left it
         self._attend = torch.zeros(B, dtype=torch.int32, device=device)
+        self._none = torch.full((B,), -1, dtype=torch.int32, device=device)
         self.positions = torch.zeros(B, dtype=torch.int64, device=device)
         self.slots = torch.full((B,), -1, dtype=torch.int64, device=device)
         self.freqs = ops.rope_freqs(hd, c["theta"], device)
@@ -272,12 +276,11 @@ class CachedDecodeStep:
             else:
                 self.ids.copy_(torch.tensor([int(t) for t in token_id], dtype=torch.int64))
         held = self._held_now()
-        self.slots.copy_(next_slots(held, self.table, self.page, self.pages))
-        stored = self.slots >= 0
+        _, stored = next_slots(held, self.table, self.page, self.pages, self.slots)
         torch.add(held, stored, out=self.held)
         # (a row without its token attends to nothing: no length, so that its
         # output is NaN and its weights stay)
-        self._attend.copy_(self.held.masked_fill(~stored, -1))
+        torch.where(stored, self.held, self._none, out=self._attend)
         self.lens.add_(self.lens >= 0)
         self._left.copy_(self.lens)
         ops.launch_embedding_q(self.model["embed"], self.ids, self.rows, self.model["cfg"]["hidden"], self.h0)

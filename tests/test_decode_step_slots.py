@@ -6,6 +6,14 @@ import torch
 from infer_amd.chain import next_slots
 
 
+def slots(lens, table, page, pages=2 ** 31):
+    """next_slots, -1 where it says that there is none."""
+    at, there = next_slots(lens, table, page, pages)
+    assert at.dtype == torch.int64 and there.dtype == torch.bool
+    assert torch.all(there | (at < 0) | (at >= pages * page))
+    return torch.where(there, at, -1).tolist()
+
+
 def plain(lens, table, page, pages=2 ** 31):
     got = []
     for b, n in enumerate(lens):
@@ -20,18 +28,18 @@ def test_slots(page):
     for n in (0, 1, page - 1, page, 2 * page - 1, 2 * page, 3 * page - 1, 3 * page, 3 * page + 1, 2 ** 31 - 1,
               -1, -2, -page, -page - 1, -2 ** 31):
         lens = [n, 0, n]
-        got = next_slots(torch.tensor(lens, dtype=torch.int32), torch.tensor(table, dtype=torch.int32), page)
-        assert got.dtype == torch.int64 and got.tolist() == plain(lens, table, page), n
+        got = slots(torch.tensor(lens, dtype=torch.int32), torch.tensor(table, dtype=torch.int32), page)
+        assert got == plain(lens, table, page), n
 
 
 def test_slots_in_a_part_of_a_table():
     wide = torch.arange(24, dtype=torch.int32).view(3, 8)
     lens = torch.tensor([0, 9, 31], dtype=torch.int32)
-    assert next_slots(lens, wide[:, 2:5], 10).tolist() == [20, 109, -1]
+    assert slots(lens, wide[:, 2:5], 10) == [20, 109, -1]
 
 
 def test_pages_outside_the_pool():
     table = [[3, 8, 9], [9, 0, 2 ** 31 - 1]]
     for n in range(12):
-        got = next_slots(torch.tensor([n, n]), torch.tensor(table, dtype=torch.int32), 4, 9)
-        assert got.tolist() == plain([n, n], table, 4, 9), n
+        got = slots(torch.tensor([n, n]), torch.tensor(table, dtype=torch.int32), 4, 9)
+        assert got == plain([n, n], table, 4, 9), n
