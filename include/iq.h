@@ -269,9 +269,13 @@ int iq_kv_append(const float* q, const float* k, const float* v, const int64_t* 
  * whatever they hold.
  * weights (may be NULL): fp32 [B][kv_heads][weights_ld], weights_ld >=
  * max_pages * page_size; weights[b][j][t] += sum over the heads h of key/value
- * head j of p[b,h,t], for t < lens[b]; the rest is left as it was.  A
- * sequence's scores lie in the workspace: max_pages * page_size * q_heads may
- * be at most 20971520 with weights (IQ_ETOOLARGE).
+ * head j of p[b,h,t], for t < lens[b]; the rest is left as it was.  The
+ * scores lie in the workspace, as much room a sequence as its table row can
+ * hold tokens: max_pages * page_size * q_heads may be at most 20971520 with
+ * weights (IQ_ETOOLARGE), and of a larger batch 20971520 / (max_pages *
+ * page_size * q_heads) sequences go at a time, one group behind the other
+ * however short they are.  Where weights are wanted, max_pages should be no
+ * more than the longest sequence needs.
  * A sequence of length 0 gives zeros.  A length below 0 or above max_pages *
  * page_size gives NaN, its weights left as they were.  A page id outside [0,
  * pages) among the sequence's pages, a q that is not finite or a key of NaN

@@ -200,8 +200,8 @@ class CachedDecodeStep:
     part from lens after an eviction), and for a new sequence in a row its
     weights, to 0.  held (int32 [B]) is how many of the tokens lie in the cache:
     lens, less those that found no place (see step) since the caller or evict()
-    last set lens.  step() issues only device work, so it can be captured into
-    a graph (after ops.init on the capturing stream)."""
+    last set lens.  step() without a list of ids issues only device work, so it
+    can be captured into a graph (after ops.init on the capturing stream)."""
 
     def __init__(self, model, caches, table, weights=False, device="cuda"):
         c = model["cfg"]

@@ -6,7 +6,7 @@
 // cycles and lane, too many beside the unpacking; on the matrix cores the up
 // to 16 heads of a group are the 16 columns of one product and cost nothing.
 // What bounds the operator is the read of the cache: 131072 tokens, 4 heads of
-// 128 in bf16 take 56.3 us (4.77 TB/s; a device copy reaches 4.74), every byte
+// 128 in bf16 take 57 us (4.71 TB/s; a device copy reaches 4.74), every byte
 // read once, the matrix cores busy for 12 % of it; 32 sequences of up to 8192
 // tokens, 2 heads, 21 us (4.1 TB/s).  A join adds 4 to 5 us.
 //
@@ -151,8 +151,9 @@ struct Terms<IQ_KV_BF16> {
     }
 };
 
-// x = t0 + t1 to 22 bits.  p is scaled by 2^12 (and its sum with it), so that
-// what the terms drop stays below 2^-36 of the largest p.
+// x = t0 + t1, off by at most 2^-23 of x (each term rounds to 11 bits), and by
+// 2^-25 where t1 is subnormal.  p is scaled by 2^12 (and its sum with it), which
+// makes the latter 2^-37 of the largest p.
 template <>
 struct Terms<IQ_KV_F16> {
     static constexpr int N = 2;

@@ -414,7 +414,8 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, char* pool, int b,
         int64_t go[kMoveUnroll];
     };
     // (past the end the last row again, not written: no branch between the
-    // loads, which would wait for one another; likewise a unit past the row)
+    // loads of the rows, which would wait for one another; likewise a unit past
+    // the row)
     if (u < a.c.d / 8) pool += u * 16;
     auto read = [&](int m, Chunk& c) {
         int f[kMoveUnroll], t[kMoveUnroll];
@@ -484,7 +485,8 @@ __global__ __launch_bounds__(TH, TH == kMoveThreads ? 4 : 1) void evict_shift_ke
     const int32_t* dst = a.dst + row * a.m;
     const int32_t* src = a.src + row * a.m;
     // (past the free places entry 0 is named, which is there to be read even
-    // where no place is free; it is not used then)
+    // where no place is free, and is not used then; the compiler puts the load
+    // behind a branch all the same)
     auto from = [&](int i) {
         const int s = src[i < holes ? i : 0];
         return i < holes ? s : n - recent + (i - holes);

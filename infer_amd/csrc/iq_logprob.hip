@@ -363,7 +363,9 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int64_t t, const St
     }
 }
 
-// Workgroups a CU that a call is split into (and that its registers allow for).
+// Workgroups a CU that a call is split into (and that its registers allow for:
+// with the list and five a CU, 96 of them and one that is spilled, 8 bytes of
+// scratch memory a lane).
 constexpr int kPerCu = 4, kPerCuTop = 5;
 
 template <bool TOP>
