@@ -243,7 +243,7 @@ typedef struct iq_kv {
     void* v;
 } iq_kv;
 
-/* Adds T tokens to the cache: k, v fp32 [T][kv_heads][head_dim] are written
+/* Adds T >= 1 tokens to the cache: k, v fp32 [T][kv_heads][head_dim] are written
  * to slot slots[t] = page * page_size + slot (rounded to the cache's type,
  * to nearest even), q fp32 [T][q_heads][head_dim] goes to q_out; q and k with
  * rotary embedding on their first rot_dim values (pairs i, i + rot_dim/2
@@ -265,7 +265,8 @@ int iq_kv_append(const float* q, const float* k, const float* v, const int64_t* 
  * [B][table_ld] of which the first max_pages entries of a row may be used
  * (entries past a sequence's last page are not read), lens int32 [B], 1 <= B
  * <= 1024.  Scores, softmax and sums are fp32; the 16-bit keys and values
- * are taken as they are.  Keys and values past a sequence's length have no influence,
+ * are taken as they are (over an fp16 cache, q and p enter the products to 2^-23
+ * of themselves, and to 2^-38 of the head's largest |q| and 2^-37 of the largest p).  Keys and values past a sequence's length have no influence,
  * whatever they hold.
  * weights (may be NULL): fp32 [B][kv_heads][weights_ld], weights_ld >=
  * max_pages * page_size; weights[b][j][t] += sum over the heads h of key/value
