@@ -265,8 +265,9 @@ int iq_kv_append(const float* q, const float* k, const float* v, const int64_t* 
  * [B][table_ld] of which the first max_pages entries of a row may be used
  * (entries past a sequence's last page are not read), lens int32 [B], 1 <= B
  * <= 1024.  Scores, softmax and sums are fp32; the 16-bit keys and values
- * are taken as they are (over an fp16 cache, q and p enter the products to 2^-23
- * of themselves, and to 2^-38 of the head's largest |q| and 2^-37 of the largest p).  Keys and values past a sequence's length have no influence,
+ * are taken as they are (over an fp16 cache, q and p enter the products to
+ * 2^-23 of themselves, and to 2^-38 of the head's largest |q| and 2^-37 of its
+ * largest p).  Keys and values past a sequence's length have no influence,
  * whatever they hold.
  * weights (may be NULL): fp32 [B][kv_heads][weights_ld], weights_ld >=
  * max_pages * page_size; weights[b][j][t] += sum over the heads h of key/value
