@@ -231,17 +231,34 @@ void iq_chain_destroy(iq_chain* chain);
  * (in elements; v alike), head_dim contiguous values.  Any order of pages,
  * slots and heads in memory can be described, and pages may be shared between
  * sequences as long as nothing writes them.  k, v 16-byte aligned, the strides
- * multiples of 8, head_dim a multiple of 8 in 8..256. */
-enum { IQ_KV_BF16 = 0, IQ_KV_F16 = 1 };
+ * multiples of 8, head_dim a multiple of 8 in 8..256 (8-bit types: of 16).
+ *
+ * A cache holds bf16 or fp16 values, or 8-bit codes (signed integers
+ * -127..127, or e4m3 numbers up to 448) with a scale for every `block`
+ * consecutive slots of a page and key/value head: the value of a code is code *
+ * scale.  iq_kv_append, iq_attn_decode and iq_kv_evict take 16-bit caches
+ * (IQ_EKIND); iq_kv_extend, iq_kv_read and iq_attn_decode_window take all. */
+enum { IQ_KV_BF16 = 0, IQ_KV_F16 = 1, IQ_KV_I8 = 2, IQ_KV_E4M3 = 3 };
 
 typedef struct iq_kv {
-    int32_t type;                              /* IQ_KV_BF16, IQ_KV_F16 */
+    int32_t type;                              /* IQ_KV_* */
     int32_t kv_heads, head_dim, page_size;     /* page_size: any number of slots >= 1 */
     int64_t pages;                             /* in the pool, < 2^31 */
     int64_t page_stride, slot_stride, head_stride;
     void* k;
     void* v;
 } iq_kv;
+
+/* The scales of an 8-bit cache: that of slot s of a page and head h is at
+ *   k + page * page_stride + (s / block) * block_stride + h * head_stride
+ * (in floats; v alike).  block divides page_size (1: a scale for each token
+ * and head). */
+typedef struct iq_kv_scales {
+    int32_t block;
+    int64_t page_stride, block_stride, head_stride;
+    float* k;
+    float* v;
+} iq_kv_scales;
 
 /* Adds T >= 1 tokens to the cache: k, v fp32 [T][kv_heads][head_dim] are written
  * to slot slots[t] = page * page_size + slot (rounded to the cache's type,
@@ -317,6 +334,60 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
 int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t max_pages, const int32_t* lens,
                 int B, int64_t budget, int64_t recent, float* weights, int64_t weights_ld, int32_t* new_lens,
                 void* stream);
+
+/* Adds T new tokens of B sequences behind what each has cached, the first
+ * lens[b] tokens in the pages table[b]: rows starts[b] <= t < starts[b + 1] of q,
+ * k, v and positions are sequence b's tokens lens[b], lens[b] + 1, ... (starts
+ * int32 [B + 1], ascending, from 0 to T; NULL: one token each, T = B).  lens is read
+ * only: the sequence's length is lens[b] + its new tokens afterwards.
+ *   norms     q_norm, k_norm (bf16 [head_dim], each may be NULL): every head of q
+ *             (k) becomes x / sqrt(mean(x^2) + eps) * norm first, eps >= 0
+ *   rotation  as in iq_kv_append, behind the norms
+ *   q         goes to q_out in fp32 (every row below T, whatever its sequence)
+ *   k, v      are rounded into the cache, to nearest even
+ * A token behind the table's last page, in a page whose id lies outside [0,
+ * pages) or of a sequence whose length is below 0 or above max_pages * page_size is
+ * not stored.  Rows that belong to no sequence are not either.  Pages that are
+ * written must not be shared between the sequences nor appear twice in one.
+ *
+ * An 8-bit cache's blocks start anew with their first slot: with a = max |x| over
+ * the call's tokens of the block (one head's k or v), in fp32, and Q = 127 (448),
+ *   - a block whose first slot is among them, or whose scale is 0, gets the
+ *     scale s = max(a / Q, 2^-126), or 0 if a is 0;
+ *   - a block that holds older tokens (the sequence's, below lens[b]) keeps its
+ *     scale if a <= Q * s; otherwise s doubles until it is so and the older
+ *     tokens' codes are halved as often, at once, to nearest even.  So a stored
+ *     value is off by less than one step of its block's scale (int8; half a
+ *     step where the scale did not grow), however often it grew.
+ * Codes are x / s to nearest even.  A value that is not finite makes its block's
+ * scale NaN, and all that is read from the block, until the block starts anew. */
+int iq_kv_extend(const float* q, const float* k, const float* v, int64_t T, int q_heads, const uint16_t* q_norm,
+                 const uint16_t* k_norm, float eps, const int64_t* positions, const double* freqs, int rot_dim,
+                 const iq_kv* kv, const iq_kv_scales* scales, const int32_t* table, int64_t table_ld,
+                 int64_t max_pages, const int32_t* lens, const int32_t* starts, int B, float* q_out, void* stream);
+
+/* Cached tokens back as numbers: rows starts[b] <= t < starts[b + 1] of k_out
+ * and v_out ([T][kv_heads][head_dim], one of them may be NULL) become sequence
+ * b's tokens first[b], first[b] + 1, ... (first NULL: 0).  out_type IQ_READ_*; a
+ * code times its scale is rounded once, to nearest even.  Rows that belong to no
+ * sequence are left as they were; a token outside the table, or in a page whose
+ * id lies outside [0, pages), is NaN. */
+enum { IQ_READ_F32 = 0, IQ_READ_BF16 = 1, IQ_READ_F16 = 2 };
+int iq_kv_read(const iq_kv* kv, const iq_kv_scales* scales, const int32_t* table, int64_t table_ld, int64_t max_pages,
+               const int32_t* first, const int32_t* starts, int B, int64_t T, int out_type, void* k_out, void* v_out,
+               void* stream);
+
+/* iq_attn_decode, without weights, over a cache of any type (scales: of an
+ * 8-bit one; not used otherwise), and optionally under a window: with window > 0 a
+ * sequence sees its newest `window` tokens and its first `sinks` ones, t >= lens[b]
+ * - window or t < sinks.  Pages that hold none of these are not read, and their
+ * table entries may be anything.  window = 0: all tokens, whatever sinks is.
+ * Keys and values are the codes times their scales, in fp32: a scale of a key
+ * multiplies its score, that of a value its weight (in full precision from scales of
+ * 2^-86 on).  A NaN or infinite scale is like a NaN key or value. */
+int iq_attn_decode_window(const float* q, const iq_kv* kv, const iq_kv_scales* scales, const int32_t* table,
+                          int64_t table_ld, int64_t max_pages, const int32_t* lens, int B, int q_heads, float scale,
+                          int64_t window, int64_t sinks, float* out, void* stream);
 
 /* Log probabilities over rows of logits, fp32 [T][V] with `ld` >= V floats
  * from row to row (V < 2^31 - 65536):

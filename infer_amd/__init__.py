@@ -14,6 +14,8 @@ from .ops import (  # noqa: F401
     attn_decode,
     kv_append,
     kv_evict,
+    kv_extend,
+    kv_read,
     launch_embedding_q,
     launch_gemm_bf16x,
     launch_gemm_tiled_q,

@@ -24,7 +24,7 @@ HOST_CXX_FLAGS = ["-std=c++17", "-O2", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__
                   "-I" + os.path.join(os.path.dirname(HERE), "include"), "-I" + os.path.join(HERE, "host"),
                   "-I" + os.path.join(ROCM, "include")]
 SOURCES = ["iq_abi.hip", "iq_quant.hip", "iq_gemv.hip", "iq_gemm.hip", "iq_gemmw.hip", "iq_chain.hip",
-           "iq_kv.hip", "iq_attn.hip", "iq_logprob.hip"]
+           "iq_kv.hip", "iq_kv8.hip", "iq_attn.hip", "iq_attn8.hip", "iq_logprob.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",

@@ -34,147 +34,15 @@
 // chunk, else the chunk's maximum, sum and unnormalised rows, which
 // attn_join_kernel adds up.  Nothing is kept between calls and no order of
 // additions depends on timing.
-#include <algorithm>
-
-#include "iq_attn_plan.h"
-#include "iq_kv.h"
+#include "iq_attn.h"
 
 namespace iq {
 namespace {
 
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
-typedef short s16x8_t __attribute__((ext_vector_type(8)));
-
-struct AttnArgs {
-    KvView c;
-    KvTable t;
-    const float* q;
-    float* out;
-    int hq, group, B;
-    int ht;           // 16-head tiles of a group
-    uint32_t nh;      // hk * ht
-    uint32_t target;
-    int lines;        // heads share cache lines
-    float mul;        // scale * log2(e): scores in powers of two
-    float* ml;        // [partials][16][2]: a chunk's maximum and sum of every head
-    float* part;      // [partials][16][d]
-    uint2* plan;      // [B]: chunks, first partial
-    float* sc;        // scores [B][hk][cap][group] for the weights, or null
-    float* fin;       // [B][hq][2]: maximum and sum of every head, for the weights
-};
-
-// The maximum of no scores: finite, so that scores of -inf (products past
-// fp32's range) and runs without scores count nothing instead of giving NaN.
-constexpr float kNone = -3.4e38f;
-
-// 1 / a head's sum.  It is 0 only where every score is -inf: the head's values
-// are then 0 times 0 (or NaN, where a value is not finite), its weights 0.
-__device__ __forceinline__ float inv_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
-
-struct Item {
-    int b, n;            // sequence and its length (as given)
-    uint32_t j, c, chunks, first;  // chunk, tiles of a chunk, chunks of the sequence, its first partial
-};
-
-// The (sequence, chunk) number w of the batch's plan; false past the last.
-// Every wave finds it from the lengths by itself (64 sequences a step).
-__device__ bool find_item(const AttnArgs& a, uint32_t w, Item* it) {
-    const int lane = threadIdx.x & 63;
-    auto length = [&](int b) { return b < a.B ? a.t.lens[b] : 0; };
-    auto tiles_of = [&](int n) { return n < 0 || n > a.t.cap ? 0u : attn_tiles(n); };
-    int n = length(lane);
-    const int n0 = n;
-    uint32_t total = lane_of(wave_scan(tiles_of(n)), 63);
-    for (int b0 = 64; b0 < a.B; b0 += 64) total += lane_of(wave_scan(tiles_of(length(b0 + lane))), 63);
-    const uint32_t least = attn_chunk_tiles(total, a.nh, a.target);
-    uint32_t c = least;
-    for (int i = 0; i < kAttnTries && uint32_t(a.B) * a.nh <= a.target; i++) {
-        uint32_t items = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 64)
-            items += lane_of(wave_scan(b0 + lane < a.B ? attn_chunks(tiles_of(b0 ? length(b0 + lane) : n0), c) : 0), 63);
-        if (items * a.nh <= a.target) break;
-        c = attn_more_tiles(c, least);
-    }
-    uint32_t before = 0, first = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        if (b0) n = length(b0 + lane);
-        const uint32_t k = b0 + lane < a.B ? attn_chunks(tiles_of(n), c) : 0;
-        const uint32_t upto = wave_scan(k), many = k > 1 ? k : 0, pupto = wave_scan(many);
-        const uint64_t past = __ballot(w < before + upto);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            it->b = b0 + l;
-            it->n = __builtin_amdgcn_readlane(n, l);
-            it->chunks = lane_of(k, l);
-            it->j = w - before - (lane_of(upto, l) - it->chunks);
-            it->first = first + lane_of(pupto, l) - lane_of(many, l);
-            it->c = c;
-            return true;
-        }
-        before += lane_of(upto, 63);
-        first += lane_of(pupto, 63);
-    }
-    return false;
-}
-
-// ------------------------------------------------------- operands of q and p
-template <int TYPE>
-struct Terms;
-
-// x = t0 + t1 + t2 exactly, each the upper 16 bits of what is left.
-template <>
-struct Terms<IQ_KV_BF16> {
-    static constexpr int N = 3;
-    static constexpr float kUp = 0.0f;
-    static __device__ __forceinline__ void cut(const float (&x)[8], s16x8_t (&t)[N]) {
-        float r[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) r[i] = x[i];
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-            u32x4_t u;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t lo = __float_as_uint(r[2 * i]), hi = __float_as_uint(r[2 * i + 1]);
-                u[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-                if (k + 1 < N) {
-                    r[2 * i] -= __uint_as_float(lo & 0xffff0000u);
-                    r[2 * i + 1] -= __uint_as_float(hi & 0xffff0000u);
-                }
-            }
-            t[k] = __builtin_bit_cast(s16x8_t, u);
-        }
-    }
-    static __device__ __forceinline__ float4_t mma(s16x8_t a, s16x8_t b, float4_t c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
-                                                       c, 0, 0, 0);
-    }
-};
-
-// x = t0 + t1, off by at most 2^-23 of x (each term rounds to 11 bits), and by
-// 2^-25 where t1 is subnormal.  p is scaled by 2^12 (and its sum with it), which
-// makes the latter 2^-37 of the largest p.
-template <>
-struct Terms<IQ_KV_F16> {
-    static constexpr int N = 2;
-    static constexpr float kUp = 12.0f;
-    static __device__ __forceinline__ void cut(const float (&x)[8], s16x8_t (&t)[N]) {
-        half8_t h, l;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            h[i] = _Float16(x[i]);
-            l[i] = _Float16(x[i] - float(h[i]));
-        }
-        t[0] = __builtin_bit_cast(s16x8_t, h);
-        t[1] = __builtin_bit_cast(s16x8_t, l);
-    }
-    static __device__ __forceinline__ float4_t mma(s16x8_t a, s16x8_t b, float4_t c) {
-        return mfma16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
-    }
-};
-
-// DP: head_dim rounded up to 32, 64, 128 or 256.
-template <int TYPE, int DP>
+// DP: head_dim rounded up to 32, 64, 128 or 256.  WIN: of a sequence longer
+// than a.visible only the first a.sinks tokens and the newest others are seen;
+// they are numbered without the gap.
+template <int TYPE, int DP, bool WIN>
 __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel(AttnArgs a) {
     using T = Terms<TYPE>;
     constexpr int CH = DP / 8, RPI = 64 / CH, NI = kAttnTile / RPI;  // 16-byte chunks of a row, rows of a load, loads
@@ -188,7 +56,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     // chunk: workgroups are dealt to the 8 of them in turn.
     const uint32_t turn = a.lines ? 8 : 1, round = blockIdx.x / (turn * a.nh), in = blockIdx.x % (turn * a.nh);
     const uint32_t hidx = in / turn;
-    if (!find_item(a, round * turn + in % turn, &it)) return;
+    if (!find_item<WIN>(a, round * turn + in % turn, &it)) return;
     const int b = it.b, n = it.n, d = a.c.d;
     const int j = int(hidx) / a.ht, h0 = int(hidx) % a.ht * 16, gh = min(16, a.group - h0);
     float* out = a.out + (int64_t(b) * a.hq + j * a.group + h0) * d;
@@ -198,15 +66,16 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
         for (int i = threadIdx.x; i < gh * d; i += 64 * kAttnWaves) out[i] = x;
         return;
     }
-    const int t0 = int(it.j * it.c) * kAttnTile, t1 = t0 + min(n - t0, int(it.c) * kAttnTile);
+    const int t0 = int(it.j * it.c) * kAttnTile, t1 = t0 + min(it.seen - t0, int(it.c) * kAttnTile);
     const int ntiles = (t1 - t0 + kAttnTile - 1) / kAttnTile;
 
     // row r of a tile: element offset of its (page, slot), 0 where there is none
     bool poison = false;
     const int32_t* table = a.t.table + b * a.t.ld;
     auto row_offset = [&](int tile) -> int64_t {
-        const int tok = t0 + tile * kAttnTile + (lane & 31);
+        int tok = t0 + tile * kAttnTile + (lane & 31);
         if (tok >= t1) return 0;
+        if (WIN && tok >= a.sinks) tok += n - it.seen;
         const uint32_t p = page_of(uint32_t(tok), a.c.div), s = uint32_t(tok) - p * uint32_t(a.c.ps);
         const int32_t id = table[p];
         const bool ok = id >= 0 && id < a.c.pages;
@@ -551,12 +420,92 @@ __global__ __launch_bounds__(TH) void attn_weights_kernel(AttnArgs a, float* wei
     if (t < n) weights[row * wld + t] += sum;
 }
 
-template <int TYPE>
+template <int TYPE, bool WIN>
 void launch_attn(const AttnArgs& a, unsigned grid, hipStream_t s) {
-    if (a.c.d <= 32) attn_kernel<TYPE, 32><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else if (a.c.d <= 64) attn_kernel<TYPE, 64><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else if (a.c.d <= 128) attn_kernel<TYPE, 128><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else attn_kernel<TYPE, 256><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    if (a.c.d <= 32) attn_kernel<TYPE, 32, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else if (a.c.d <= 64) attn_kernel<TYPE, 64, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else if (a.c.d <= 128) attn_kernel<TYPE, 128, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else attn_kernel<TYPE, 256, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+}
+
+// The call behind either entry point; a: cache, scales and table, checked.
+int attn_decode(AttnArgs a, const float* q, int B, int q_heads, float scale, int64_t window, int64_t sinks, float* out,
+                float* weights, int64_t weights_ld, hipStream_t s) {
+    if (!q || !out) return IQ_ENULL;
+    a.mul = scale * 1.44269504088896340736f;
+    if (q_heads < 1 || q_heads > 16384 || q_heads % a.c.hk || !std::isfinite(a.mul)) return IQ_ESHAPE;
+    if (window < 0 || sinks < 0) return IQ_ESHAPE;
+    if (weights && weights_ld < a.t.cap) return IQ_ESHAPE;
+    const int64_t row = int64_t(q_heads) * a.c.d;
+    if (ranges_overlap(q, B * row * 4, out, B * row * 4)) return IQ_EALIAS;
+    Workspace* ws = nullptr;
+    const hipError_t e = get_workspace(s, &ws);
+    if (e != hipSuccess) return e == hipErrorOutOfMemory ? IQ_ENOMEM : int(e);
+    const bool bits8 = a.c.type == IQ_KV_I8 || a.c.type == IQ_KV_E4M3;
+    a.hq = q_heads;
+    a.group = q_heads / a.c.hk;
+    a.ht = (a.group + 15) / 16;
+    a.nh = uint32_t(a.c.hk * a.ht);
+    // what a sequence sees at most; a window that no sequence can reach is none
+    const bool win = window > 0 && window < a.t.cap && sinks < a.t.cap - window;
+    a.sinks = win ? int32_t(sinks) : 0;
+    a.visible = win ? int32_t(window + sinks) : a.t.cap;
+    // as many work items as run at once: 4, 3, 2 or 1 workgroups a CU by the
+    // registers (d <= 64) and the LDS of an instance.  Measured for d = 128 on
+    // 131072 tokens / 32 sequences of up to 8192: 1 a CU 69.9 / 30.4 us, 2 61.8
+    // / 24.7, 3 69.1 / 27.8, 4 66.0 / 29.4; for d = 64 (24 of up to 2047, 16
+    // heads) 18.1, 19.0, 17.2, 18.8.
+    const int groups = bits8 ? attn8_groups(a.c.d) : a.c.d <= 32 ? 4 : a.c.d <= 64 ? 3 : a.c.d <= 128 ? 2 : 1;
+    a.target = uint32_t(groups * device_cu_count());
+    // Neighbouring heads' rows meet in a cache line, or several head tiles read
+    // the same rows: one XCD's L2 then serves them (8 sequences of 16384, 8 heads
+    // of 32: 49.7 -> 38.8 us; of 8192, heads of 80: 50.1 -> 44.6).  Whole lines
+    // are better spread (131072 tokens, 4 heads of 128: 61.9 and 64.0).
+    a.lines = a.nh > 1 && (a.ht > 1 || (bits8 ? 1 : 2) * a.c.hstr % 128 != 0);
+    const int64_t capt = attn_tiles(a.visible);
+    // the workspace's partial sums: plan | final (maximum, sum) | chunks' | rows;
+    // its GEMM operand area: the scores that the weights are made of
+    const int64_t slots = attn_max_partials(a.target);
+    int64_t step = B;
+    step = std::min<int64_t>(step, (int64_t(1) << 30) / (capt * a.nh));
+    if (weights) step = std::min<int64_t>(step, int64_t(ws->gx_bytes / 4) / (int64_t(a.t.cap) * q_heads));
+    const int64_t room = ws->part_floats - 2 * kMaxSeqs - slots * 16 * (2 + a.c.d) - 63;
+    step = std::min<int64_t>(step, room / (2 * q_heads));
+    if (step < 1) return IQ_ETOOLARGE;
+    const int64_t fin = (step * q_heads * 2 + 63) / 64 * 64;
+    a.plan = reinterpret_cast<uint2*>(ws->partials);
+    a.fin = ws->partials + 2 * kMaxSeqs;
+    a.ml = a.fin + fin;
+    a.part = a.ml + slots * 32;
+    a.sc = weights ? static_cast<float*>(ws->gx) : nullptr;
+    const KvTable t = a.t;
+    for (int b0 = 0; b0 < B; b0 += int(step)) {
+        a.B = int(std::min<int64_t>(step, B - b0));
+        a.q = q + b0 * row;
+        a.out = out + b0 * row;
+        a.t.table = t.table + b0 * t.ld;
+        a.t.lens = t.lens + b0;
+        int64_t grid = attn_max_items(a.B, a.nh, a.visible, a.target);
+        if (a.lines) grid = (grid / a.nh + 7) / 8 * 8 * a.nh;
+        if (bits8) launch_attn8(a, win, unsigned(grid), s);
+        else if (a.c.type == IQ_KV_BF16) (win ? launch_attn<IQ_KV_BF16, true> : launch_attn<IQ_KV_BF16, false>)(a, unsigned(grid), s);
+        else (win ? launch_attn<IQ_KV_F16, true> : launch_attn<IQ_KV_F16, false>)(a, unsigned(grid), s);
+        // (a sequence has at most target / nh chunks and one more)
+        const bool many = a.B <= 4 && std::min<int64_t>(capt / kAttnWaves, a.target / a.nh) > 64;
+        const int th = many ? 1024 : 256;
+        const dim3 heads{unsigned(q_heads), unsigned(a.B)};
+        if (weights) {
+            float* w = weights + int64_t(b0) * a.c.hk * weights_ld;
+            const float up = a.c.type == IQ_KV_F16 ? Terms<IQ_KV_F16>::kUp : Terms<IQ_KV_BF16>::kUp;
+            const dim3 all{unsigned(q_heads + (int64_t(a.t.cap) + th - 1) / th * a.c.hk), unsigned(a.B)};
+            if (many) attn_weights_kernel<1024><<<all, 1024, 0, s>>>(a, w, weights_ld, up);
+            else attn_weights_kernel<256><<<all, 256, 0, s>>>(a, w, weights_ld, up);
+        } else if (capt > kAttnWaves) {  // (else no sequence has two chunks)
+            if (many) attn_join_kernel<1024><<<heads, 1024, 0, s>>>(a);
+            else attn_join_kernel<256><<<heads, 256, 0, s>>>(a);
+        }
+    }
+    return int(hipGetLastError());
 }
 
 }  // namespace
@@ -572,73 +521,18 @@ int iq_attn_decode(const float* q, const iq_kv* kv, const int32_t* table, int64_
     if (rc) return rc;
     rc = iq::check_table(a.c, table, table_ld, max_pages, lens, B, &a.t);
     if (rc) return rc;
-    if (!q || !out) return IQ_ENULL;
-    a.mul = scale * 1.44269504088896340736f;
-    if (q_heads < 1 || q_heads > 16384 || q_heads % a.c.hk || !std::isfinite(a.mul)) return IQ_ESHAPE;
-    if (weights && weights_ld < a.t.cap) return IQ_ESHAPE;
-    const int64_t row = int64_t(q_heads) * a.c.d;
-    if (iq::ranges_overlap(q, B * row * 4, out, B * row * 4)) return IQ_EALIAS;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    iq::Workspace* ws = nullptr;
-    const hipError_t e = iq::get_workspace(s, &ws);
-    if (e != hipSuccess) return e == hipErrorOutOfMemory ? IQ_ENOMEM : int(e);
-    a.hq = q_heads;
-    a.group = q_heads / a.c.hk;
-    a.ht = (a.group + 15) / 16;
-    a.nh = uint32_t(a.c.hk * a.ht);
-    // as many work items as run at once: 4, 3, 2 or 1 workgroups a CU by the
-    // registers (d <= 64) and the LDS of an instance.  Measured for d = 128 on
-    // 131072 tokens / 32 sequences of up to 8192: 1 a CU 69.9 / 30.4 us, 2 61.8
-    // / 24.7, 3 69.1 / 27.8, 4 66.0 / 29.4; for d = 64 (24 of up to 2047, 16
-    // heads) 18.1, 19.0, 17.2, 18.8.
-    a.target = uint32_t((a.c.d <= 32 ? 4 : a.c.d <= 64 ? 3 : a.c.d <= 128 ? 2 : 1) * iq::device_cu_count());
-    // Neighbouring heads' rows meet in a cache line, or several head tiles read
-    // the same rows: one XCD's L2 then serves them (8 sequences of 16384, 8 heads
-    // of 32: 49.7 -> 38.8 us; of 8192, heads of 80: 50.1 -> 44.6).  Whole lines
-    // are better spread (131072 tokens, 4 heads of 128: 61.9 and 64.0).
-    a.lines = a.nh > 1 && (a.ht > 1 || 2 * a.c.hstr % 128 != 0);
-    const int64_t capt = iq::attn_tiles(a.t.cap);
-    // the workspace's partial sums: plan | final (maximum, sum) | chunks' | rows;
-    // its GEMM operand area: the scores that the weights are made of
-    const int64_t slots = iq::attn_max_partials(a.target);
-    int64_t step = B;
-    step = std::min<int64_t>(step, (int64_t(1) << 30) / (capt * a.nh));
-    if (weights) step = std::min<int64_t>(step, int64_t(ws->gx_bytes / 4) / (int64_t(a.t.cap) * q_heads));
-    const int64_t room = ws->part_floats - 2 * iq::kMaxSeqs - slots * 16 * (2 + a.c.d) - 63;
-    step = std::min<int64_t>(step, room / (2 * q_heads));
-    if (step < 1) return IQ_ETOOLARGE;
-    const int64_t fin = (step * q_heads * 2 + 63) / 64 * 64;
-    a.plan = reinterpret_cast<uint2*>(ws->partials);
-    a.fin = ws->partials + 2 * iq::kMaxSeqs;
-    a.ml = a.fin + fin;
-    a.part = a.ml + slots * 32;
-    a.sc = weights ? static_cast<float*>(ws->gx) : nullptr;
-    for (int b0 = 0; b0 < B; b0 += int(step)) {
-        a.B = int(std::min<int64_t>(step, B - b0));
-        a.q = q + b0 * row;
-        a.out = out + b0 * row;
-        a.t.table = table + b0 * table_ld;
-        a.t.lens = lens + b0;
-        int64_t grid = iq::attn_max_items(a.B, a.nh, a.t.cap, a.target);
-        if (a.lines) grid = (grid / a.nh + 7) / 8 * 8 * a.nh;
-        if (kv->type == IQ_KV_BF16) iq::launch_attn<IQ_KV_BF16>(a, unsigned(grid), s);
-        else iq::launch_attn<IQ_KV_F16>(a, unsigned(grid), s);
-        // (a sequence has at most target / nh chunks and one more)
-        const bool many = a.B <= 4 && std::min<int64_t>(capt / iq::kAttnWaves, a.target / a.nh) > 64;
-        const int th = many ? 1024 : 256;
-        const dim3 heads{unsigned(q_heads), unsigned(a.B)};
-        if (weights) {
-            float* w = weights + int64_t(b0) * a.c.hk * weights_ld;
-            const float up = kv->type == IQ_KV_F16 ? iq::Terms<IQ_KV_F16>::kUp : iq::Terms<IQ_KV_BF16>::kUp;
-            const dim3 all{unsigned(q_heads + (int64_t(a.t.cap) + th - 1) / th * a.c.hk), unsigned(a.B)};
-            if (many) iq::attn_weights_kernel<1024><<<all, 1024, 0, s>>>(a, w, weights_ld, up);
-            else iq::attn_weights_kernel<256><<<all, 256, 0, s>>>(a, w, weights_ld, up);
-        } else if (capt > iq::kAttnWaves) {  // (else no sequence has two chunks)
-            if (many) iq::attn_join_kernel<1024><<<heads, 1024, 0, s>>>(a);
-            else iq::attn_join_kernel<256><<<heads, 256, 0, s>>>(a);
-        }
-    }
-    return int(hipGetLastError());
+    return iq::attn_decode(a, q, B, q_heads, scale, 0, 0, out, weights, weights_ld, static_cast<hipStream_t>(stream));
+}
+
+int iq_attn_decode_window(const float* q, const iq_kv* kv, const iq_kv_scales* scales, const int32_t* table,
+                          int64_t table_ld, int64_t max_pages, const int32_t* lens, int B, int q_heads, float scale,
+                          int64_t window, int64_t sinks, float* out, void* stream) {
+    iq::AttnArgs a{};
+    int rc = iq::check_any_kv(kv, scales, &a.c, &a.scales);
+    if (rc) return rc;
+    rc = iq::check_table(a.c, table, table_ld, max_pages, lens, B, &a.t);
+    if (rc) return rc;
+    return iq::attn_decode(a, q, B, q_heads, scale, window, sinks, out, nullptr, 0, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -10,8 +10,8 @@
 
 namespace iq {
 
-// Kernel-argument copy of iq_kv, strides in elements of 2 bytes (at most
-// 2^30, so that a product with an index is one 32 x 32 bit multiplication).
+// Kernel-argument copy of iq_kv, strides in elements of 2 bytes, or of 1 (at
+// most 2^30, so that a product with an index is one 32 x 32 bit multiplication).
 struct KvView {
     int32_t type, hk, d, ps;
     int64_t pages;
@@ -19,6 +19,15 @@ struct KvView {
     const char* k;
     const char* v;
     PageDiv div;  // by ps
+};
+
+// Kernel-argument copy of iq_kv_scales (block 0: a 16-bit cache).
+struct KvScales {
+    int32_t block;
+    uint32_t pstr, bstr, hstr;
+    float* k;
+    float* v;
+    PageDiv div;  // by block
 };
 
 // A batch's block table: row b's page ids at table + b * ld, at most
@@ -35,6 +44,11 @@ constexpr int kMaxSeqs = 1024;
 // Element offset of (page id, slot, head) in either pool, id in [0, pages).
 __device__ __forceinline__ int64_t kv_element(const KvView& c, uint32_t id, uint32_t slot, uint32_t head) {
     return int64_t(uint64_t(id) * c.pstr + uint64_t(slot) * c.sstr + uint64_t(head) * c.hstr);
+}
+
+// The scale of (page id, slot, head) in either array of scales.
+__device__ __forceinline__ int64_t kv_scale(const KvScales& c, uint32_t id, uint32_t slot, uint32_t head) {
+    return int64_t(uint64_t(id) * c.pstr + uint64_t(page_of(slot, c.div)) * c.bstr + uint64_t(head) * c.hstr);
 }
 
 // Element of a 16-bit cache as fp32, and back (to nearest even).
@@ -72,21 +86,27 @@ inline bool ranges_overlap(const void* a, int64_t abytes, const void* b, int64_t
     return a && b && x < y + uintptr_t(bbytes) && y < x + uintptr_t(abytes);
 }
 
+inline bool is_kv8(int type) { return type == IQ_KV_I8 || type == IQ_KV_E4M3; }
+
+// Strides over n things, of which a single one's is not used, in elements.
+inline bool kv_strides(const int64_t (&n)[3], int64_t (&stride)[3], int64_t unit) {
+    for (int i = 0; i < 3; i++) {
+        if (n[i] == 1) stride[i] = 0;
+        else if (stride[i] < unit || stride[i] > int64_t(1) << 30 || stride[i] % unit) return false;
+    }
+    return true;
+}
+
+// A cache whose rows and strides are whole `unit`s of elements (16 bytes).
 // The limits keep every byte offset (below 2 * 3 * 2^31 * 2^30) inside 64 bits
 // and every page id inside an int32.
-inline int check_kv(const iq_kv* kv, KvView* out) {
-    if (!kv) return IQ_ENULL;
-    if (kv->type != IQ_KV_BF16 && kv->type != IQ_KV_F16) return IQ_EKIND;
+inline int fill_kv(const iq_kv* kv, int unit, KvView* out) {
     if (kv->kv_heads < 1 || kv->kv_heads > 1024 || kv->page_size < 1) return IQ_ESHAPE;
-    if (kv->head_dim < 8 || kv->head_dim > 256 || kv->head_dim % 8) return IQ_ESHAPE;
+    if (kv->head_dim < unit || kv->head_dim > 256 || kv->head_dim % unit) return IQ_ESHAPE;
     if (kv->pages < 1 || kv->pages > 0x7fffffff) return IQ_ESHAPE;
-    // (a stride over a single page, slot or head is not used)
     const int64_t count[3] = {kv->pages, kv->page_size, kv->kv_heads};
     int64_t stride[3] = {kv->page_stride, kv->slot_stride, kv->head_stride};
-    for (int i = 0; i < 3; i++) {
-        if (count[i] == 1) stride[i] = 0;
-        else if (stride[i] < 8 || stride[i] > int64_t(1) << 30 || stride[i] % 8) return IQ_ESHAPE;
-    }
+    if (!kv_strides(count, stride, unit)) return IQ_ESHAPE;
     if (!kv->k || !kv->v) return IQ_ENULL;
     if (reinterpret_cast<uintptr_t>(kv->k) % 16 || reinterpret_cast<uintptr_t>(kv->v) % 16) return IQ_ESHAPE;
     out->type = kv->type;
@@ -100,6 +120,36 @@ inline int check_kv(const iq_kv* kv, KvView* out) {
     out->k = static_cast<const char*>(kv->k);
     out->v = static_cast<const char*>(kv->v);
     out->div = page_div(uint32_t(kv->page_size));
+    return IQ_OK;
+}
+
+// A 16-bit cache.
+inline int check_kv(const iq_kv* kv, KvView* out) {
+    if (!kv) return IQ_ENULL;
+    if (kv->type != IQ_KV_BF16 && kv->type != IQ_KV_F16) return IQ_EKIND;
+    return fill_kv(kv, 8, out);
+}
+
+// A cache of any type, an 8-bit one with its scales.
+inline int check_any_kv(const iq_kv* kv, const iq_kv_scales* sc, KvView* out, KvScales* scales) {
+    *scales = KvScales{};
+    if (!kv) return IQ_ENULL;
+    if (!is_kv8(kv->type)) return check_kv(kv, out);
+    const int rc = fill_kv(kv, 16, out);
+    if (rc) return rc;
+    if (!sc || !sc->k || !sc->v) return IQ_ENULL;
+    if (sc->block < 1 || kv->page_size % sc->block) return IQ_ESHAPE;
+    const int64_t count[3] = {kv->pages, kv->page_size / sc->block, kv->kv_heads};
+    int64_t stride[3] = {sc->page_stride, sc->block_stride, sc->head_stride};
+    if (!kv_strides(count, stride, 1)) return IQ_ESHAPE;
+    if (reinterpret_cast<uintptr_t>(sc->k) % 4 || reinterpret_cast<uintptr_t>(sc->v) % 4) return IQ_ESHAPE;
+    scales->block = sc->block;
+    scales->pstr = uint32_t(stride[0]);
+    scales->bstr = uint32_t(stride[1]);
+    scales->hstr = uint32_t(stride[2]);
+    scales->k = sc->k;
+    scales->v = sc->v;
+    scales->div = page_div(uint32_t(sc->block));
     return IQ_OK;
 }
 

@@ -10,7 +10,8 @@ Mirrors, with the same names, argument meaning and order:
   upload_q                        kernels/model_gpu_internal.cuh:67-83
 
 and, without counterparts in the reference's quantised path, the operators of
-a decode step around it: KvCache, kv_append, attn_decode, kv_evict, logprobs.
+a decode step around it: KvCache, kv_append, kv_extend, kv_read, attn_decode,
+kv_evict, logprobs.
 
 Every call goes through the C ABI of include/iq.h (ctypes); torch is used
 only for device memory and the current stream.  Launches are asynchronous
@@ -81,11 +82,24 @@ class IqKv(ctypes.Structure):
     ]
 
 
+class IqKvScales(ctypes.Structure):
+    """iq_kv_scales (include/iq.h): the scales of an 8-bit cache."""
+    _fields_ = [
+        ("block", ctypes.c_int32),
+        ("page_stride", ctypes.c_int64),
+        ("block_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+    ]
+
+
 # Every function include/iq.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _VP = ctypes.POINTER(IqView)
 _KV = ctypes.POINTER(IqKv)
+_SC = ctypes.POINTER(IqKvScales)
 _INT = ctypes.c_int
 SIGNATURES = {
     "iq_gemv": ([_P, _VP, _P, ctypes.c_int, _I64, _I64, _P, _P], ctypes.c_int),
@@ -104,6 +118,10 @@ SIGNATURES = {
     "iq_chain_destroy": ([_P], None),
     "iq_kv_append": ([_P, _P, _P, _P, _P, _I64, _INT, _P, _INT, _KV, _P, _P], _INT),
     "iq_attn_decode": ([_P, _KV, _P, _I64, _I64, _P, _INT, _INT, ctypes.c_float, _P, _P, _I64, _P], _INT),
+    "iq_kv_extend": ([_P, _P, _P, _I64, _INT, _P, _P, ctypes.c_float, _P, _P, _INT, _KV, _SC, _P, _I64, _I64, _P, _P, _INT,
+                      _P, _P], _INT),
+    "iq_kv_read": ([_KV, _SC, _P, _I64, _I64, _P, _P, _INT, _I64, _INT, _P, _P, _P], _INT),
+    "iq_attn_decode_window": ([_P, _KV, _SC, _P, _I64, _I64, _P, _INT, _INT, ctypes.c_float, _I64, _I64, _P, _P], _INT),
     "iq_kv_evict": ([_KV, _P, _I64, _I64, _P, _INT, _I64, _I64, _P, _I64, _P, _P], _INT),
     "iq_logprobs": ([_P, _I64, _I64, _I64, _P, _INT, _P, _P, _P, _P, _P], _INT),
     "iq_init": ([ctypes.c_int], ctypes.c_int),
@@ -327,7 +345,9 @@ def linear(x, W, bias=None, stream=None):
 
 
 # ------------------------------------------------ the cache of a decode step
-KV_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+KV_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.int8: 2, torch.float8_e4m3fn: 3}
+KV_CODES = (torch.int8, torch.float8_e4m3fn)  # 8-bit codes with scales
+READ_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _addr(t):
@@ -339,34 +359,71 @@ class KvCache:
     [pages, page_size, kv_heads, head_dim], torch.bfloat16 or torch.float16,
     which it keeps alive.  Any memory order of pages, slots and heads (a
     permuted view, a slice of a larger tensor) whose rows of head_dim values
-    are contiguous, with the same strides for k and v."""
+    are contiguous, with the same strides for k and v.
 
-    def __init__(self, k, v):
+    With k and v of torch.int8 or torch.float8_e4m3fn, codes: k_scales and
+    v_scales, float32 [pages, page_size / block, kv_heads] (any strides, the
+    same for both), hold a scale for every `block` slots of a page and head."""
+
+    def __init__(self, k, v, k_scales=None, v_scales=None):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("KvCache: k and v must be [pages, page_size, kv_heads, head_dim] of one shape and type")
         if k.dtype not in KV_TYPES:
-            raise TypeError("KvCache: k and v must be torch.bfloat16 or torch.float16")
-        # (the stride over a single page, slot or head means nothing)
-        strides = [[0 if n == 1 else s for n, s in zip(t.shape, t.stride())] for t in (k, v)]
-        if strides[0] != strides[1] or strides[0][3] not in (0, 1):
+            raise TypeError("KvCache: k and v must be torch.bfloat16, torch.float16, torch.int8 or torch.float8_e4m3fn")
+
+        def strides(t):  # (the stride over a single page, slot or head means nothing)
+            return [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+        st = strides(k)
+        if st != strides(v) or st[3] not in (0, 1):
             raise ValueError("KvCache: k and v need the same strides and contiguous rows of head_dim values")
         self.k, self.v = k, v
         self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
         self.device = k.get_device()
-        if v.get_device() != self.device:
-            raise ValueError("KvCache: k and v must be on one device")
+        self.block = 0
+        self._s = None
+        if k.dtype in KV_CODES:
+            ks, vs = k_scales, v_scales
+            if ks is None or vs is None:
+                raise ValueError("KvCache: codes need k_scales and v_scales")
+            if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+                raise TypeError("KvCache: scales must be torch.float32")
+            if (ks.dim() != 3 or ks.shape != vs.shape or ks.shape[0] != self.pages or ks.shape[2] != self.kv_heads
+                    or ks.shape[1] < 1 or self.page_size % ks.shape[1] or strides(ks) != strides(vs)):
+                raise ValueError("KvCache: scales must be [pages, page_size / block, kv_heads], of the same strides")
+            self.block = self.page_size // ks.shape[1]
+            self._s = IqKvScales(self.block, *strides(ks), ks.data_ptr(), vs.data_ptr())
+        elif k_scales is not None or v_scales is not None:
+            raise ValueError("KvCache: scales belong to a cache of codes")
+        self.k_scales, self.v_scales = k_scales, v_scales
+        for t in (v, k_scales, v_scales):
+            if t is not None and t.get_device() != self.device:
+                raise ValueError("KvCache: k and v must be on one device")
         self._c = IqKv(KV_TYPES[k.dtype], self.kv_heads, self.head_dim, self.page_size, self.pages,
-                       *strides[0][:3], k.data_ptr(), v.data_ptr())
+                       *st[:3], k.data_ptr(), v.data_ptr())
 
     @property
     def c(self):
         return ctypes.byref(self._c)
 
+    @property
+    def scales_c(self):
+        return None if self._s is None else ctypes.byref(self._s)
 
-def alloc_kv(pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
-    """An empty cache (zeros) in the order [pages, page_size, kv_heads, head_dim]."""
+
+def alloc_kv(pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda", block=None):
+    """An empty cache (zeros) in the order [pages, page_size, kv_heads, head_dim];
+    of codes with a scale for every `block` slots (page_size by default)."""
     shape = (pages, page_size, kv_heads, head_dim)
-    return KvCache(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+    scales = (None, None)
+    if dtype in KV_CODES:
+        block = page_size if block is None else block
+        if block < 1 or page_size % block:
+            raise ValueError("alloc_kv: block must divide page_size")
+        scales = [torch.zeros(pages, page_size // block, kv_heads, device=device) for _ in range(2)]
+    elif block is not None:
+        raise ValueError("alloc_kv: block belongs to a cache of codes")
+    return KvCache(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
+                   *scales)
 
 
 def rope_freqs(rot_dim, theta, device="cuda"):
@@ -435,11 +492,11 @@ def kv_append(q, k, v, positions, slots, freqs, cache, q_out=None, stream=None):
     return q_out
 
 
-def _check_table(what, table, lens):
+def _check_table(what, table, lens, name="lens", more=0):
     if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"{what}: table must be int32 [sequences, pages] with contiguous rows")
     B, pages = table.shape
-    _need(what, "lens", lens, torch.int32, B)
+    _need(what, name, lens, torch.int32, B + more)
     ld = table.stride(0) if B > 1 else pages
     return B, pages, ld
 
@@ -453,14 +510,103 @@ def _check_sums(what, weights, B, kv_heads):
     return weights.shape[2]
 
 
-def attn_decode(q, cache, table, lens, out=None, weights=None, scale=None, stream=None):
+def kv_extend(q, k, v, positions, freqs, cache, table, lens, starts=None, q_norm=None, k_norm=None, eps=1e-6,
+              q_out=None, stream=None):
+    """Adds new tokens behind the first lens[b] (int32 [B]) of each sequence,
+    in the pages table[b] (int32 [B, pages]) of a cache of any type: rows
+    starts[b] to starts[b + 1] (int32 [B + 1]; None: one token a sequence) of q
+    [T, heads, head_dim], k and v [T, kv_heads, head_dim], fp32.  Optional norms
+    of every head of q and k (bf16 [head_dim]), then rotary embedding as in
+    kv_append, then k and v are rounded into the cache (an 8-bit one: with its
+    blocks' scales, which grow with their tokens), q into q_out (may be q).  q
+    may be None (cache only).  lens stays as it is.  Returns q_out.
+    include/iq.h, iq_kv_extend."""
+    what = "kv_extend"
+    B, pages, ld = _check_table(what, table, lens)
+    hk, d = cache.kv_heads, cache.head_dim
+    T = k.numel() // (hk * d)
+    _need(what, "k", k, torch.float32, T * hk * d)
+    _need(what, "v", v, torch.float32, T * hk * d)
+    if starts is not None:
+        _need(what, "starts", starts, torch.int32, B + 1)
+    elif T != B:
+        raise ValueError(f"{what}: one token a sequence without starts")
+    rot = 0
+    if freqs is not None:
+        if positions is None:
+            raise ValueError(f"{what}: freqs need positions")
+        _need(what, "freqs", freqs, torch.float64)
+        _need(what, "positions", positions, torch.int64, T)
+        rot = 2 * freqs.numel()
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is not None:
+            if t.dtype not in (torch.bfloat16, torch.int16):
+                raise TypeError(f"{what}: {name} must be bf16 (torch.bfloat16 or int16 bits)")
+            _need(what, name, t, t.dtype, d)
+    heads = 0
+    if q is not None:
+        heads = q.numel() // max(1, T * d)
+        _need(what, "q", q, torch.float32, T * heads * d)
+        if q_out is not None:
+            _need(what, "q_out", q_out, torch.float32, T * heads * d)
+    _on_device(what, cache.device, q, k, v, positions if rot else None, freqs, table, lens, starts, q_norm, k_norm, q_out)
+    if q is not None and q_out is None:
+        q_out = _new(stream, torch.empty_like, q)
+    rc = lib().iq_kv_extend(_addr(q), _addr(k), _addr(v), T, heads, _addr(q_norm), _addr(k_norm), eps,
+                            _addr(positions) if rot else None, _addr(freqs) if rot else None, rot, cache.c,
+                            cache.scales_c, _addr(table), ld, pages, _addr(lens), _addr(starts), B,
+                            _addr(q_out) if heads else None, _stream(stream))
+    _check(rc, "iq_kv_extend")
+    return q_out
+
+
+def kv_read(cache, table, starts, T=None, first=None, dtype=torch.float32, out=None, stream=None):
+    """Cached tokens back as numbers: rows starts[b] to starts[b + 1] (int32 [B
+    + 1]) of the outputs are the tokens first[b] on (int32 [B]; None: 0) in the
+    pages table[b] of a cache of any type.  Returns (k, v), [T, kv_heads,
+    head_dim] of dtype torch.float32, bfloat16 or float16, or `out`, two such
+    tensors (one may be None).  Rows of no sequence are left as they were (zeros
+    in tensors made here), tokens without a page are NaN.  include/iq.h,
+    iq_kv_read."""
+    what = "kv_read"
+    B, pages, ld = _check_table(what, table, starts, "starts", 1)
+    if first is not None:
+        _need(what, "first", first, torch.int32, B)
+    row = cache.kv_heads * cache.head_dim
+    if out is None:
+        if T is None:
+            raise ValueError(f"{what}: T or out is needed")
+        _on_device(what, cache.device, table, starts, first)
+        out = tuple(_new(stream, torch.zeros, T, cache.kv_heads, cache.head_dim, dtype=dtype, device=table.device)
+                    for _ in range(2))
+    k, v = out
+    some = k if k is not None else v
+    if some is None:
+        raise ValueError(f"{what}: out has neither k nor v")
+    T = some.numel() // row if T is None else T
+    if some.dtype not in READ_TYPES:
+        raise TypeError(f"{what}: outputs must be torch.float32, bfloat16 or float16")
+    for name, t in (("k", k), ("v", v)):
+        if t is not None:
+            _need(what, name, t, some.dtype, T * row)
+    _on_device(what, cache.device, table, starts, first, k, v)
+    rc = lib().iq_kv_read(cache.c, cache.scales_c, _addr(table), ld, pages, _addr(first), _addr(starts), B, T,
+                          READ_TYPES[some.dtype], _addr(k), _addr(v), _stream(stream))
+    _check(rc, "iq_kv_read")
+    return k, v
+
+
+def attn_decode(q, cache, table, lens, out=None, weights=None, scale=None, stream=None, window=0, sinks=0):
     """Attention of one token a sequence, q [B, heads, head_dim] fp32, over
     the first lens[b] (int32 [B]) tokens in the pages table[b] (int32 [B,
     pages]) of the cache; heads / kv_heads query heads share a key/value head.
     scale: head_dim^-0.5 by default.  weights: fp32 [B, kv_heads, tokens],
     tokens >= pages * page_size; every cached token's attention weight, summed
-    over the heads that share it, is added to it.  Returns out, shaped as q.
-    include/iq.h, iq_attn_decode."""
+    over the heads that share it, is added to it.  window > 0: a sequence sees
+    its newest `window` tokens and its first `sinks` only, and pages without any
+    of these need not be there.  Returns out, shaped as q.  weights go with
+    16-bit caches and no window.  include/iq.h, iq_attn_decode and
+    iq_attn_decode_window."""
     what = "attn_decode"
     B, pages, ld = _check_table(what, table, lens)
     d = cache.head_dim
@@ -469,12 +615,23 @@ def attn_decode(q, cache, table, lens, out=None, weights=None, scale=None, strea
     wld = 0 if weights is None else _check_sums(what, weights, B, cache.kv_heads)
     if out is not None:
         _need(what, "out", out, torch.float32, B * heads * d)
+    if window < 0 or sinks < 0:
+        raise ValueError(f"{what}: window and sinks must not be negative")
+    plain = not window and cache.block == 0
+    if weights is not None and not plain:
+        raise ValueError(f"{what}: weights are added up over 16-bit caches and without a window")
     _on_device(what, cache.device, q, table, lens, out, weights)
     if out is None:
         out = _new(stream, torch.empty_like, q)
-    rc = lib().iq_attn_decode(_addr(q), cache.c, _addr(table), ld, pages, _addr(lens), B, heads,
-                              d ** -0.5 if scale is None else scale, _addr(out), _addr(weights), wld, _stream(stream))
-    _check(rc, "iq_attn_decode")
+    scale = d ** -0.5 if scale is None else scale
+    if plain:
+        rc = lib().iq_attn_decode(_addr(q), cache.c, _addr(table), ld, pages, _addr(lens), B, heads, scale, _addr(out),
+                                  _addr(weights), wld, _stream(stream))
+        _check(rc, "iq_attn_decode")
+    else:
+        rc = lib().iq_attn_decode_window(_addr(q), cache.c, cache.scales_c, _addr(table), ld, pages, _addr(lens), B,
+                                         heads, scale, window, sinks, _addr(out), _stream(stream))
+        _check(rc, "iq_attn_decode_window")
     return out
 
 
