@@ -188,12 +188,20 @@ class CachedDecodeStep:
     """One decode step of B sequences over paged key/value caches, one
     ops.KvCache a layer: every sequence's next token, at the position and
     cache length that `positions` and `lens` hold, through all layers to
-    logits.  `model` as for DecodeStep, with cfg["theta"] (rotary base).
+    logits.  `model` as for DecodeStep, with cfg["theta"] (rotary base) and, in
+    its layers, optional bf16 tensors q_norm, k_norm [head_dim]: norms of every
+    head of q and k (with cfg["eps"]) ahead of the rotation.
+
+    caches: of any type; an 8-bit one's blocks fill in the order of the steps.
+    window > 0: attention sees the newest `window` tokens in the cache and its
+    first `sinks` only (ops.attn_decode); pages without any of these may be given
+    to other sequences.
 
     table: int32 [B, pages], the pages of every sequence (the same ids in all
     layers); enough of them have to be there before the step that fills them.
     weights: keep the attention weight every cached token has received, per
-    layer [B, kv_heads, pages * page_size], for evict().
+    layer [B, kv_heads, pages * page_size], for evict(); with 16-bit caches and
+    no window.
 
     Device state, which the caller may set between steps: lens (int32 [B],
     tokens of each sequence), positions (int64 [B], of the next token; they
@@ -203,16 +211,24 @@ class CachedDecodeStep:
     last set lens.  step() without a list of ids issues only device work, so it
     can be captured into a graph (after ops.init on the capturing stream)."""
 
-    def __init__(self, model, caches, table, weights=False, device="cuda"):
+    def __init__(self, model, caches, table, weights=False, device="cuda", window=0, sinks=0):
         c = model["cfg"]
         H, I, V = c["hidden"], c["inter"], c["vocab"]
         nh, nkv, hd, L = c["heads"], c["kv_heads"], c["head_dim"], c["layers"]
+        if window < 0 or sinks < 0:
+            raise ValueError("CachedDecodeStep: window and sinks must not be negative")
+        if weights and (window or any(k.block for k in caches)):
+            raise ValueError("CachedDecodeStep: weights are kept over 16-bit caches and without a window")
         if len(caches) != L or any((k.kv_heads, k.head_dim) != (nkv, hd) for k in caches):
             raise ValueError("CachedDecodeStep: one cache a layer, of the model's key/value heads and head size")
         if len({k.page_size for k in caches}) != 1:
             raise ValueError("CachedDecodeStep: caches of one page size")
         B = self.rows = table.shape[0]
         self.model, self.caches, self.table = model, list(caches), table
+        self.window, self.sinks = window, sinks
+        # layers whose tokens are added by kv_extend: 8-bit caches, or norms
+        self._norms = [(Lw.get("q_norm"), Lw.get("k_norm")) for Lw in model["layers"]]
+        self._extends = [bool(k.block) or any(n is not None for n in w) for k, w in zip(caches, self._norms)]
         self.page = caches[0].page_size
         self.pages = min(k.pages for k in caches)
         self.capacity = table.shape[1] * self.page
@@ -226,6 +242,7 @@ class CachedDecodeStep:
         self.held = torch.zeros(B, dtype=torch.int32, device=device)
         self._left = torch.zeros(B, dtype=torch.int32, device=device)  # lens as step() or evict() left it
         self._attend = torch.zeros(B, dtype=torch.int32, device=device)
+        self._behind = torch.zeros(B, dtype=torch.int32, device=device)  # held before the step, -1 without a place
         self._none = torch.full((B,), -1, dtype=torch.int32, device=device)
         self.positions = torch.zeros(B, dtype=torch.int64, device=device)
         self.slots = torch.full((B,), -1, dtype=torch.int64, device=device)
@@ -281,15 +298,23 @@ class CachedDecodeStep:
         # (a row without its token attends to nothing: no length, so that its
         # output is NaN and its weights stay)
         torch.where(stored, self.held, self._none, out=self._attend)
+        if any(self._extends):
+            torch.where(stored, held, self._none, out=self._behind)
         self.lens.add_(self.lens >= 0)
         self._left.copy_(self.lens)
         ops.launch_embedding_q(self.model["embed"], self.ids, self.rows, self.model["cfg"]["hidden"], self.h0)
         self.chains[0].run()
         for li, b in enumerate(self.per_layer):
-            ops.kv_append(b["q"], b["k"], b["v"], self.positions, self.slots, self.freqs, self.caches[li],
-                          q_out=b["q_rot"])
+            if self._extends[li]:
+                q_norm, k_norm = self._norms[li]
+                ops.kv_extend(b["q"], b["k"], b["v"], self.positions, self.freqs, self.caches[li], self.table,
+                              self._behind, q_norm=q_norm, k_norm=k_norm, eps=self.model["cfg"]["eps"],
+                              q_out=b["q_rot"])
+            else:
+                ops.kv_append(b["q"], b["k"], b["v"], self.positions, self.slots, self.freqs, self.caches[li],
+                              q_out=b["q_rot"])
             ops.attn_decode(b["q_rot"], self.caches[li], self.table, self._attend, out=b["attn"],
-                            weights=self.weights[li] if self.weights else None)
+                            weights=self.weights[li] if self.weights else None, window=self.window, sinks=self.sinks)
             self.chains[li + 1].run()
         self.positions.add_(stored)
 
