@@ -367,9 +367,10 @@ int iq_kv_extend(const float* q, const float* k, const float* v, int64_t T, int 
                  int64_t max_pages, const int32_t* lens, const int32_t* starts, int B, float* q_out, void* stream);
 
 /* Cached tokens back as numbers: rows starts[b] <= t < starts[b + 1] of k_out
- * and v_out ([T][kv_heads][head_dim], one of them may be NULL) become sequence
+ * and v_out ([T][kv_heads][head_dim], 16-byte aligned, one of them may be NULL) become sequence
  * b's tokens first[b], first[b] + 1, ... (first NULL: 0).  out_type IQ_READ_*; a
- * code times its scale is rounded once, to nearest even.  Rows that belong to no
+ * code times its scale is an fp32 product, then rounded to the type, both to
+ * nearest even.  Rows that belong to no
  * sequence are left as they were; a token outside the table, or in a page whose
  * id lies outside [0, pages), is NaN. */
 enum { IQ_READ_F32 = 0, IQ_READ_BF16 = 1, IQ_READ_F16 = 2 };

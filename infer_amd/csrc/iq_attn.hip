@@ -69,18 +69,22 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     const int t0 = int(it.j * it.c) * kAttnTile, t1 = t0 + min(it.seen - t0, int(it.c) * kAttnTile);
     const int ntiles = (t1 - t0 + kAttnTile - 1) / kAttnTile;
 
-    // row r of a tile: element offset of its (page, slot), 0 where there is none
+    // token r of a tile and its page's id (0 past the end), and from these the
+    // element offset of its (page, slot), 0 where there is none
     bool poison = false;
     const int32_t* table = a.t.table + b * a.t.ld;
-    auto row_offset = [&](int tile) -> int64_t {
-        int tok = t0 + tile * kAttnTile + (lane & 31);
-        if (tok >= t1) return 0;
-        if (WIN && tok >= a.sinks) tok += n - it.seen;
-        const uint32_t p = page_of(uint32_t(tok), a.c.div), s = uint32_t(tok) - p * uint32_t(a.c.ps);
-        const int32_t id = table[p];
-        const bool ok = id >= 0 && id < a.c.pages;
-        poison |= !ok;
-        return ok ? kv_element(a.c, uint32_t(id), s, 0) : 0;
+    auto token = [&](int tile) {
+        const int tok = t0 + tile * kAttnTile + (lane & 31);
+        return WIN && tok >= a.sinks ? tok + (n - it.seen) : tok;
+    };
+    auto page_id = [&](int tile) -> int32_t {
+        return t0 + tile * kAttnTile + (lane & 31) < t1 ? table[page_of(uint32_t(token(tile)), a.c.div)] : 0;
+    };
+    auto row_offset = [&](int tile, int32_t id) -> int64_t {
+        const uint32_t tok = uint32_t(token(tile)), s = tok - page_of(tok, a.c.div) * uint32_t(a.c.ps);
+        const bool live = t0 + tile * kAttnTile + (lane & 31) < t1, ok = id >= 0 && id < a.c.pages;
+        poison |= live && !ok;
+        return live && ok ? kv_element(a.c, uint32_t(id), s, 0) : 0;
     };
     // chunks past the row's end repeat its first one (q is 0 there, and the
     // sums of those columns are not written)
@@ -109,7 +113,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     // The chain of loads that nothing shortens is length, page id, rows: q,
     // needed last, is requested behind the first page ids and cut while the
     // first rows come.
-    const int64_t off0 = row_offset(wave);
+    const int32_t id0 = page_id(wave);
+    int32_t next_id = page_id(wave + kAttnWaves);
     // q: column = head, 8 values of each 32-value step a lane
     s16x8_t qt[KC][T::N];
     float mul = a.mul;
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
 #pragma unroll
             for (int i = 0; i < 8; i++) x[c][i] = q[(e < d ? e : 0) + i];
         }
-        if (wave < ntiles) load(off0);
+        if (wave < ntiles) load(row_offset(wave, id0));
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const bool in = col < gh && c * 32 + g * 8 < d;
@@ -155,7 +160,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     float m = kNone, l = 0.0f;
     float* sc = a.sc ? a.sc + ((int64_t(b) * a.c.hk + j) * a.t.cap) * a.group + h0 + col : nullptr;
 
-    int64_t off_next = wave + kAttnWaves < ntiles ? row_offset(wave + kAttnWaves) : 0;
     for (int tile = wave; tile < ntiles; tile += kAttnWaves) {
         const int tk = t0 + tile * kAttnTile;  // first token
         const bool whole = tk + kAttnTile <= t1;
@@ -168,8 +172,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
             *reinterpret_cast<u32x4_t*>(vl + r * ROWB + (ch ^ vsw(r)) * 16) = whole || tk + r < t1 ? vr[i] : zero;
         }
         if (tile + kAttnWaves < ntiles) {
-            load(off_next);
-            if (tile + 2 * kAttnWaves < ntiles) off_next = row_offset(tile + 2 * kAttnWaves);
+            // (the id behind it first: a wait for it then leaves the tile's loads in flight)
+            const int64_t off = row_offset(tile + kAttnWaves, next_id);
+            next_id = page_id(tile + 2 * kAttnWaves);
+            load(off);
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
@@ -222,7 +228,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
         T::cut(p, pt);
 #pragma unroll
         for (int v = 0; v < VT; v++) {
-            if (v * 16 >= d) continue;
             // rows 4g..4g+3 of either half: lane 4r + c of 16 gives row r's
             // 8-byte piece c, lane i gets the 4 rows' value of column i
             s16x8_t av;

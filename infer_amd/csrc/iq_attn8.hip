@@ -53,6 +53,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
     using T = Terms<IQ_KV_BF16>;
     constexpr int CH = DP / 16, RPI = 64 / CH, NI = kAttnTile / RPI;  // 16-byte chunks of a row, rows of a load, loads
     constexpr int KC = DP / 32, VT = DP / 16;                         // steps of the first product, tiles of the second
+#ifndef IQ_D8
+#define IQ_D8 1
+#endif
+    constexpr int DEPTH = IQ_D8;
     constexpr int KVB = kAttnTile * DP;
     constexpr int OST = DP + 4;  // floats from head to head of a wave's sums
     constexpr int WB = 2 * KVB > 16 * OST * 4 ? 2 * KVB : 16 * OST * 4;
@@ -76,21 +80,25 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
     const int t0 = int(it.j * it.c) * kAttnTile, t1 = t0 + min(it.seen - t0, int(it.c) * kAttnTile);
     const int ntiles = (t1 - t0 + kAttnTile - 1) / kAttnTile;
 
-    // row r of a tile: element offset of its (page, slot) and its scales'; 0 where there is none
+    // token r of a tile and its page's id (0 past the end), and from these the
+    // element offset of its (page, slot) and its scales'; 0 where there is none
     bool poison = false;
     const int32_t* table = a.t.table + b * a.t.ld;
     struct Row {
         int64_t at, scale;
     };
-    auto row_of = [&](int tile) -> Row {
-        int tok = t0 + tile * kAttnTile + (lane & 31);
-        if (tok >= t1) return {0, 0};
-        if (WIN && tok >= a.sinks) tok += n - it.seen;
-        const uint32_t p = page_of(uint32_t(tok), a.c.div), s = uint32_t(tok) - p * uint32_t(a.c.ps);
-        const int32_t id = table[p];
-        const bool ok = id >= 0 && id < a.c.pages;
-        poison |= !ok;
-        if (!ok) return {0, 0};
+    auto token = [&](int tile) {
+        const int tok = t0 + tile * kAttnTile + (lane & 31);
+        return WIN && tok >= a.sinks ? tok + (n - it.seen) : tok;
+    };
+    auto page_id = [&](int tile) -> int32_t {
+        return t0 + tile * kAttnTile + (lane & 31) < t1 ? table[page_of(uint32_t(token(tile)), a.c.div)] : 0;
+    };
+    auto row_of = [&](int tile, int32_t id) -> Row {
+        const uint32_t tok = uint32_t(token(tile)), s = tok - page_of(tok, a.c.div) * uint32_t(a.c.ps);
+        const bool live = t0 + tile * kAttnTile + (lane & 31) < t1, ok = id >= 0 && id < a.c.pages;
+        poison |= live && !ok;
+        if (!live || !ok) return {0, 0};
         return {kv_element(a.c, uint32_t(id), s, 0), kv_scale(a.scales, uint32_t(id), s, uint32_t(j))};
     };
     // chunks past the row's end repeat its first one (q is 0 there, and the
@@ -99,16 +107,19 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
     const int64_t lane_off = int64_t(uint64_t(j) * a.c.hstr) + chsrc * 16;
     const char* kp = a.c.k + lane_off;
     const char* vp = a.c.v + lane_off;
-    u32x4_t kr[NI], vr[NI];
-    float ks, vs;
-    auto load = [&](Row r) {
-        ks = a.scales.k[r.scale];
-        vs = a.scales.v[r.scale];
+    struct Tile {
+        u32x4_t k[NI], v[NI];
+        float ks, vs;
+    };
+    Tile ahead[DEPTH];
+    auto load = [&](Tile& t, Row r) {
+        t.ks = a.scales.k[r.scale];
+        t.vs = a.scales.v[r.scale];
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const int64_t o = __shfl(r.at, i * RPI + lane / CH);
-            kr[i] = *reinterpret_cast<const u32x4_t*>(kp + o);
-            vr[i] = *reinterpret_cast<const u32x4_t*>(vp + o);
+            t.k[i] = *reinterpret_cast<const u32x4_t*>(kp + o);
+            t.v[i] = *reinterpret_cast<const u32x4_t*>(vp + o);
         }
     };
     // Chunk c of row r lies at chunk c ^ swizzle(r) of the row's place.  A K
@@ -120,7 +131,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
     char* kl = lds[wave];
     char* vl = lds[wave] + KVB;
 
-    const Row row0 = row_of(wave);
+    int32_t ids[DEPTH], next_id = 0;
+#pragma unroll
+    for (int i = 0; i < DEPTH; i++) ids[i] = page_id(wave + i * kAttnWaves);
+    next_id = page_id(wave + DEPTH * kAttnWaves);
     // q: column = head, 8 values of each 32-value step a lane
     s16x8_t qt[KC][T::N];
     {
@@ -134,7 +148,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
 #pragma unroll
             for (int i = 0; i < 8; i++) x[c][i] = q[(e < d ? e : 0) + i];
         }
-        if (wave < ntiles) load(row0);
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++)
+            if (wave + i * kAttnWaves < ntiles) load(ahead[i], row_of(wave + i * kAttnWaves, ids[i]));
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const bool in = col < gh && first_of(c) < d;
@@ -149,26 +165,26 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
     for (int i = 0; i < VT; i++) o[i] = float4_t{0, 0, 0, 0};
     float m = kNone, l = 0.0f;
 
-    Row next = {0, 0};
-    if (wave + kAttnWaves < ntiles) next = row_of(wave + kAttnWaves);
-    for (int tile = wave; tile < ntiles; tile += kAttnWaves) {
+    auto step = [&](int tile, Tile& t) {
         const int tk = t0 + tile * kAttnTile;  // first token
         const bool whole = tk + kAttnTile <= t1;
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const int r = i * RPI + lane / CH;
-            *reinterpret_cast<u32x4_t*>(kl + r * DP + (ch ^ ksw(r)) * 16) = kr[i];
+            *reinterpret_cast<u32x4_t*>(kl + r * DP + (ch ^ ksw(r)) * 16) = t.k[i];
             // (a row past the end may hold anything: 0 times NaN is NaN)
             const u32x4_t zero = {0, 0, 0, 0};
-            *reinterpret_cast<u32x4_t*>(vl + r * DP + (ch ^ vsw(r)) * 16) = whole || tk + r < t1 ? vr[i] : zero;
+            *reinterpret_cast<u32x4_t*>(vl + r * DP + (ch ^ vsw(r)) * 16) = whole || tk + r < t1 ? t.v[i] : zero;
         }
         if (lane < kAttnTile) {
-            tile_ks[wave][lane] = ks * a.mul;
-            tile_vs[wave][lane] = tk + lane < t1 ? vs : 0.0f;
+            tile_ks[wave][lane] = t.ks * a.mul;
+            tile_vs[wave][lane] = tk + lane < t1 ? t.vs : 0.0f;
         }
-        if (tile + kAttnWaves < ntiles) {
-            load(next);
-            if (tile + 2 * kAttnWaves < ntiles) next = row_of(tile + 2 * kAttnWaves);
+        if (tile + DEPTH * kAttnWaves < ntiles) {
+            // (the id behind it first: a wait for it then leaves the tile's loads in flight)
+            const Row r = row_of(tile + DEPTH * kAttnWaves, next_id);
+            next_id = page_id(tile + (DEPTH + 1) * kAttnWaves);
+            load(t, r);
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
@@ -224,7 +240,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
         T::cut(w, pt);
 #pragma unroll
         for (int v = 0; v < VT; v++) {
-            if (v * 16 >= d) continue;
             // rows 4g..4g+3 of either half: lane 2r + c of 16 gives row r's
             // 8-byte piece c, lane i gets the 8 rows' value of column i
             const int r8 = col >> 1, r = (r8 >> 2) * 16 + g * 4 + (r8 & 3);
@@ -238,6 +253,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
+    };
+    for (int tile = wave; tile < ntiles;) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++) {
+            step(tile, ahead[i]);
+            tile += kAttnWaves;
+            if (tile >= ntiles) break;
+        }
     }
     // the waves' results; the tiles' places are free once every wave is here
     l += __shfl_xor(l, 16);
@@ -294,7 +317,12 @@ void launch(const AttnArgs& a, unsigned grid, hipStream_t s) {
 
 }  // namespace
 
-int attn8_groups(int head_dim) { return head_dim <= 32 ? 4 : head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1; }
+int attn8_groups(int head_dim) { 
+#ifdef IQ_G8
+    return IQ_G8;
+#endif
+    return head_dim <= 32 ? 4 : head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
+}
 
 void launch_attn8(const AttnArgs& a, bool window, unsigned grid, hipStream_t s) {
     if (a.c.type == IQ_KV_I8) (window ? launch<IQ_KV_I8, true> : launch<IQ_KV_I8, false>)(a, grid, s);

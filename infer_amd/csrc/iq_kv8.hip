@@ -373,83 +373,113 @@ struct ReadArgs {
 
 constexpr int kReadRows = 16;
 
-// 16 bytes of a cache as numbers: N values.
+// N values from their codes (or 16-bit values), N * their size bytes.
 template <int TYPE, int N>
-__device__ __forceinline__ void numbers(u32x4_t x, float s, float (&y)[N]) {
+__device__ __forceinline__ void numbers(const char* src, float s, float (&y)[N]) {
+    if constexpr (TYPE == IQ_KV_I8 || TYPE == IQ_KV_E4M3) {
+        uint32_t x[N / 4];
+        __builtin_memcpy(x, __builtin_assume_aligned(src, N), N);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (TYPE == IQ_KV_I8) {
+        for (int i = 0; i < N / 4; i++) {
+            if constexpr (TYPE == IQ_KV_I8) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[i * 4 + r] = float(int8_t(x[i] >> (8 * r))) * s;
-        } else if constexpr (TYPE == IQ_KV_E4M3) {
-            y[i * 4 + 0] = __builtin_amdgcn_cvt_f32_fp8(x[i], 0) * s;
-            y[i * 4 + 1] = __builtin_amdgcn_cvt_f32_fp8(x[i], 1) * s;
-            y[i * 4 + 2] = __builtin_amdgcn_cvt_f32_fp8(x[i], 2) * s;
-            y[i * 4 + 3] = __builtin_amdgcn_cvt_f32_fp8(x[i], 3) * s;
-        } else {
+                for (int r = 0; r < 4; r++) y[i * 4 + r] = float(int8_t(x[i] >> (8 * r))) * s;
+            } else {
+                y[i * 4 + 0] = __builtin_amdgcn_cvt_f32_fp8(x[i], 0) * s;
+                y[i * 4 + 1] = __builtin_amdgcn_cvt_f32_fp8(x[i], 1) * s;
+                y[i * 4 + 2] = __builtin_amdgcn_cvt_f32_fp8(x[i], 2) * s;
+                y[i * 4 + 3] = __builtin_amdgcn_cvt_f32_fp8(x[i], 3) * s;
+            }
+        }
+    } else {
+        uint32_t x[N / 2];
+        __builtin_memcpy(x, __builtin_assume_aligned(src, 2 * N), 2 * N);
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
             y[i * 2] = kv_to_f32<TYPE>(uint16_t(x[i]));
             y[i * 2 + 1] = kv_to_f32<TYPE>(uint16_t(x[i] >> 16));
         }
     }
 }
 
-// One workgroup per `rows` rows of the outputs, whose places it finds first
-// (a row's sequence is the number of sequences that end at or before it).
+// One workgroup per `rows` rows of the outputs.  Its first wave finds the rows'
+// places, a lane each (a row's sequence is the number of sequences that end at or
+// before it); then a thread has one 16-byte column of the outputs' rows, k's and v's
+// (or several, where a row has more than the workgroup threads), and goes
+// through the rows, so that neighbouring threads write neighbouring bytes.
 template <int TYPE, int OUT>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
     constexpr bool kCodes = TYPE == IQ_KV_I8 || TYPE == IQ_KV_E4M3;
-    constexpr int kSize = kCodes ? 1 : 2, N = 16 / kSize, kOut = OUT == IQ_READ_F32 ? 4 : 2;
-    __shared__ int64_t at[kReadRows], scale_at[kReadRows];  // at: -1 NaN, -2 none
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int kSize = kCodes ? 1 : 2, kOut = OUT == IQ_READ_F32 ? 4 : 2, N = 16 / kOut;
+    struct Place {
+        int64_t at, scale;  // at: -1 NaN, -2 none
+    };
+    __shared__ Place places[kReadRows];
+    const int tid = threadIdx.x, lane = tid & 63;
     const int64_t r0 = a.r0 + int64_t(blockIdx.x) * a.rows;
-    for (int r = wave; r < a.rows; r += kThreads / 64) {
-        const int64_t row = r0 + r;
+    if (tid < 64) {
         int b = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 64)
-            b += __popcll(__ballot(b0 + lane < a.B && a.starts[min(b0 + lane, a.B - 1) + 1] <= row));
-        if (lane == 0) {
-            int64_t to = -2, sc = 0;
-            if (row < a.T && b < a.B && row >= a.starts[b]) {
-                const int64_t tok = (a.t.lens ? int64_t(a.t.lens[b]) : 0) + (row - a.starts[b]);
-                to = -1;
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
+            const int end = a.starts[min(b0 + lane, a.B - 1) + 1];
+            for (int r = 0; r < a.rows; r++) {
+                const int n = __popcll(__ballot(b0 + lane < a.B && end <= r0 + r));
+                if (lane == r) b += n;
+            }
+        }
+        if (lane < a.rows) {
+            const int64_t row = r0 + lane;
+            Place p{-2, 0};
+            const int start = a.starts[min(b, a.B)];
+            if (row < a.T && b < a.B && row >= start) {
+                const int64_t tok = (a.t.lens ? int64_t(a.t.lens[b]) : 0) + (row - start);
+                p.at = -1;
                 if (tok >= 0 && tok < a.t.cap) {
-                    const uint32_t p = page_of(uint32_t(tok), a.c.div), slot = uint32_t(tok) - p * uint32_t(a.c.ps);
-                    const int32_t id = a.t.table[b * a.t.ld + p];
+                    const uint32_t g = page_of(uint32_t(tok), a.c.div), slot = uint32_t(tok) - g * uint32_t(a.c.ps);
+                    const int32_t id = a.t.table[b * a.t.ld + g];
                     if (id >= 0 && id < a.c.pages) {
-                        to = kv_element(a.c, uint32_t(id), slot, 0);
-                        if (kCodes) sc = kv_scale(a.sc, uint32_t(id), slot, 0);
+                        p.at = kv_element(a.c, uint32_t(id), slot, 0);
+                        if (kCodes) p.scale = kv_scale(a.sc, uint32_t(id), slot, 0);
                     }
                 }
             }
-            at[r] = to;
-            scale_at[r] = sc;
+            places[lane] = p;
         }
     }
     __syncthreads();
-    const int per = a.c.d / N, row_units = a.c.hk * per, units = a.rows * row_units;
-    for (int i = tid; i < 2 * units; i += kThreads) {
-        const bool is_v = i >= units;
-        const int u = is_v ? i - units : i, r = u / row_units, x = u - r * row_units, h = x / per, e = (x - h * per) * N;
-        char* out = is_v ? a.v : a.k;
-        const int64_t from = at[r];
-        if (!out || from == -2) continue;
-        float y[N];
-        if (from < 0) {
+    const int per = a.c.d / N, half = a.c.hk * per, pools = (a.k != nullptr) + (a.v != nullptr);
+    const int cols = half * pools, way = min(cols, kThreads), lanes = kThreads / way;
+    if (tid >= way * lanes) return;
+    for (int x = tid % way; x < cols; x += way) {
+        const bool is_v = x >= half || !a.k;
+        const int u = x >= half ? x - half : x, h = u / per, e = (u - h * per) * N;
+        const char* src = (is_v ? a.c.v : a.c.k) + kSize * (int64_t(uint64_t(uint32_t(h)) * a.c.hstr) + e);
+        const float* scales = (is_v ? a.sc.v : a.sc.k) + int64_t(uint64_t(uint32_t(h)) * a.sc.hstr);
+        char* to = (is_v ? a.v : a.k) + (r0 * half + u) * 16;
+#pragma unroll 4
+        for (int r = tid / way; r < a.rows; r += lanes) {
+            const Place p = places[r];
+            if (p.at == -2) continue;
+            const int64_t from = p.at < 0 ? 0 : p.at;
+            const float s = p.at < 0 ? __builtin_nanf("") : kCodes ? scales[p.scale] : 1.0f;
+            float y[N];
+            numbers<TYPE, N>(src + kSize * from, s, y);
+            // (the product is fp32's: without this its rounding is merged with fp16's)
 #pragma unroll
-            for (int k = 0; k < N; k++) y[k] = __builtin_nanf("");
-        } else {
-            const char* src = (is_v ? a.c.v : a.c.k) + kSize * (from + int64_t(uint64_t(h) * a.c.hstr) + e);
-            const float s = kCodes ? (is_v ? a.sc.v : a.sc.k)[scale_at[r] + int64_t(uint64_t(h) * a.sc.hstr)] : 1.0f;
-            numbers<TYPE>(*reinterpret_cast<const u32x4_t*>(src), s, y);
-        }
-        char* to = out + (((r0 + r) * a.c.hk + h) * a.c.d + e) * kOut;
-        if constexpr (OUT == IQ_READ_F32) {
+            for (int k = 0; k < N; k++) asm("" : "+v"(y[k]));
+            u32x4_t out;
+            if constexpr (OUT == IQ_READ_F32) {
 #pragma unroll
-            for (int k = 0; k < N; k++) reinterpret_cast<float*>(to)[k] = y[k];
-        } else {
+                for (int k = 0; k < 4; k++) out[k] = __float_as_uint(y[k]);
+            } else {
+                constexpr int T16 = OUT == IQ_READ_BF16 ? IQ_KV_BF16 : IQ_KV_F16;
 #pragma unroll
-            for (int k = 0; k < N; k++)
-                reinterpret_cast<uint16_t*>(to)[k] = f32_to_kv<OUT == IQ_READ_BF16 ? IQ_KV_BF16 : IQ_KV_F16>(y[k]);
+                for (int k = 0; k < 4; k++) out[k] = f32_to_kv<T16>(y[2 * k]) | uint32_t(f32_to_kv<T16>(y[2 * k + 1])) << 16;
+            }
+            if (!kCodes && p.at < 0) {  // (codes: the scale)
+                constexpr uint32_t nan = OUT == IQ_READ_F32 ? 0x7fc00000u : OUT == IQ_READ_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
+                out = u32x4_t{nan, nan, nan, nan};
+            }
+            *reinterpret_cast<u32x4_t*>(to + int64_t(r) * half * 16) = out;
         }
     }
 }
@@ -547,6 +577,7 @@ int iq_kv_read(const iq_kv* kv, const iq_kv_scales* scales, const int32_t* table
     if (T > iq::kMostRows) return IQ_ETOOLARGE;
     if (!k_out && !v_out) return IQ_ENULL;
     const int64_t bytes = T * a.c.hk * a.c.d * (out_type == IQ_READ_F32 ? 4 : 2);
+    if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16) return IQ_ESHAPE;
     if (iq::ranges_overlap(k_out, bytes, v_out, bytes)) return IQ_EALIAS;
     a.t.lens = first;
     a.starts = starts;
