@@ -12,9 +12,9 @@ namespace {
 // rounded up to 8 W): two runs of 4, the halves of 4 rotary pairs, or
 // neighbours.
 constexpr int kThreads = 256;
-constexpr int kSpan = 16;     // tokens of a 16-bit cache's unit
-constexpr int kChunk = 16;    // tokens whose angles a workgroup holds
-constexpr int kMaxHeads = 16; // heads of a workgroup
+constexpr int kSpan = 16;      // tokens of a 16-bit cache's unit
+constexpr int kMaxHeads = 16;  // heads of a workgroup
+constexpr int kHeld = 4;       // rows that a thread can hold
 
 struct ExtendArgs {
     const float *q, *k, *v;
@@ -33,7 +33,7 @@ struct ExtendArgs {
     PageDiv span_div;
     uint32_t groups;      // of the 2 hk rows that a token has in the cache
     int heads;            // of a group
-    uint32_t qgroups;     // of 16 query heads
+    uint32_t qgroups;     // of the query heads
     int64_t cached;       // workgroups of the cache's part, then T * qgroups
     int64_t w0;           // first workgroup of this launch
 };
@@ -53,15 +53,6 @@ struct Unit {
 };
 
 __device__ __forceinline__ bool find_unit(const ExtendArgs& a, uint32_t u, Unit* it) {
-    if (!a.starts) {
-        it->b = int(u);
-        it->tok = a.t.lens[u];
-        it->count = 1;
-        it->row = u;
-        if (it->tok < 0 || it->tok >= a.t.cap) return false;
-        it->begin = int(page_of(uint32_t(it->tok), a.span_div)) * a.span;
-        return true;
-    }
     const int lane = threadIdx.x & 63;
     uint32_t before = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -89,91 +80,137 @@ __device__ __forceinline__ bool find_unit(const ExtendArgs& a, uint32_t u, Unit*
     return false;
 }
 
-// A thread's two runs of 4 values of a row.
+// 4 values of any alignment (their own).
+typedef float float4u_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t ushort4u_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// A thread's two runs of 4 values of a row.  A thread past the row's end (on
+// false) reads the row's first ones and takes them as 0.
 struct Runs {
     int e0, e1;
     bool turn, on;
 };
 __device__ __forceinline__ Runs runs_of(int i, int rot, int d) {
     Runs r;
+    r.on = i * 2 < d;
+    if (!r.on) i = 0;
     r.turn = i < rot / 2;
     r.e0 = r.turn ? i : rot + (i - rot / 2) * 2;
     r.e1 = r.turn ? i + rot / 2 : r.e0 + 4;
-    r.on = i * 2 < d;
     return r;
 }
 
-// One head's row: loaded, normed (norm may be null), turned by cs.
-template <int W>
-__device__ __forceinline__ void make_row(const float* src, const Runs& p, const uint16_t* norm, float eps, int d,
-                                         const float2* cs, float (&y0)[4], float (&y1)[4]) {
-    float x0[4], x1[4];
+__device__ __forceinline__ void load_row(const float* src, const Runs& p, float (&x)[8]) {
+    const float4u_t a = *reinterpret_cast<const float4u_t*>(src + p.e0), b = *reinterpret_cast<const float4u_t*>(src + p.e1);
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        x0[r] = p.on ? src[p.e0 + r] : 0.0f;
-        x1[r] = p.on ? src[p.e1 + r] : 0.0f;
-    }
-    if (norm) {
-        // squares and their root in 64 bits: no x in fp32's range over- or underflows
-        double ss = 0.0;
-#pragma unroll
-        for (int r = 0; r < 4; r++) ss += double(x0[r]) * x0[r] + double(x1[r]) * x1[r];
-        ss = over_row<W>(ss, [](double u, double v) { return u + v; });
-        const double inv = 1.0 / sqrt(ss / d + double(eps));
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            x0[r] = float(x0[r] * inv) * bf16_to_f32(p.on ? norm[p.e0 + r] : 0);
-            x1[r] = float(x1[r] * inv) * bf16_to_f32(p.on ? norm[p.e1 + r] : 0);
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const float2 w = p.turn ? cs[p.e0 + r] : make_float2(1.0f, 0.0f);
-        y0[r] = p.turn ? x0[r] * w.x - x1[r] * w.y : x0[r];
-        y1[r] = p.turn ? x1[r] * w.x + x0[r] * w.y : x1[r];
+        x[r] = p.on ? a[r] : 0.0f;
+        x[4 + r] = p.on ? b[r] : 0.0f;
     }
 }
 
-// The cosines and sines of `tokens` tokens from row t on (at most kChunk).  The
-// angle is reduced to a fraction of a turn in 64 bits: in 32 a far position's
-// has lost its last bits.
-__device__ __forceinline__ void make_angles(const ExtendArgs& a, int64_t t, int tokens, float2 (*cs)[128]) {
-    const int half = a.rot / 2;
-    for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
-        const int k = i / half, e = i - k * half;
-        const double turns = double(a.pos[t + k]) * a.freqs[e] * 0.15915494309189533577;
-        const float r = float((turns - rint(turns)) * 6.28318530717958647693);
-        cs[k][e] = make_float2(cosf(r), sinf(r));
+__device__ __forceinline__ void store_row(float* dst, const Runs& p, const float (&x)[8]) {
+    if (!p.on) return;
+    *reinterpret_cast<float4u_t*>(dst + p.e0) = float4u_t{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<float4u_t*>(dst + p.e1) = float4u_t{x[4], x[5], x[6], x[7]};
+}
+
+// x / sqrt(mean(x^2) + eps) * norm; the squares and their root in 64 bits: no x
+// in fp32's range over- or underflows.
+template <int W>
+__device__ __forceinline__ void norm_row(float (&x)[8], const Runs& p, const uint16_t* norm, float eps, int d) {
+    const ushort4u_t n0 = *reinterpret_cast<const ushort4u_t*>(norm + p.e0), n1 = *reinterpret_cast<const ushort4u_t*>(norm + p.e1);
+    double ss = 0.0;
+#pragma unroll
+    for (int r = 0; r < 8; r++) ss += double(x[r]) * x[r];
+    ss = over_row<W>(ss, [](double u, double v) { return u + v; });
+    const double inv = 1.0 / sqrt(ss / d + double(eps));
+#pragma unroll
+    for (int r = 0; r < 8; r++) x[r] = float(x[r] * inv) * bf16_to_f32(r < 4 ? n0[r] : n1[r - 4]);
+}
+
+// Cosine and sine of pos * freq.  The angle is reduced to a part of a quarter turn
+// in 64 bits (in 32 a far position's has lost its last bits), y in -pi/4..pi/4;
+// there the series up to y^9 and y^10 are off by less than 2^-29.
+__device__ __forceinline__ float2 angle(double pos, double freq) {
+    double t = pos * freq * 0.15915494309189533577;
+    t = (t - rint(t)) * 4.0;
+    const double quarter = rint(t);
+    const float y = float(t - quarter) * 1.57079632679489661923f, z = y * y;
+    const float s = y * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), 1.0f);
+    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+    const int q = int(quarter);
+    const float a = q & 1 ? s : c, b = q & 1 ? c : s;
+    return make_float2((q + 1) & 2 ? -a : a, q & 2 ? -b : b);
+}
+
+// The pairs turned by w.
+__device__ __forceinline__ void turn_row(float (&x)[8], const Runs& p, const float2 (&w)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const float u = x[r], v = x[4 + r];
+        x[r] = p.turn ? u * w[r].x - v * w[r].y : u;
+        x[4 + r] = p.turn ? v * w[r].x + u * w[r].y : v;
     }
+}
+
+template <int W>
+__device__ __forceinline__ uint32_t largest(const float (&x)[8]) {  // |x|'s bits: NaN above infinity
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) big = max(big, __float_as_uint(fabsf(x[i])));
+    return over_row<W>(big, [](uint32_t u, uint32_t v) { return max(u, v); });
 }
 
 template <int TYPE>
 constexpr float kMostCode = TYPE == IQ_KV_I8 ? 127.0f : 448.0f;
 
-// 4 values as codes (or 16-bit values), to nearest even; s: the block's scale.
+// A thread's values as codes (or 16-bit values), to nearest even; s: the
+// block's scale.
 template <int TYPE>
-__device__ __forceinline__ void put4(char* at, const float (&y)[4], float s) {
-    if constexpr (TYPE == IQ_KV_I8 || TYPE == IQ_KV_E4M3) {
-        float c[4];
+__device__ __forceinline__ void put8(char* row, const Runs& p, const float (&x)[8], float s) {
 #pragma unroll
-        for (int r = 0; r < 4; r++)  // (no scale: zeros, and what a NaN block holds)
-            c[r] = s > 0.0f ? fminf(fmaxf(y[r] / s, -kMostCode<TYPE>), kMostCode<TYPE>) : 0.0f;
-        uint32_t u;
-        if constexpr (TYPE == IQ_KV_I8) {
-            u = 0;
+    for (int half = 0; half < 2; half++) {
+        const int e = half ? p.e1 : p.e0;
+        if constexpr (TYPE == IQ_KV_I8 || TYPE == IQ_KV_E4M3) {
+            float c[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) u |= (uint32_t(int(rintf(c[r]))) & 255u) << (8 * r);
+            for (int r = 0; r < 4; r++)  // (no scale: zeros, and what a NaN block holds)
+                c[r] = s > 0.0f ? fminf(fmaxf(x[half * 4 + r] / s, -kMostCode<TYPE>), kMostCode<TYPE>) : 0.0f;
+            uint32_t u;
+            if constexpr (TYPE == IQ_KV_I8) {
+                u = 0;
+#pragma unroll
+                for (int r = 0; r < 4; r++) u |= (uint32_t(int(rintf(c[r]))) & 255u) << (8 * r);
+            } else {
+                const int v = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+                u = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], v, true));
+            }
+            *reinterpret_cast<uint32_t*>(row + e) = u;
         } else {
-            int v = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
-            u = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], v, true));
+            uint2 u;
+            u.x = f32_to_kv<TYPE>(x[half * 4]) | uint32_t(f32_to_kv<TYPE>(x[half * 4 + 1])) << 16;
+            u.y = f32_to_kv<TYPE>(x[half * 4 + 2]) | uint32_t(f32_to_kv<TYPE>(x[half * 4 + 3])) << 16;
+            *reinterpret_cast<uint2*>(row + 2 * e) = u;
         }
-        *reinterpret_cast<uint32_t*>(at) = u;
-    } else {
-        uint2 u;
-        u.x = f32_to_kv<TYPE>(y[0]) | uint32_t(f32_to_kv<TYPE>(y[1])) << 16;
-        u.y = f32_to_kv<TYPE>(y[2]) | uint32_t(f32_to_kv<TYPE>(y[3])) << 16;
-        *reinterpret_cast<uint2*>(at) = u;
     }
+}
+
+// The scale of a block with scale `old` (0: a new one) that receives values up
+// to the one with these bits, and how often it doubles.
+template <int TYPE>
+__device__ __forceinline__ float new_scale(float old, uint32_t bits, int* up) {
+    const float big = __uint_as_float(bits);
+    *up = 0;
+    if (!(big < INFINITY) || !(fabsf(old) < INFINITY)) return __builtin_nanf("");
+    if (!(old > 0.0f)) return big > 0.0f ? fmaxf(big / kMostCode<TYPE>, 0x1p-126f) : 0.0f;
+    // the ratio in 64 bits: exact where it is 1, 2, 4, ...
+    const double ratio = double(big) / (double(kMostCode<TYPE>) * double(old));
+    if (!(ratio > 1.0)) return old;
+    int e;
+    const double f = frexp(ratio, &e);
+    *up = f == 0.5 ? e - 1 : e;
+    return ldexpf(old, *up);
 }
 
 // 4 codes halved `up` times, to nearest even.
@@ -197,38 +234,123 @@ __device__ __forceinline__ uint32_t halved4(uint32_t u, int up) {
     }
 }
 
-// One workgroup per unit (a block's new tokens, or kSpan tokens of a 16-bit
-// cache) and group of its heads (key heads, then value heads), and one per token
-// and 16 query heads.  An 8-bit cache's workgroup makes the rows, finds each
-// head's largest value, settles the scales, and stores the rows (made a second
-// time if there are more than its threads hold); where a scale grew, it halves
-// the older tokens' codes.  No other workgroup touches these rows and scales.
+// `rows` rows of 16 byte pieces from `base`, halved, by `threads` threads.
+template <int TYPE>
+__device__ __forceinline__ void halve_rows(char* base, int rows, int d, uint32_t stride, int up, int first, int threads) {
+    const int per = d / 16, n = rows * per;
+#pragma unroll 4
+    for (int i = first; i < n; i += threads) {
+        const int r = i / per;
+        u32x4_t* at = reinterpret_cast<u32x4_t*>(base + uint64_t(uint32_t(r)) * stride + (i - r * per) * 16);
+        u32x4_t x = *at;
+#pragma unroll
+        for (int c = 0; c < 4; c++) x[c] = halved4<TYPE>(x[c], up);
+        *at = x;
+    }
+}
+
+// One token a sequence: a workgroup per kRows rows of a token (query, key, value
+// heads), W threads a row, which have all that the row's block needs: no barrier,
+// and nothing between the loads that they could wait for (rows, angles and the
+// chain of length, page id and scale are requested together).
+template <int TYPE, int W>
+__global__ __launch_bounds__(kThreads) void extend_one_kernel(ExtendArgs a) {
+    constexpr bool kCodes = TYPE == IQ_KV_I8 || TYPE == IQ_KV_E4M3;
+    constexpr int kSize = kCodes ? 1 : 2, kRows = kThreads / W;
+    const int tid = threadIdx.x, d = a.c.d, heads = a.hq + 2 * a.c.hk;
+    const uint32_t w = uint32_t(a.w0) + blockIdx.x, t = w / a.groups;
+    const int h = int(w % a.groups) * kRows + tid / W;
+    if (h >= heads) return;
+    const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.c.hk;
+    const uint32_t j = uint32_t(is_q ? h : is_k ? h - a.hq : h - a.hq - a.c.hk);
+    const int n = a.t.lens[t];
+    const Runs p = runs_of(tid % W * 4, is_q || is_k ? a.rot : 0, d);
+    const int64_t at = (int64_t(t) * (is_q ? a.hq : a.c.hk) + j) * d;
+    float x[8];
+    load_row((is_q ? a.q : is_k ? a.k : a.v) + at, p, x);
+    double pos = 0.0, freqs[4] = {};
+    if (p.turn) {
+        pos = double(a.pos[t]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) freqs[r] = a.freqs[p.e0 + r];
+    }
+    const bool inside = n >= 0 && n < a.t.cap;
+    const uint32_t tok = inside ? uint32_t(n) : 0, page = page_of(tok, a.c.div), slot = tok - page * uint32_t(a.c.ps);
+    const int32_t id = a.t.table[t * a.t.ld + page];
+    const bool live = inside && id >= 0 && id < a.c.pages;
+    const uint32_t pid = live ? uint32_t(id) : 0;
+    int older = 0;
+    float* scale = nullptr;
+    float old = 0.0f;
+    if constexpr (kCodes) {
+        scale = (is_k ? a.sc.k : a.sc.v) + kv_scale(a.sc, pid, slot, is_q ? 0 : j);
+        older = int(slot - page_of(slot, a.sc.div) * uint32_t(a.sc.block));
+        old = *scale;
+        if (older == 0) old = 0.0f;
+    }
+    float2 turn[4];
+    if (p.turn) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) turn[r] = angle(pos, freqs[r]);
+    }
+    const uint16_t* norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+    if (norm) norm_row<W>(x, p, norm, a.eps, d);
+    turn_row(x, p, turn);
+    if (is_q) {
+        store_row(a.qo + at, p, x);
+        return;
+    }
+    if (!live) return;
+    char* row = const_cast<char*>(is_k ? a.c.k : a.c.v) + kSize * kv_element(a.c, pid, slot, j);
+    if constexpr (kCodes) {
+        int up;
+        const float s = new_scale<TYPE>(old, largest<W>(x), &up);
+        if (p.on) put8<TYPE>(row, p, x, s);
+        if (tid % W == 0 && (older == 0 || !(s == old))) *scale = s;
+        if (up) halve_rows<TYPE>(row - uint64_t(uint32_t(older)) * a.c.sstr, older, d, a.c.sstr, up, tid % W, W);
+    } else {
+        if (p.on) put8<TYPE>(row, p, x, 0.0f);
+    }
+}
+
+// Runs of tokens: one workgroup per unit (a block's new tokens, or kSpan tokens of
+// a 16-bit cache) and group of its heads (key heads, then value heads), and one per
+// token and up to 2 kRows query heads.  An 8-bit cache's workgroup makes its rows,
+// finds each head's largest value, settles the scales, and stores the rows (made
+// a second time if there are more than its threads hold); where a scale grew, it
+// halves the older tokens' codes.  No other workgroup touches these rows and
+// scales.
 template <int TYPE, int W>
 __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
     constexpr bool kCodes = TYPE == IQ_KV_I8 || TYPE == IQ_KV_E4M3;
     constexpr int kSize = kCodes ? 1 : 2, kRows = kThreads / W;
-    __shared__ float2 cs[kChunk][128];
+    __shared__ __align__(16) float2 cs[128];
     __shared__ uint32_t most[kMaxHeads];
     __shared__ float scale[kMaxHeads];
     __shared__ int ups[kMaxHeads];
-    const int tid = threadIdx.x, d = a.c.d, i4 = tid % W * 4;
+    const int tid = threadIdx.x, d = a.c.d, mine = tid / W;
     const int64_t w = a.w0 + blockIdx.x;
+    const Runs pk = runs_of(tid % W * 4, a.rot, d), pv = runs_of(tid % W * 4, 0, d);
     if (w >= a.cached) {
+        // (two rows a thread, requested ahead of the angles that they share)
         const int64_t t = (w - a.cached) / a.qgroups;
-        const int h0 = int((w - a.cached) % a.qgroups) * 16, h1 = min(h0 + 16, a.hq);
-        make_angles(a, t, 1, cs);
-        __syncthreads();
-        const Runs p = runs_of(i4, a.rot, d);
-        for (int h = h0 + tid / W; h < h1; h += kRows) {
-            const int64_t at = (t * a.hq + h) * d;
-            float y0[4], y1[4];
-            make_row<W>(a.q + at, p, a.q_norm, a.eps, d, cs[0], y0, y1);
-            if (!p.on) continue;
+        const int h0 = int((w - a.cached) % a.qgroups) * 2 * kRows + mine;
+        const int64_t at = (t * a.hq + h0) * d, next = int64_t(kRows) * d;
+        float x[2][8];
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                a.qo[at + p.e0 + r] = y0[r];
-                a.qo[at + p.e1 + r] = y1[r];
-            }
+        for (int i = 0; i < 2; i++)
+            if (h0 + i * kRows < a.hq) load_row(a.q + at + i * next, pk, x[i]);
+        if (tid < a.rot / 2) cs[tid] = angle(double(a.pos[t]), a.freqs[tid]);
+        __syncthreads();
+        float2 turn[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) turn[r] = pk.turn ? cs[pk.e0 + r] : make_float2(1.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (h0 + i * kRows >= a.hq) break;
+            if (a.q_norm) norm_row<W>(x[i], pk, a.q_norm, a.eps, d);
+            turn_row(x[i], pk, turn);
+            store_row(a.qo + at + i * next, pk, x[i]);
         }
         return;
     }
@@ -236,127 +358,112 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
     if (!find_unit(a, uint32_t(w / a.groups), &u)) return;
     const int g0 = int(w % a.groups) * a.heads, G = min(a.heads, 2 * a.c.hk - g0), rows = u.count * G;
     const int32_t* table = a.t.table + u.b * a.t.ld;
-    // the page and slot of a token; -1 without a page
-    auto place = [&](int tok, uint32_t* slot) -> int {
-        const uint32_t p = page_of(uint32_t(tok), a.c.div);
-        *slot = uint32_t(tok) - p * uint32_t(a.c.ps);
-        const int32_t id = table[p];
-        return id >= 0 && id < a.c.pages ? id : -1;
+    auto head = [&](int h) { return uint32_t(h < a.c.hk ? h : h - a.c.hk); };
+    auto pool = [&](int h) { return const_cast<char*>(h < a.c.hk ? a.c.k : a.c.v); };
+    auto page_id = [&](int tok) { return table[page_of(uint32_t(tok), a.c.div)]; };
+    auto there = [&](int32_t id) { return id >= 0 && id < a.c.pages; };
+    // Row r of the unit: its values and position (requested ahead of what waits for
+    // the page), and from these what is stored.
+    struct Raw {
+        float x[8];
+        int64_t pos;
     };
-    uint32_t slot0 = 0;
-    int page = 0;
-    float old = 0.0f;
-    float* my_scale = nullptr;
-    if constexpr (kCodes) {  // (a block lies in one page)
-        page = place(u.begin, &slot0);
-        if (page < 0) return;
-        if (tid < G) {
-            const int h = g0 + tid;
-            my_scale = (h < a.c.hk ? a.sc.k : a.sc.v) + kv_scale(a.sc, uint32_t(page), slot0, uint32_t(h < a.c.hk ? h : h - a.c.hk));
-            if (u.tok > u.begin) old = *my_scale;
-            most[tid] = 0;
-        }
+    const bool turns = a.rot > 0 && g0 < a.c.hk && pk.turn;
+    double freqs[4] = {};
+    if (turns) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) freqs[r] = a.freqs[pk.e0 + r];
     }
-    const Runs pk = runs_of(i4, a.rot, d), pv = runs_of(i4, 0, d);
-    float y0[4], y1[4];
-    auto angles = [&](int c0) {
-        if (a.rot && g0 < a.c.hk) make_angles(a, u.row + c0, min(kChunk, u.count - c0), cs);
-        __syncthreads();
-    };
-    auto make = [&](int c0, int r) {  // row r of the chunk of tokens from c0 on
+    auto get = [&](int r, Raw& y) {
         const int k = r / G, h = g0 + r - k * G;
-        const int64_t t = u.row + c0 + k;
-        if (h < a.c.hk) make_row<W>(a.k + (t * a.c.hk + h) * d, pk, a.k_norm, a.eps, d, cs[k], y0, y1);
-        else make_row<W>(a.v + (t * a.c.hk + h - a.c.hk) * d, pv, nullptr, 0.0f, d, cs[k], y0, y1);
+        const int64_t t = u.row + k;
+        load_row((h < a.c.hk ? a.k : a.v) + (t * a.c.hk + head(h)) * d, h < a.c.hk ? pk : pv, y.x);
+        y.pos = turns ? a.pos[t] : 0;
     };
-    auto store = [&](int c0, int r) {
-        const int k = r / G, h = g0 + r - k * G, tok = u.tok + c0 + k;
-        uint32_t slot;
-        int id = page;
-        if constexpr (kCodes) slot = slot0 + uint32_t(tok - u.begin);
-        else id = place(tok, &slot);
+    auto make = [&](int r, Raw& y) {
+        if (g0 + r % G >= a.c.hk) return;
+        float2 turn[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) turn[i] = angle(double(y.pos), freqs[i]);
+        if (a.k_norm) norm_row<W>(y.x, pk, a.k_norm, a.eps, d);
+        turn_row(y.x, pk, turn);
+    };
+    const int32_t first_id = kCodes ? page_id(u.begin) : 0;  // (a block lies in one page)
+    const uint32_t slot0 = uint32_t(u.begin) - page_of(uint32_t(u.begin), a.c.div) * uint32_t(a.c.ps);
+    auto store = [&](int r, const Raw& y) {
+        const int k = r / G, h = g0 + r - k * G, tok = u.tok + k;
         const Runs& p = h < a.c.hk ? pk : pv;
-        if (id < 0 || !p.on) return;
-        char* to = const_cast<char*>(h < a.c.hk ? a.c.k : a.c.v) +
-                   kSize * kv_element(a.c, uint32_t(id), slot, uint32_t(h < a.c.hk ? h : h - a.c.hk));
-        const float s = kCodes ? scale[h - g0] : 0.0f;
-        put4<TYPE>(to + kSize * p.e0, y0, s);
-        put4<TYPE>(to + kSize * p.e1, y1, s);
+        uint32_t slot = slot0 + uint32_t(tok - u.begin);
+        int32_t id = first_id;
+        if constexpr (!kCodes) {
+            slot = uint32_t(tok) - page_of(uint32_t(tok), a.c.div) * uint32_t(a.c.ps);
+            id = page_id(tok);
+            if (!there(id)) return;
+        }
+        if (p.on) put8<TYPE>(pool(h) + kSize * kv_element(a.c, uint32_t(id), slot, head(h)), p, y.x, kCodes ? scale[h - g0] : 0.0f);
     };
-    const int mine = tid / W;
     if constexpr (!kCodes) {
-        angles(0);  // (kSpan <= kChunk)
         for (int r = mine; r < rows; r += kRows) {
-            make(0, r);
-            store(0, r);
+            Raw y;
+            get(r, y);
+            make(r, y);
+            store(r, y);
         }
         return;
     }
-    for (int c0 = 0; c0 < u.count; c0 += kChunk) {
-        if (c0) __syncthreads();  // (the angles before are no longer read)
-        angles(c0);
-        const int n = min(kChunk, u.count - c0) * G;
-        for (int r = mine; r < n; r += kRows) {
-            make(c0, r);
-            uint32_t big = 0;
+    Raw held[kHeld];
 #pragma unroll
-            for (int i = 0; i < 4; i++) big = max(big, max(__float_as_uint(fabsf(y0[i])), __float_as_uint(fabsf(y1[i]))));
-            big = over_row<W>(big, [](uint32_t x, uint32_t y) { return max(x, y); });
-            if (tid % W == 0) atomicMax(&most[r % G], big);
+    for (int i = 0; i < kHeld; i++)
+        if (mine + i * kRows < rows) get(mine + i * kRows, held[i]);
+    if (!there(first_id)) return;
+    float* at = nullptr;
+    float old = 0.0f;
+    if (tid < G) {
+        most[tid] = 0;
+        at = (g0 + tid < a.c.hk ? a.sc.k : a.sc.v) + kv_scale(a.sc, uint32_t(first_id), slot0, head(g0 + tid));
+        if (u.tok > u.begin) old = *at;
+    }
+    __syncthreads();
+    auto note = [&](int r, const Raw& y) {
+        const uint32_t big = largest<W>(y.x);
+        if (tid % W == 0) atomicMax(&most[r % G], big);
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) {
+        if (mine + i * kRows < rows) {
+            make(mine + i * kRows, held[i]);
+            note(mine + i * kRows, held[i]);
         }
+    }
+    for (int r = mine + kHeld * kRows; r < rows; r += kRows) {
+        Raw y;
+        get(r, y);
+        make(r, y);
+        note(r, y);
     }
     __syncthreads();
     if (tid < G) {
-        const float big = __uint_as_float(most[tid]);
-        float s = old;
-        int up = 0;
-        if (!(big < INFINITY) || !(fabsf(old) < INFINITY)) {
-            s = __builtin_nanf("");
-        } else if (!(old > 0.0f)) {
-            s = big > 0.0f ? fmaxf(big / kMostCode<TYPE>, 0x1p-126f) : 0.0f;
-        } else {
-            // the ratio in 64 bits: exact where it is 1, 2, 4, ...
-            const double ratio = double(big) / (double(kMostCode<TYPE>) * double(old));
-            if (ratio > 1.0) {
-                int e;
-                const double f = frexp(ratio, &e);
-                up = f == 0.5 ? e - 1 : e;
-                s = ldexpf(old, up);
-            }
-        }
+        int up;
+        const float s = new_scale<TYPE>(old, most[tid], &up);
         scale[tid] = s;
         ups[tid] = up;
-        if (!(s == old) || u.tok == u.begin) *my_scale = s;
+        if (u.tok == u.begin || !(s == old)) *at = s;
     }
     __syncthreads();
-    const bool held = rows <= kRows && u.count <= kChunk;
-    for (int c0 = 0; c0 < u.count; c0 += kChunk) {
-        if (u.count > kChunk) {
-            __syncthreads();
-            angles(c0);
-        }
-        const int n = min(kChunk, u.count - c0) * G;
-        for (int r = mine; r < n; r += kRows) {
-            if (!held) make(c0, r);
-            store(c0, r);
-        }
-    }
-    if (u.tok > u.begin) {
-        for (int h = 0; h < G; h++) {
-            const int up = ups[h], hh = g0 + h;
-            if (up == 0) continue;
-            char* base = const_cast<char*>(hh < a.c.hk ? a.c.k : a.c.v) +
-                         kv_element(a.c, uint32_t(page), slot0, uint32_t(hh < a.c.hk ? hh : hh - a.c.hk));
-            const int per = d / 16;
-            for (int i = tid; i < (u.tok - u.begin) * per; i += kThreads) {
-                const int r = i / per;
-                u32x4_t* at = reinterpret_cast<u32x4_t*>(base + uint64_t(r) * a.c.sstr + (i - r * per) * 16);
-                u32x4_t x = *at;
 #pragma unroll
-                for (int c = 0; c < 4; c++) x[c] = halved4<TYPE>(x[c], up);
-                *at = x;
-            }
-        }
+    for (int i = 0; i < kHeld; i++)
+        if (mine + i * kRows < rows) store(mine + i * kRows, held[i]);
+    for (int r = mine + kHeld * kRows; r < rows; r += kRows) {
+        Raw y;
+        get(r, y);
+        make(r, y);
+        store(r, y);
+    }
+    if (u.tok == u.begin) return;
+    for (int h = g0; h < g0 + G; h++) {
+        if (ups[h - g0] == 0) continue;
+        halve_rows<TYPE>(pool(h) + kv_element(a.c, uint32_t(first_id), slot0, head(h)), u.tok - u.begin, d, a.c.sstr,
+                         ups[h - g0], tid, kThreads);
     }
 }
 
@@ -484,12 +591,18 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
     }
 }
 
+template <int TYPE, int W>
+void launch_rows(const ExtendArgs& a, unsigned grid, hipStream_t s) {
+    if (a.starts) extend_kernel<TYPE, W><<<grid, kThreads, 0, s>>>(a);
+    else extend_one_kernel<TYPE, W><<<grid, kThreads, 0, s>>>(a);
+}
+
 template <int TYPE>
 void launch_extend(const ExtendArgs& a, unsigned grid, hipStream_t s) {
-    if (a.c.d <= 32) extend_kernel<TYPE, 4><<<grid, kThreads, 0, s>>>(a);
-    else if (a.c.d <= 64) extend_kernel<TYPE, 8><<<grid, kThreads, 0, s>>>(a);
-    else if (a.c.d <= 128) extend_kernel<TYPE, 16><<<grid, kThreads, 0, s>>>(a);
-    else extend_kernel<TYPE, 32><<<grid, kThreads, 0, s>>>(a);
+    if (a.c.d <= 32) launch_rows<TYPE, 4>(a, grid, s);
+    else if (a.c.d <= 64) launch_rows<TYPE, 8>(a, grid, s);
+    else if (a.c.d <= 128) launch_rows<TYPE, 16>(a, grid, s);
+    else launch_rows<TYPE, 32>(a, grid, s);
 }
 
 template <int TYPE>
@@ -541,16 +654,20 @@ int iq_kv_extend(const float* q, const float* k, const float* v, int64_t T, int 
     a.starts = starts;
     a.span = codes ? a.sc.block : iq::kSpan;
     a.span_div = iq::page_div(uint32_t(a.span));
-    // as many heads as fill a workgroup's threads once, of the tokens that a unit has
     const int rows = iq::kThreads / (a.c.d <= 32 ? 4 : a.c.d <= 64 ? 8 : a.c.d <= 128 ? 16 : 32);
-    const int tokens = starts ? std::min(a.span, rows) : 1;
-    a.heads = std::min({2 * a.c.hk, iq::kMaxHeads, std::max(1, rows / tokens)});
-    a.groups = uint32_t((2 * a.c.hk + a.heads - 1) / a.heads);
-    a.qgroups = uint32_t((q_heads + 15) / 16);
-    // n tokens touch at most (n - 1) / span + 2 units
-    const int64_t units = starts ? T / a.span + 2 * std::min<int64_t>(B, T) : B;
-    a.cached = units * a.groups;
-    const int64_t all = a.cached + T * a.qgroups;
+    int64_t all;
+    if (starts) {
+        // as many heads as fill a workgroup's threads once, of the tokens that a unit has
+        a.heads = std::min({2 * a.c.hk, iq::kMaxHeads, std::max(1, rows / std::min(a.span, rows))});
+        a.groups = uint32_t((2 * a.c.hk + a.heads - 1) / a.heads);
+        a.qgroups = uint32_t((q_heads + 2 * rows - 1) / (2 * rows));
+        // n tokens touch at most (n - 1) / span + 2 units
+        a.cached = (T / a.span + 2 * std::min<int64_t>(B, T)) * a.groups;
+        all = a.cached + T * a.qgroups;
+    } else {
+        a.groups = uint32_t((q_heads + 2 * a.c.hk + rows - 1) / rows);
+        all = T * a.groups;
+    }
     const hipStream_t s = static_cast<hipStream_t>(stream);
     for (; a.w0 < all; a.w0 += iq::kMaxGrid256) {
         const unsigned grid = unsigned(std::min(all - a.w0, iq::kMaxGrid256));
