@@ -449,6 +449,26 @@ def _on_device(what, device, *tensors):
         raise ValueError(f"{what}: tensors must be on the current CUDA device")
 
 
+def _arg(what, device, name, t, dtype, numel):
+    """The address of a contiguous tensor of this type, number of elements and
+    device; None for none.  (_need, _on_device and _addr in one, for calls of
+    many tensors, whose checks take longer than their kernels.)"""
+    if t is None:
+        return None
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+    if t.numel() != numel or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous with {numel} elements")
+    if t.get_device() != device:
+        raise ValueError(f"{what}: tensors on different devices")
+    return t.data_ptr()
+
+
+def _current(what, device):
+    if device < 0 or device != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors must be on the current CUDA device")
+
+
 def _new(stream, make, *args, **kw):
     """An output made here: from the memory of the stream that writes it."""
     if stream is None:
@@ -492,11 +512,11 @@ def kv_append(q, k, v, positions, slots, freqs, cache, q_out=None, stream=None):
     return q_out
 
 
-def _check_table(what, table, lens, name="lens", more=0):
+def _check_table(what, table, lens):
     if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"{what}: table must be int32 [sequences, pages] with contiguous rows")
     B, pages = table.shape
-    _need(what, name, lens, torch.int32, B + more)
+    _need(what, "lens", lens, torch.int32, B)
     ld = table.stride(0) if B > 1 else pages
     return B, pages, ld
 
@@ -508,6 +528,22 @@ def _check_sums(what, weights, B, kv_heads):
     if not weights.is_contiguous():
         raise ValueError(f"{what}: weights must be contiguous")
     return weights.shape[2]
+
+
+def _table(what, table):
+    """A block table's rows, pages and row stride."""
+    if table.dtype is not torch.int32 or table.dim() != 2:
+        raise ValueError(f"{what}: table must be int32 [sequences, pages] with contiguous rows")
+    (B, pages), (ld, one) = table.shape, table.stride()
+    if pages > 1 and one != 1:
+        raise ValueError(f"{what}: table must be int32 [sequences, pages] with contiguous rows")
+    return B, pages, ld if B > 1 else pages
+
+
+def _norm(what, device, name, t, d):
+    if t is not None and t.dtype is torch.int16:
+        return _arg(what, device, name, t, torch.int16, d)
+    return _arg(what, device, name, t, torch.bfloat16, d)
 
 
 def kv_extend(q, k, v, positions, freqs, cache, table, lens, starts=None, q_norm=None, k_norm=None, eps=1e-6,
@@ -522,40 +558,36 @@ def kv_extend(q, k, v, positions, freqs, cache, table, lens, starts=None, q_norm
     may be None (cache only).  lens stays as it is.  Returns q_out.
     include/iq.h, iq_kv_extend."""
     what = "kv_extend"
-    B, pages, ld = _check_table(what, table, lens)
-    hk, d = cache.kv_heads, cache.head_dim
-    T = k.numel() // (hk * d)
-    _need(what, "k", k, torch.float32, T * hk * d)
-    _need(what, "v", v, torch.float32, T * hk * d)
-    if starts is not None:
-        _need(what, "starts", starts, torch.int32, B + 1)
-    elif T != B:
+    B, pages, ld = _table(what, table)
+    hk, d, dev = cache.kv_heads, cache.head_dim, cache.device
+    n = k.numel()
+    T = n // (hk * d)
+    f32 = torch.float32
+    kp, vp = _arg(what, dev, "k", k, f32, T * hk * d), _arg(what, dev, "v", v, f32, n)
+    if table.get_device() != dev:
+        raise ValueError(f"{what}: tensors on different devices")
+    lp = _arg(what, dev, "lens", lens, torch.int32, B)
+    sp = _arg(what, dev, "starts", starts, torch.int32, B + 1)
+    if starts is None and T != B:
         raise ValueError(f"{what}: one token a sequence without starts")
-    rot = 0
+    rot, fp, pp = 0, None, None
     if freqs is not None:
         if positions is None:
             raise ValueError(f"{what}: freqs need positions")
-        _need(what, "freqs", freqs, torch.float64)
-        _need(what, "positions", positions, torch.int64, T)
         rot = 2 * freqs.numel()
-    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None:
-            if t.dtype not in (torch.bfloat16, torch.int16):
-                raise TypeError(f"{what}: {name} must be bf16 (torch.bfloat16 or int16 bits)")
-            _need(what, name, t, t.dtype, d)
-    heads = 0
+        fp, pp = _arg(what, dev, "freqs", freqs, torch.float64, rot // 2), _arg(what, dev, "positions", positions, torch.int64, T)
+    qn, kn = _norm(what, dev, "q_norm", q_norm, d), _norm(what, dev, "k_norm", k_norm, d)
+    heads, qp, op = 0, None, None
     if q is not None:
-        heads = q.numel() // max(1, T * d)
-        _need(what, "q", q, torch.float32, T * heads * d)
-        if q_out is not None:
-            _need(what, "q_out", q_out, torch.float32, T * heads * d)
-    _on_device(what, cache.device, q, k, v, positions if rot else None, freqs, table, lens, starts, q_norm, k_norm, q_out)
+        n = q.numel()
+        heads = n // max(1, T * d)
+        qp, op = _arg(what, dev, "q", q, f32, T * heads * d), _arg(what, dev, "q_out", q_out, f32, n)
+    _current(what, dev)
     if q is not None and q_out is None:
         q_out = _new(stream, torch.empty_like, q)
-    rc = lib().iq_kv_extend(_addr(q), _addr(k), _addr(v), T, heads, _addr(q_norm), _addr(k_norm), eps,
-                            _addr(positions) if rot else None, _addr(freqs) if rot else None, rot, cache.c,
-                            cache.scales_c, _addr(table), ld, pages, _addr(lens), _addr(starts), B,
-                            _addr(q_out) if heads else None, _stream(stream))
+        op = q_out.data_ptr()
+    rc = lib().iq_kv_extend(qp, kp, vp, T, heads, qn, kn, eps, pp if rot else None, fp if rot else None, rot, cache.c,
+                            cache.scales_c, table.data_ptr(), ld, pages, lp, sp, B, op if heads else None, _stream(stream))
     _check(rc, "iq_kv_extend")
     return q_out
 
@@ -569,29 +601,31 @@ def kv_read(cache, table, starts, T=None, first=None, dtype=torch.float32, out=N
     in tensors made here), tokens without a page are NaN.  include/iq.h,
     iq_kv_read."""
     what = "kv_read"
-    B, pages, ld = _check_table(what, table, starts, "starts", 1)
-    if first is not None:
-        _need(what, "first", first, torch.int32, B)
-    row = cache.kv_heads * cache.head_dim
+    B, pages, ld = _table(what, table)
+    dev, row = cache.device, cache.kv_heads * cache.head_dim
+    if table.get_device() != dev:
+        raise ValueError(f"{what}: tensors on different devices")
+    sp = _arg(what, dev, "starts", starts, torch.int32, B + 1)
+    fp = _arg(what, dev, "first", first, torch.int32, B)
     if out is None:
         if T is None:
             raise ValueError(f"{what}: T or out is needed")
-        _on_device(what, cache.device, table, starts, first)
+        _current(what, dev)
         out = tuple(_new(stream, torch.zeros, T, cache.kv_heads, cache.head_dim, dtype=dtype, device=table.device)
                     for _ in range(2))
     k, v = out
     some = k if k is not None else v
     if some is None:
         raise ValueError(f"{what}: out has neither k nor v")
-    T = some.numel() // row if T is None else T
-    if some.dtype not in READ_TYPES:
+    if T is None:
+        T = some.numel() // row
+    code = READ_TYPES.get(some.dtype)
+    if code is None:
         raise TypeError(f"{what}: outputs must be torch.float32, bfloat16 or float16")
-    for name, t in (("k", k), ("v", v)):
-        if t is not None:
-            _need(what, name, t, some.dtype, T * row)
-    _on_device(what, cache.device, table, starts, first, k, v)
-    rc = lib().iq_kv_read(cache.c, cache.scales_c, _addr(table), ld, pages, _addr(first), _addr(starts), B, T,
-                          READ_TYPES[some.dtype], _addr(k), _addr(v), _stream(stream))
+    kp, vp = _arg(what, dev, "k", k, some.dtype, T * row), _arg(what, dev, "v", v, some.dtype, T * row)
+    _current(what, dev)
+    rc = lib().iq_kv_read(cache.c, cache.scales_c, table.data_ptr(), ld, pages, fp, sp, B, T, code, kp, vp,
+                          _stream(stream))
     _check(rc, "iq_kv_read")
     return k, v
 
@@ -608,30 +642,39 @@ def attn_decode(q, cache, table, lens, out=None, weights=None, scale=None, strea
     16-bit caches and no window.  include/iq.h, iq_attn_decode and
     iq_attn_decode_window."""
     what = "attn_decode"
-    B, pages, ld = _check_table(what, table, lens)
+    if window < 0 or sinks < 0:
+        raise ValueError(f"{what}: window and sinks must not be negative")
     d = cache.head_dim
+    if window or cache.block:
+        if weights is not None:
+            raise ValueError(f"{what}: weights are added up over 16-bit caches and without a window")
+        B, pages, ld = _table(what, table)
+        dev, n = cache.device, q.numel()
+        heads = n // max(1, B * d)
+        if table.get_device() != dev:
+            raise ValueError(f"{what}: tensors on different devices")
+        qp, lp = _arg(what, dev, "q", q, torch.float32, B * heads * d), _arg(what, dev, "lens", lens, torch.int32, B)
+        op = _arg(what, dev, "out", out, torch.float32, n)
+        _current(what, dev)
+        if out is None:
+            out = _new(stream, torch.empty_like, q)
+            op = out.data_ptr()
+        rc = lib().iq_attn_decode_window(qp, cache.c, cache.scales_c, table.data_ptr(), ld, pages, lp, B, heads,
+                                         d ** -0.5 if scale is None else scale, window, sinks, op, _stream(stream))
+        _check(rc, "iq_attn_decode_window")
+        return out
+    B, pages, ld = _check_table(what, table, lens)
     heads = q.numel() // max(1, B * d)
     _need(what, "q", q, torch.float32, B * heads * d)
     wld = 0 if weights is None else _check_sums(what, weights, B, cache.kv_heads)
     if out is not None:
         _need(what, "out", out, torch.float32, B * heads * d)
-    if window < 0 or sinks < 0:
-        raise ValueError(f"{what}: window and sinks must not be negative")
-    plain = not window and cache.block == 0
-    if weights is not None and not plain:
-        raise ValueError(f"{what}: weights are added up over 16-bit caches and without a window")
     _on_device(what, cache.device, q, table, lens, out, weights)
     if out is None:
         out = _new(stream, torch.empty_like, q)
-    scale = d ** -0.5 if scale is None else scale
-    if plain:
-        rc = lib().iq_attn_decode(_addr(q), cache.c, _addr(table), ld, pages, _addr(lens), B, heads, scale, _addr(out),
-                                  _addr(weights), wld, _stream(stream))
-        _check(rc, "iq_attn_decode")
-    else:
-        rc = lib().iq_attn_decode_window(_addr(q), cache.c, cache.scales_c, _addr(table), ld, pages, _addr(lens), B,
-                                         heads, scale, window, sinks, _addr(out), _stream(stream))
-        _check(rc, "iq_attn_decode_window")
+    rc = lib().iq_attn_decode(_addr(q), cache.c, _addr(table), ld, pages, _addr(lens), B, heads,
+                              d ** -0.5 if scale is None else scale, _addr(out), _addr(weights), wld, _stream(stream))
+    _check(rc, "iq_attn_decode")
     return out
 
 
