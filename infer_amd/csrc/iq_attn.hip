@@ -50,7 +50,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     constexpr int ROWB = DP * 2, KVB = kAttnTile * ROWB;
     __shared__ __align__(16) char lds[kAttnWaves][2 * KVB];
     __shared__ float wm[kAttnWaves][16], wl[kAttnWaves][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
     Item it;
     // Heads that share cache lines (see the host side) go to one XCD for a
     // chunk: workgroups are dealt to the 8 of them in turn.
