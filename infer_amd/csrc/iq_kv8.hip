@@ -3,6 +3,7 @@
 // block of tokens and head), and cached tokens read back.
 #include <algorithm>
 
+#include "iq_extend_plan.h"
 #include "iq_kv.h"
 
 namespace iq {
@@ -45,35 +46,23 @@ __device__ __forceinline__ V over_row(V v, F f) {
     return v;
 }
 
-// A new token run of one sequence inside one span of its tokens.
-struct Unit {
-    int b, tok, count;  // its first token, and how many
-    int begin;          // the span's first token
-    int64_t row;        // of the first token's q, k, v
-};
-
-__device__ __forceinline__ bool find_unit(const ExtendArgs& a, uint32_t u, Unit* it) {
+// The uth unit of the batch, false past the last.  Every wave finds it from
+// the lengths and starts by itself (64 sequences a step).
+__device__ __forceinline__ bool find_unit(const ExtendArgs& a, uint32_t u, int* seq, Unit* unit) {
     const int lane = threadIdx.x & 63;
     uint32_t before = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int b = min(b0 + lane, a.B - 1);
-        const int T = int(a.T), s0 = min(max(a.starts[b], 0), T), s1 = min(a.starts[b + 1], T), L = a.t.lens[b];
-        const int n = L < 0 || L >= a.t.cap || b0 + lane >= a.B ? 0 : min(s1 - s0, a.t.cap - L);
-        const uint32_t f = page_of(uint32_t(max(L, 0)), a.span_div);
-        const uint32_t k = n > 0 ? page_of(uint32_t(L + n - 1), a.span_div) - f + 1 : 0;
-        const uint32_t upto = before + wave_scan(k);
+        const int b = min(b0 + lane, a.B - 1), len = a.t.lens[b];
+        NewTokens n = new_tokens(a.starts[b], a.starts[b + 1], len, int32_t(a.T), a.t.cap);
+        if (b0 + lane >= a.B) n.count = 0;
+        const uint32_t k = units_of(len, n.count, a.span_div), upto = before + wave_scan(k);
         const uint64_t past = __ballot(u < upto);
         if (past) {
             const int l = __builtin_ctzll(past);
-            const int len = __builtin_amdgcn_readlane(L, l), cnt = __builtin_amdgcn_readlane(n, l);
-            const int s = int(lane_of(f, l) + (u - (lane_of(upto, l) - lane_of(k, l))));
-            it->b = b0 + l;
-            it->begin = s * a.span;
-            it->tok = max(len, it->begin);
-            // (in 64 bits: the span behind the last token may end past 2^31)
-            it->count = int(min(int64_t(len) + cnt, int64_t(it->begin) + a.span) - it->tok);
-            it->row = int64_t(__builtin_amdgcn_readlane(s0, l)) + (it->tok - len);
-            return true;
+            const NewTokens mine{__builtin_amdgcn_readlane(n.row, l), __builtin_amdgcn_readlane(n.count, l)};
+            *seq = b0 + l;
+            *unit = unit_at(u - (lane_of(upto, l) - lane_of(k, l)), __builtin_amdgcn_readlane(len, l), mine, a.span, a.span_div);
+            return unit->count > 0;
         }
         before = lane_of(upto, 63);
     }
@@ -355,9 +344,10 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
         return;
     }
     Unit u;
-    if (!find_unit(a, uint32_t(w / a.groups), &u)) return;
+    int seq;
+    if (!find_unit(a, uint32_t(w / a.groups), &seq, &u)) return;
     const int g0 = int(w % a.groups) * a.heads, G = min(a.heads, 2 * a.c.hk - g0), rows = u.count * G;
-    const int32_t* table = a.t.table + u.b * a.t.ld;
+    const int32_t* table = a.t.table + seq * a.t.ld;
     auto head = [&](int h) { return uint32_t(h < a.c.hk ? h : h - a.c.hk); };
     auto pool = [&](int h) { return const_cast<char*>(h < a.c.hk ? a.c.k : a.c.v); };
     auto page_id = [&](int tok) { return table[page_of(uint32_t(tok), a.c.div)]; };
@@ -376,7 +366,7 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
     }
     auto get = [&](int r, Raw& y) {
         const int k = r / G, h = g0 + r - k * G;
-        const int64_t t = u.row + k;
+        const int64_t t = int64_t(u.row) + k;
         load_row((h < a.c.hk ? a.k : a.v) + (t * a.c.hk + head(h)) * d, h < a.c.hk ? pk : pv, y.x);
         y.pos = turns ? a.pos[t] : 0;
     };
@@ -661,8 +651,7 @@ int iq_kv_extend(const float* q, const float* k, const float* v, int64_t T, int 
         a.heads = std::min({2 * a.c.hk, iq::kMaxHeads, std::max(1, rows / std::min(a.span, rows))});
         a.groups = uint32_t((2 * a.c.hk + a.heads - 1) / a.heads);
         a.qgroups = uint32_t((q_heads + 2 * rows - 1) / (2 * rows));
-        // n tokens touch at most (n - 1) / span + 2 units
-        a.cached = (T / a.span + 2 * std::min<int64_t>(B, T)) * a.groups;
+        a.cached = iq::max_units(T, B, a.span) * a.groups;
         all = a.cached + T * a.qgroups;
     } else {
         a.groups = uint32_t((q_heads + 2 * a.c.hk + rows - 1) / rows);

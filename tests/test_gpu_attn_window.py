@@ -205,3 +205,23 @@ def test_long_rows_past_32_bits():
     got, K = out.cpu().numpy(), rk.double().cpu().numpy()
     ref, _, ck, cv = attn_f64(q[0].double().cpu().numpy(), K, K, d ** -0.5)
     assert np.all(np.abs(got[0] - ref) <= rel(d, ck)[:, None] * cv)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (9, 2)])
+@pytest.mark.parametrize("dtype", [I8, F8, FP])
+def test_most_sequences(dtype, window, sinks):
+    """1024 sequences of a few tokens, in a slice of a wider table."""
+    rng = np.random.default_rng(21)
+    B, hq, hk, d, page = 1024, 3, 1, 16, 8
+    lens = rng.integers(0, 41, B)
+    pool = Pool(rng, B, 5, page, hk, d, dtype, 4)
+    pool.fill(rng, lens)
+    q = rng.standard_normal((B, hq, d)).astype(np.float32)
+    wide = torch.full((B, 9), -3, dtype=torch.int32, device="cuda")
+    wide[:, 1:6] = pool.table
+    out = ops.attn_decode(torch.from_numpy(q).cuda(), pool.cache, wide[:, 1:6], torch.from_numpy(lens).int().cuda(),
+                          window=window, sinks=sinks)
+    torch.cuda.synchronize()
+    got, raw = out.cpu().numpy(), pool.raw()
+    pool.raw = lambda: raw
+    check(pool, q, lens, got, window, sinks)

@@ -266,3 +266,50 @@ def test_in_place_and_on_another_stream():
     torch.cuda.synchronize()
     assert got is q and torch.equal(got, want)
     same(pool.raw(), raw, "stream")
+
+
+@pytest.mark.parametrize("dtype", [F8, BF])
+def test_most_sequences_and_a_part_of_a_table(dtype):
+    """1024 sequences, a token each; the table is a slice of a wider one."""
+    rng = np.random.default_rng(12)
+    B, page, block, hk, d = 1024, 4, 2, 1, 16
+    pool = Pool(rng, B, 3, page, hk, d, dtype, block)
+    lens = rng.integers(-1, 13, B)
+    pool.fill(rng, np.minimum(lens, 12))
+    raw = pool.raw()
+    wide = torch.full((B, 7), -9, dtype=torch.int32, device="cuda")
+    wide[:, 2:5] = pool.table
+    k, v = rows(rng, B, hk, d), rows(rng, B, hk, d)
+    q = rows(rng, B, 3, d)
+    got = ops.kv_extend(dev(q), dev(k), dev(v), None, None, pool.cache, wide[:, 2:5], dev(lens, torch.int32))
+    torch.cuda.synchronize()
+    extend_plain(pool, raw, k, lens, [1] * B, 0)
+    extend_plain(pool, raw, v, lens, [1] * B, 1)
+    same(pool.raw(), raw, "most")
+    assert np.array_equal(got.cpu().numpy(), q)
+
+
+def test_unaligned_inputs():
+    """q, k, v, norms and q_out at any multiple of their own size."""
+    rng = np.random.default_rng(13)
+    B, hq, hk, d = 3, 6, 2, 64
+    fr, pos = ops.rope_freqs(d, 1e6), dev(np.array([5, 6, 7]))
+    got = []
+    for off in (0, 1, 3):
+        for starts in (None, torch.tensor([0, 1, 2, 3], dtype=torch.int32).cuda()):
+            rng = np.random.default_rng(13)
+            pool = Pool(rng, B, 2, 16, hk, d, I8, 8)
+            pool.fill(rng, [5, 6, 7])
+
+            def at(shape):
+                x = torch.empty(int(np.prod(shape)) + off, device="cuda")[off:].view(shape)
+                return x.copy_(dev(rows(rng, *shape)))
+            q, k, v = at((B, hq, d)), at((B, hk, d)), at((B, hk, d))
+            w = torch.empty(d + off, dtype=BF, device="cuda")[off:].copy_(dev(1 + 0.1 * rng.standard_normal(d)))
+            out = torch.empty(B * hq * d + off, device="cuda")[off:].view(B, hq, d)
+            ops.kv_extend(q, k, v, pos, fr, pool.cache, pool.table, dev(np.array([5, 6, 7]), torch.int32), starts=starts,
+                          q_norm=w, k_norm=w, q_out=out)
+            torch.cuda.synchronize()
+            got.append([out.cpu().numpy(), *pool.raw()])
+    for g in got[1:]:
+        assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(g, got[0]))
