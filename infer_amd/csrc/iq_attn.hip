@@ -6,9 +6,11 @@
 // cycles and lane, too many beside the unpacking; on the matrix cores the up
 // to 16 heads of a group are the 16 columns of one product and cost nothing.
 // What bounds the operator is the read of the cache: 131072 tokens, 4 heads of
-// 128 in bf16 take 57 us (4.71 TB/s; a device copy reaches 4.74), every byte
-// read once, the matrix cores busy for 12 % of it; 32 sequences of up to 8192
-// tokens, 2 heads, 21 us (4.1 TB/s).  A join adds 4 to 5 us.
+// 128 in bf16 take 52.8 us (5.1 TB/s; a device copy reaches 4.7, a plain read
+// 6.2), every byte read once, the matrix cores busy for 13 % of it; 32 sequences
+// of up to 8192 tokens, 2 heads, 20.4 us (4.2 TB/s).  A join adds 4 to 5 us.
+// Under a window a sequence is its visible tokens: 16 of up to 16384 that see
+// 4100 each, 4 heads, 19.1 us (4.1 TB/s).
 //
 //   scores  S^T[token][head] = K[token][d] . q^T[d][head]
 //   sums    O^T[d][head]    += V^T[d][token] . P^T[token][head]
@@ -456,10 +458,11 @@ int attn_decode(AttnArgs a, const float* q, int B, int q_heads, float scale, int
     a.sinks = win ? int32_t(sinks) : 0;
     a.visible = win ? int32_t(window + sinks) : a.t.cap;
     // as many work items as run at once: 4, 3, 2 or 1 workgroups a CU by the
-    // registers (d <= 64) and the LDS of an instance.  Measured for d = 128 on
-    // 131072 tokens / 32 sequences of up to 8192: 1 a CU 69.9 / 30.4 us, 2 61.8
-    // / 24.7, 3 69.1 / 27.8, 4 66.0 / 29.4; for d = 64 (24 of up to 2047, 16
-    // heads) 18.1, 19.0, 17.2, 18.8.
+    // registers (d <= 64) and the LDS of an instance.  Both launches with 1, 2, 3
+    // and 4 a CU: d = 128, 131072 tokens 56.5, 57.3, 61.1, 62 us, 32 sequences of up
+    // to 8192 23.8, 24.2, 27.3, 27.4; d = 64, 24 of up to 2047, 16 heads 16.0,
+    // 16.5, 16.9, 18.3; d = 32, 8 of 16384 46.9, 38.3, 37.7, 38.6.  (The choice goes
+    // into the order of a result's sums; 8-bit caches have their own.)
     const int groups = bits8 ? attn8_groups(a.c.d) : a.c.d <= 32 ? 4 : a.c.d <= 64 ? 3 : a.c.d <= 128 ? 2 : 1;
     a.target = uint32_t(groups * device_cu_count());
     // Neighbouring heads' rows meet in a cache line, or several head tiles read
