@@ -347,8 +347,9 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
  *   k, v      are rounded into the cache, to nearest even
  * A token behind the table's last page, in a page whose id lies outside [0,
  * pages) or of a sequence whose length is below 0 or above max_pages * page_size is
- * not stored.  Rows that belong to no sequence are not either.  Pages that are
- * written must not be shared between the sequences nor appear twice in one.
+ * not stored.  Rows that belong to no sequence are not either.  The pages that a
+ * call writes must be different ones (a row of the table may name a page again
+ * once no token of its earlier place is read any more, as under a window).
  *
  * An 8-bit cache's blocks start anew with their first slot: with a = max |x| over
  * the call's tokens of the block (one head's k or v), in fp32, and Q = 127 (448),

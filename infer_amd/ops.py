@@ -659,6 +659,7 @@ def attn_decode(q, cache, table, lens, out=None, weights=None, scale=None, strea
         if out is None:
             out = _new(stream, torch.empty_like, q)
             op = out.data_ptr()
+        window, sinks = min(window, 2 ** 62), min(sinks, 2 ** 62)  # (more is not an int64)
         rc = lib().iq_attn_decode_window(qp, cache.c, cache.scales_c, table.data_ptr(), ld, pages, lp, B, heads,
                                          d ** -0.5 if scale is None else scale, window, sinks, op, _stream(stream))
         _check(rc, "iq_attn_decode_window")

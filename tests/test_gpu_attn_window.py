@@ -179,7 +179,7 @@ def test_window_as_the_whole():
     for dtype in (BF, FP, I8, F8):
         pool, q, out = run(rng, [700, 33, 5], 12, 2, 128, 16, 16, dtype)
         lens = torch.tensor([700, 33, 5], dtype=torch.int32).cuda()
-        for window, sinks in ((704, 0), (700, 4), (2 ** 62, 3), (1, 703)):
+        for window, sinks in ((704, 0), (700, 4), (2 ** 62, 3), (1, 703), (2 ** 70, 2 ** 64)):
             again = ops.attn_decode(torch.from_numpy(q).cuda(), pool.cache, pool.table, lens, window=window, sinks=sinks)
             torch.cuda.synchronize()
             assert torch.equal(again, out), (dtype, window, sinks)

@@ -253,3 +253,23 @@ def test_capture_without_workspace_is_refused():
             x.add_(0.0)  # (a non-empty capture)
             ops.attn_decode(q, cache, table, lens, out=out, stream=s)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtypes", [(I8, F8), (BF, I8)])
+def test_a_ring_of_pages_under_a_window(dtypes):
+    """A window of 20 and 3 first tokens need the first page and the last three:
+    the table names the same few pages over and over, with the answers of a table
+    that names new ones."""
+    got = []
+    for ring in (False, True):
+        rng, host, step, table = build(6, 2, dtypes, window=20, sinks=3, pages=8)
+        if ring:
+            for b in range(2):
+                for p in range(4, 8):
+                    table[b, p] = table[b, p - 3]
+            step.table.copy_(torch.from_numpy(table))
+        for it in range(120):
+            step.step([it, 299 - it])
+            got.append(step.logits.clone())
+    assert all(torch.equal(a, b) for a, b in zip(got[:120], got[120:]))
+    assert torch.isfinite(got[-1]).all()
