@@ -32,6 +32,7 @@ struct ExtendArgs {
     const double* freqs;
     float* qo;
     float eps;
+    double inv_d;  // 1 / head_dim
     int hq, rot, B;
     int64_t T;
     KvView c;
@@ -113,15 +114,17 @@ __device__ __forceinline__ void store_row(float* dst, const Runs& p, const float
 }
 
 // x / sqrt(mean(x^2) + eps) * norm; the squares and their root in 64 bits: no x
-// in fp32's range over- or underflows.
+// in fp32's range over- or underflows.  inv_d = 1 / d.
 template <int W>
-__device__ __forceinline__ void norm_row(float (&x)[8], const Runs& p, const uint16_t* norm, float eps, int d) {
+__device__ __forceinline__ void norm_row(float (&x)[8], const Runs& p, const uint16_t* norm, float eps, double inv_d) {
     const ushort4u_t n0 = *reinterpret_cast<const ushort4u_t*>(norm + p.e0), n1 = *reinterpret_cast<const ushort4u_t*>(norm + p.e1);
     double ss = 0.0;
 #pragma unroll
-    for (int r = 0; r < 8; r++) ss += double(x[r]) * x[r];
+    for (int r = 0; r < 8; r++) ss = fma(double(x[r]), double(x[r]), ss);
     ss = over_row<W>(ss, [](double u, double v) { return u + v; });
-    const double inv = 1.0 / sqrt(ss / d + double(eps));
+    // 1 / sqrt by a Newton step, which is no number at 0 and infinity
+    const double mean = fma(ss, inv_d, double(eps)), r0 = __builtin_amdgcn_rsq(mean);
+    const double r1 = fma(0.5 * r0, fma(-mean * r0, r0, 1.0), r0), inv = r1 == r1 ? r1 : r0;
 #pragma unroll
     for (int r = 0; r < 8; r++) x[r] = float(x[r] * inv) * bf16_to_f32(r < 4 ? n0[r] : n1[r - 4]);
 }
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void extend_one_kernel(ExtendArgs a) {
         for (int r = 0; r < 4; r++) turn[r] = angle(pos, freqs[r]);
     }
     const uint16_t* norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
-    if (norm) norm_row<W>(x, p, norm, a.eps, d);
+    if (norm) norm_row<W>(x, p, norm, a.eps, a.inv_d);
     turn_row(x, p, turn);
     if (is_q) {
         store_row(a.qo + at, p, x);
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             if (h0 + i * kRows >= a.hq) break;
-            if (a.q_norm) norm_row<W>(x[i], pk, a.q_norm, a.eps, d);
+            if (a.q_norm) norm_row<W>(x[i], pk, a.q_norm, a.eps, a.inv_d);
             turn_row(x[i], pk, turn);
             store_row(a.qo + at + i * next, pk, x[i]);
         }
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
         float2 turn[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) turn[i] = angle(double(y.pos), freqs[i]);
-        if (a.k_norm) norm_row<W>(y.x, pk, a.k_norm, a.eps, d);
+        if (a.k_norm) norm_row<W>(y.x, pk, a.k_norm, a.eps, a.inv_d);
         turn_row(y.x, pk, turn);
     };
     const int32_t first_id = kCodes ? page_id(u.begin) : 0;  // (a block lies in one page)
@@ -642,6 +645,7 @@ int iq_kv_extend(const float* q, const float* k, const float* v, int64_t T, int 
     a.q_norm = q_norm;
     a.k_norm = k_norm;
     a.eps = eps;
+    a.inv_d = 1.0 / a.c.d;
     a.pos = positions;
     a.freqs = freqs;
     a.qo = q_out;

@@ -464,9 +464,19 @@ def _arg(what, device, name, t, dtype, numel):
     return t.data_ptr()
 
 
-def _current(what, device):
-    if device < 0 or device != torch.cuda.current_device():
+# The current device without the check that CUDA is initialised, which a CUDA
+# tensor's existence answers (where torch has it).
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _current(what, device, stream):
+    """The handle of `stream` (None: the current one) on `device`, which has to
+    be the current device."""
+    if device < 0 or device != _device_now():
         raise ValueError(f"{what}: tensors must be on the current CUDA device")
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(device)
+    return _stream(stream)
 
 
 def _new(stream, make, *args, **kw):
@@ -582,12 +592,12 @@ def kv_extend(q, k, v, positions, freqs, cache, table, lens, starts=None, q_norm
         n = q.numel()
         heads = n // max(1, T * d)
         qp, op = _arg(what, dev, "q", q, f32, T * heads * d), _arg(what, dev, "q_out", q_out, f32, n)
-    _current(what, dev)
+    on = _current(what, dev, stream)
     if q is not None and q_out is None:
         q_out = _new(stream, torch.empty_like, q)
         op = q_out.data_ptr()
     rc = lib().iq_kv_extend(qp, kp, vp, T, heads, qn, kn, eps, pp if rot else None, fp if rot else None, rot, cache.c,
-                            cache.scales_c, table.data_ptr(), ld, pages, lp, sp, B, op if heads else None, _stream(stream))
+                            cache.scales_c, table.data_ptr(), ld, pages, lp, sp, B, op if heads else None, on)
     _check(rc, "iq_kv_extend")
     return q_out
 
@@ -610,7 +620,7 @@ def kv_read(cache, table, starts, T=None, first=None, dtype=torch.float32, out=N
     if out is None:
         if T is None:
             raise ValueError(f"{what}: T or out is needed")
-        _current(what, dev)
+        _current(what, dev, stream)
         out = tuple(_new(stream, torch.zeros, T, cache.kv_heads, cache.head_dim, dtype=dtype, device=table.device)
                     for _ in range(2))
     k, v = out
@@ -623,9 +633,8 @@ def kv_read(cache, table, starts, T=None, first=None, dtype=torch.float32, out=N
     if code is None:
         raise TypeError(f"{what}: outputs must be torch.float32, bfloat16 or float16")
     kp, vp = _arg(what, dev, "k", k, some.dtype, T * row), _arg(what, dev, "v", v, some.dtype, T * row)
-    _current(what, dev)
-    rc = lib().iq_kv_read(cache.c, cache.scales_c, table.data_ptr(), ld, pages, fp, sp, B, T, code, kp, vp,
-                          _stream(stream))
+    on = _current(what, dev, stream)
+    rc = lib().iq_kv_read(cache.c, cache.scales_c, table.data_ptr(), ld, pages, fp, sp, B, T, code, kp, vp, on)
     _check(rc, "iq_kv_read")
     return k, v
 
@@ -655,13 +664,13 @@ def attn_decode(q, cache, table, lens, out=None, weights=None, scale=None, strea
             raise ValueError(f"{what}: tensors on different devices")
         qp, lp = _arg(what, dev, "q", q, torch.float32, B * heads * d), _arg(what, dev, "lens", lens, torch.int32, B)
         op = _arg(what, dev, "out", out, torch.float32, n)
-        _current(what, dev)
+        on = _current(what, dev, stream)
         if out is None:
             out = _new(stream, torch.empty_like, q)
             op = out.data_ptr()
         window, sinks = min(window, 2 ** 62), min(sinks, 2 ** 62)  # (more is not an int64)
         rc = lib().iq_attn_decode_window(qp, cache.c, cache.scales_c, table.data_ptr(), ld, pages, lp, B, heads,
-                                         d ** -0.5 if scale is None else scale, window, sinks, op, _stream(stream))
+                                         d ** -0.5 if scale is None else scale, window, sinks, op, on)
         _check(rc, "iq_attn_decode_window")
         return out
     B, pages, ld = _check_table(what, table, lens)
