@@ -25,6 +25,23 @@ constexpr int kSpan = 16;      // tokens of a 16-bit cache's unit
 constexpr int kMaxHeads = 16;  // heads of a workgroup
 constexpr int kHeld = 4;       // rows that a thread can hold
 
+// Things of `groups` workgroups each, from the one that a launch begins with:
+// 32-bit divisions in the kernels, by multiplication.
+struct Parts {
+    int64_t first;       // thing
+    uint32_t group;      // of the first workgroup
+    uint32_t groups;
+    PageDiv div;
+};
+struct Part {
+    int64_t thing;
+    uint32_t group;
+};
+__device__ __forceinline__ Part part_of(const Parts& p, uint32_t block) {
+    const uint32_t x = p.group + block, n = page_of(x, p.div);
+    return {p.first + n, x - n * p.groups};
+}
+
 struct ExtendArgs {
     const float *q, *k, *v;
     const uint16_t *q_norm, *k_norm;
@@ -41,11 +58,11 @@ struct ExtendArgs {
     const int32_t* starts;
     int span;             // tokens of a unit
     PageDiv span_div;
-    uint32_t groups;      // of the 2 hk rows that a token has in the cache
-    int heads;            // of a group
-    uint32_t qgroups;     // of the query heads
-    int64_t cached;       // workgroups of the cache's part, then T * qgroups
-    int64_t w0;           // first workgroup of this launch
+    Parts cached;         // units x groups of their heads (one token each: tokens x groups of all heads)
+    Parts queries;        // tokens x groups of query heads, behind them
+    int heads;            // of a unit's group
+    PageDiv heads_div, last_div;  // by heads, and by those of the last group
+    uint32_t rest;        // workgroups of this launch that are the cache's
 };
 
 template <int W, typename V, typename F>
@@ -258,8 +275,9 @@ __global__ __launch_bounds__(kThreads) void extend_one_kernel(ExtendArgs a) {
     constexpr bool kCodes = TYPE == IQ_KV_I8 || TYPE == IQ_KV_E4M3;
     constexpr int kSize = kCodes ? 1 : 2, kRows = kThreads / W;
     const int tid = threadIdx.x, d = a.c.d, heads = a.hq + 2 * a.c.hk;
-    const uint32_t w = uint32_t(a.w0) + blockIdx.x, t = w / a.groups;
-    const int h = int(w % a.groups) * kRows + tid / W;
+    const Part part = part_of(a.cached, blockIdx.x);
+    const uint32_t t = uint32_t(part.thing);
+    const int h = int(part.group) * kRows + tid / W;
     if (h >= heads) return;
     const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.c.hk;
     const uint32_t j = uint32_t(is_q ? h : is_k ? h - a.hq : h - a.hq - a.c.hk);
@@ -329,12 +347,12 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
     __shared__ float scale[kMaxHeads];
     __shared__ int ups[kMaxHeads];
     const int tid = threadIdx.x, d = a.c.d, mine = tid / W;
-    const int64_t w = a.w0 + blockIdx.x;
     const Runs pk = runs_of(tid % W * 4, a.rot, d), pv = runs_of(tid % W * 4, 0, d);
-    if (w >= a.cached) {
+    if (blockIdx.x >= a.rest) {
         // (two rows a thread, requested ahead of the angles that they share)
-        const int64_t t = (w - a.cached) / a.qgroups;
-        const int h0 = int((w - a.cached) % a.qgroups) * 2 * kRows + mine;
+        const Part part = part_of(a.queries, blockIdx.x - a.rest);
+        const int64_t t = part.thing;
+        const int h0 = int(part.group) * 2 * kRows + mine;
         const int64_t at = (t * a.hq + h0) * d, next = int64_t(kRows) * d;
         float x[2][8];
 #pragma unroll
@@ -356,18 +374,21 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
     }
     Unit u;
     int seq;
-    if (!find_unit(a, uint32_t(w / a.groups), &seq, &u)) return;
-    const int g0 = int(w % a.groups) * a.heads, G = min(a.heads, 2 * a.c.hk - g0), rows = u.count * G;
+    const Part part = part_of(a.cached, blockIdx.x);
+    if (!find_unit(a, uint32_t(part.thing), &seq, &u)) return;
+    const int g0 = int(part.group) * a.heads, G = min(a.heads, 2 * a.c.hk - g0), rows = u.count * G;
+    const PageDiv by_heads = G == a.heads ? a.heads_div : a.last_div;
     const int32_t* table = a.t.table + seq * a.t.ld;
     auto head = [&](int h) { return uint32_t(h < a.c.hk ? h : h - a.c.hk); };
     auto pool = [&](int h) { return const_cast<char*>(h < a.c.hk ? a.c.k : a.c.v); };
     auto page_id = [&](int tok) { return table[page_of(uint32_t(tok), a.c.div)]; };
     auto there = [&](int32_t id) { return id >= 0 && id < a.c.pages; };
-    // Row r of the unit: its values and position (requested ahead of what waits for
-    // the page), and from these what is stored.
+    // Row r of the unit, a token's head: its values and position (requested ahead of
+    // what waits for the page), and from these what is stored.
     struct Raw {
         float x[8];
         int64_t pos;
+        int k, h;  // token of the unit, head of the 2 hk
     };
     const bool turns = a.rot > 0 && g0 < a.c.hk && pk.turn;
     double freqs[4] = {};
@@ -376,13 +397,14 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
         for (int r = 0; r < 4; r++) freqs[r] = a.freqs[pk.e0 + r];
     }
     auto get = [&](int r, Raw& y) {
-        const int k = r / G, h = g0 + r - k * G;
-        const int64_t t = int64_t(u.row) + k;
-        load_row((h < a.c.hk ? a.k : a.v) + (t * a.c.hk + head(h)) * d, h < a.c.hk ? pk : pv, y.x);
+        y.k = int(page_of(uint32_t(r), by_heads));
+        y.h = g0 + r - y.k * G;
+        const int64_t t = int64_t(u.row) + y.k;
+        load_row((y.h < a.c.hk ? a.k : a.v) + (t * a.c.hk + head(y.h)) * d, y.h < a.c.hk ? pk : pv, y.x);
         y.pos = turns ? a.pos[t] : 0;
     };
-    auto make = [&](int r, Raw& y) {
-        if (g0 + r % G >= a.c.hk) return;
+    auto make = [&](Raw& y) {
+        if (y.h >= a.c.hk) return;
         float2 turn[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) turn[i] = angle(double(y.pos), freqs[i]);
@@ -391,8 +413,8 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
     };
     const int32_t first_id = kCodes ? page_id(u.begin) : 0;  // (a block lies in one page)
     const uint32_t slot0 = uint32_t(u.begin) - page_of(uint32_t(u.begin), a.c.div) * uint32_t(a.c.ps);
-    auto store = [&](int r, const Raw& y) {
-        const int k = r / G, h = g0 + r - k * G, tok = u.tok + k;
+    auto store = [&](const Raw& y) {
+        const int h = y.h, tok = u.tok + y.k;
         const Runs& p = h < a.c.hk ? pk : pv;
         uint32_t slot = slot0 + uint32_t(tok - u.begin);
         int32_t id = first_id;
@@ -407,8 +429,8 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
         for (int r = mine; r < rows; r += kRows) {
             Raw y;
             get(r, y);
-            make(r, y);
-            store(r, y);
+            make(y);
+            store(y);
         }
         return;
     }
@@ -425,22 +447,22 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
         if (u.tok > u.begin) old = *at;
     }
     __syncthreads();
-    auto note = [&](int r, const Raw& y) {
+    auto note = [&](const Raw& y) {
         const uint32_t big = largest<W>(y.x);
-        if (tid % W == 0) atomicMax(&most[r % G], big);
+        if (tid % W == 0) atomicMax(&most[y.h - g0], big);
     };
 #pragma unroll
     for (int i = 0; i < kHeld; i++) {
         if (mine + i * kRows < rows) {
-            make(mine + i * kRows, held[i]);
-            note(mine + i * kRows, held[i]);
+            make(held[i]);
+            note(held[i]);
         }
     }
     for (int r = mine + kHeld * kRows; r < rows; r += kRows) {
         Raw y;
         get(r, y);
-        make(r, y);
-        note(r, y);
+        make(y);
+        note(y);
     }
     __syncthreads();
     if (tid < G) {
@@ -453,12 +475,12 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kHeld; i++)
-        if (mine + i * kRows < rows) store(mine + i * kRows, held[i]);
+        if (mine + i * kRows < rows) store(held[i]);
     for (int r = mine + kHeld * kRows; r < rows; r += kRows) {
         Raw y;
         get(r, y);
-        make(r, y);
-        store(r, y);
+        make(y);
+        store(y);
     }
     if (u.tok == u.begin) return;
     for (int h = g0; h < g0 + G; h++) {
@@ -657,21 +679,34 @@ int iq_kv_extend(const float* q, const float* k, const float* v, int64_t T, int 
     a.span = codes ? a.sc.block : iq::kSpan;
     a.span_div = iq::page_div(uint32_t(a.span));
     const int rows = iq::kThreads / (a.c.d <= 32 ? 4 : a.c.d <= 64 ? 8 : a.c.d <= 128 ? 16 : 32);
-    int64_t all;
+    // workgroups: the cache's units (or tokens), then the query heads
+    int64_t cached, all;
+    auto parts = [](iq::Parts* p, int64_t n, int64_t groups) {
+        p->groups = uint32_t(groups);
+        p->div = iq::page_div(p->groups);
+        return n * groups;
+    };
     if (starts) {
         // as many heads as fill a workgroup's threads once, of the tokens that a unit has
         a.heads = std::min({2 * a.c.hk, iq::kMaxHeads, std::max(1, rows / std::min(a.span, rows))});
-        a.groups = uint32_t((2 * a.c.hk + a.heads - 1) / a.heads);
-        a.qgroups = uint32_t((q_heads + 2 * rows - 1) / (2 * rows));
-        a.cached = iq::max_units(T, B, a.span) * a.groups;
-        all = a.cached + T * a.qgroups;
+        const int groups = (2 * a.c.hk + a.heads - 1) / a.heads;
+        a.heads_div = iq::page_div(uint32_t(a.heads));
+        a.last_div = iq::page_div(uint32_t(2 * a.c.hk - (groups - 1) * a.heads));
+        cached = parts(&a.cached, iq::max_units(T, B, a.span), groups);
+        all = cached + (q_heads ? parts(&a.queries, T, (q_heads + 2 * rows - 1) / (2 * rows)) : 0);
     } else {
-        a.groups = uint32_t((q_heads + 2 * a.c.hk + rows - 1) / rows);
-        all = T * a.groups;
+        cached = all = parts(&a.cached, T, (q_heads + 2 * a.c.hk + rows - 1) / rows);
     }
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    for (; a.w0 < all; a.w0 += iq::kMaxGrid256) {
-        const unsigned grid = unsigned(std::min(all - a.w0, iq::kMaxGrid256));
+    for (int64_t w0 = 0; w0 < all; w0 += iq::kMaxGrid256) {
+        const unsigned grid = unsigned(std::min(all - w0, iq::kMaxGrid256));
+        auto begin = [](iq::Parts* p, int64_t w) {
+            p->first = w / p->groups;
+            p->group = uint32_t(w % p->groups);
+        };
+        a.rest = uint32_t(std::max<int64_t>(0, std::min<int64_t>(cached - w0, grid)));
+        if (a.rest) begin(&a.cached, w0);
+        if (a.rest < grid) begin(&a.queries, std::max<int64_t>(0, w0 - cached));
         switch (kv->type) {
             case IQ_KV_BF16: iq::launch_extend<IQ_KV_BF16>(a, grid, s); break;
             case IQ_KV_F16: iq::launch_extend<IQ_KV_F16>(a, grid, s); break;

@@ -313,3 +313,28 @@ def test_unaligned_inputs():
             got.append([out.cpu().numpy(), *pool.raw()])
     for g in got[1:]:
         assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(g, got[0]))
+
+
+@pytest.mark.parametrize("dtype", [I8, BF])
+def test_more_workgroups_than_a_launch_has(dtype):
+    """2^24 tokens and more, in one call of several launches (the last of the
+    cache's part and the first of the queries' in one)."""
+    T, d, page = 2 ** 24 + 1001, 16, 1024
+    pages = -(-T // page)
+    cache = ops.alloc_kv(pages, page, 1, d, dtype, block=1 if dtype == I8 else None)
+    table = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device="cuda").view(1, pages)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(T, 1, d, device="cuda", generator=gen)
+    starts, zero = torch.tensor([0, T], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    say("extend", dtype, T)
+    got = ops.kv_extend(x, x, x, None, None, cache, table, zero, starts=starts)
+    assert torch.equal(got, x)
+    del got
+    k, v = ops.kv_read(cache, table, starts, T=T)
+    assert torch.equal(k, v)
+    if dtype == I8:
+        # half a step, and the roundings of the scale, the quotient and the product (each of at most 127 steps)
+        step = x.abs().amax((1, 2), keepdim=True) / 127
+        assert torch.all((k - x).abs() <= (0.5 + 4 * 127 * EPS32) * step)
+    else:
+        assert torch.equal(k, x.to(BF).float())
