@@ -3,12 +3,12 @@
 // block of tokens and head), and cached tokens read back.
 //
 // Both move bytes; what they take beyond that is latency.  One token each of 16
-// sequences (28 query and 2 x 4 cached heads, e4m3) 4.0 us, of which an empty launch
+// sequences (28 query and 2 x 4 cached heads, e4m3) 4.1 us, of which an empty launch
 // is 1.4 and three dependent loads (length, page id, scale) most of the rest; 945
-// tokens in runs (int8, blocks of 32) 9.5 us for 32 MB (3.4 TB/s, a copy of as much
-// 4.6 out of the caches); 684 with norms (12 + 2 x 2 heads, e4m3, blocks of 8) 6.1.
-// Reading back 24155 tokens of 4 e4m3 heads as bf16: 16.5 us for 74 MB (4.5 TB/s, a
-// large copy's rate).
+// tokens in runs (int8, blocks of 32) 9.6 us for 32 MB, 2.5 us and 4.8 TB/s by what
+// 2950 take (23.2), a large copy's rate; 684 with norms (12 + 2 x 2 heads, e4m3,
+// blocks of 8) 5.9.  Reading back 24155 tokens of 4 e4m3 heads as bf16: 16.5 us for
+// 74 MB (4.5 TB/s).
 #include <algorithm>
 
 #include "iq_extend_plan.h"

@@ -225,3 +225,58 @@ def test_most_sequences(dtype, window, sinks):
     got, raw = out.cpu().numpy(), pool.raw()
     pool.raw = lambda: raw
     check(pool, q, lens, got, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", [I8, F8])
+def test_scores_past_fp32(dtype):
+    """Keys whose scores lie below fp32's range weigh nothing, a head with no
+    others gives zeros; scores above it give NaN."""
+    B, d, n = 4, 32, 70
+    pool = Pool(np.random.default_rng(5), B, 5, 16, 1, d, dtype, 2)
+    pool.fill(np.random.default_rng(6), [n] * B)
+    raw, t = pool.raw(), pool.table_np
+    q = np.zeros((B, 2, d), np.float32)
+    q[:, :, 0], q[:, 1, 0] = 4.0, -4.0
+    ones = 127 if dtype == I8 else 0x7e  # the largest code
+    raw[0][:] = 0
+    raw[0][..., 0] = ones
+    raw[2][:] = 0.01
+    raw[2][t[0, :4]] = 3e38      # sequence 0: 64 huge keys, then 6 of its own size
+    raw[2][t[1]] = 3e38          # 1: all huge
+    raw[2][t[2, 2], 3] = 3e38    # 2: two tokens
+    pool.put(raw)
+    out = ops.attn_decode(torch.from_numpy(q).cuda(), pool.cache, pool.table, torch.tensor([n] * B, dtype=torch.int32).cuda())
+    torch.cuda.synchronize()
+    got = out.cpu().numpy()
+    assert np.isnan(got[:3, 0]).all() and np.isfinite(got[3]).all()  # +inf
+    V = [pool.values(b, np.arange(n))[1][:, 0] for b in range(B)]
+    keep = [np.arange(n) >= 64, np.zeros(n, bool), ~((np.arange(n) >= 38) & (np.arange(n) < 40)), np.ones(n, bool)]
+    for b in range(B):
+        w = V[b][keep[b]]
+        want = w.mean(0) if len(w) else np.zeros(d)  # (equal keys)
+        most = (64 * EPS32 + 4 * EPS32) * np.abs(w).mean(0) if len(w) else 0.0
+        assert np.all(np.abs(got[b, 1] - want) <= most), b
+
+
+def test_two_streams_at_once():
+    """Calls on two streams that overlap: each its own workspace, each the
+    answer that it has alone."""
+    rng = np.random.default_rng(7)
+    jobs = []
+    for dtype in (I8, F8):
+        lens = [3000, 1, 700, 2500]
+        pool = Pool(rng, 4, 188, 16, 2, 128, dtype, 16)
+        pool.fill(rng, lens)
+        q = torch.from_numpy(rng.standard_normal((4, 12, 128)).astype(np.float32)).cuda()
+        n = torch.tensor(lens, dtype=torch.int32).cuda()
+        jobs.append((pool, q, n, ops.attn_decode(q, pool.cache, pool.table, n).clone(),
+                     [torch.empty_like(q) for _ in range(20)], torch.cuda.Stream()))
+    for j in jobs:
+        ops.init(0, j[5])
+    torch.cuda.synchronize()
+    for i in range(20):
+        for pool, q, n, _, outs, s in jobs:
+            ops.attn_decode(q, pool.cache, pool.table, n, out=outs[i], stream=s)
+    torch.cuda.synchronize()
+    for _, _, _, want, outs, _ in jobs:
+        assert all(torch.equal(o, want) for o in outs)
