@@ -181,10 +181,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
         }
         // the next tile's loads, and the id behind it ahead of them: a wait for it
         // then leaves them in flight (131072 tokens of 4 int8 heads: 35.7 and 31.1 us)
-        const Row r = row_of(tile + kAttnWaves, next_id);
-        next_id = page_id(tile + 2 * kAttnWaves);
-        load(ahead, r);
-        __builtin_amdgcn_sched_barrier(0);
+        if (tile + kAttnWaves < ntiles) {
+            const Row r = row_of(tile + kAttnWaves, next_id);
+            next_id = page_id(tile + 2 * kAttnWaves);
+            load(ahead, r);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
         float s[8], w[8];
