@@ -353,7 +353,7 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
  *
  * An 8-bit cache's blocks start anew with their first slot: with a = max |x| over
  * the call's tokens of the block (one head's k or v), in fp32, and Q = 127 (448),
- *   - a block whose first slot is among them, or whose scale is 0, gets the
+ *   - a block whose first slot is among them, or whose scale is not above 0, gets the
  *     scale s = max(a / Q, 2^-126), or 0 if a is 0;
  *   - a block that holds older tokens (the sequence's, below lens[b]) keeps its
  *     scale if a <= Q * s; otherwise s doubles until it is so and the older

@@ -280,3 +280,22 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for _, _, _, want, outs, _ in jobs:
         assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("dtype,B,hq,hk,d,window", [(I8, 150, 3, 1, 128, 0), (F8, 97, 4, 2, 64, 0), (BF, 200, 2, 1, 128, 500),
+                                                    (FP, 130, 4, 1, 64, 0), (I8, 300, 2, 2, 32, 77)])
+def test_long_rows_of_more_sequences_than_lanes(dtype, B, hq, hk, d, window):
+    """Over 64 sequences, some of several chunks."""
+    rng = np.random.default_rng(B)
+    lens = (np.exp(rng.uniform(0, np.log(900), B))).astype(np.int64)
+    lens[[0, 70, B - 1]] = [900, 871, 899]
+    lens[[3, 66]] = 0
+    pool = Pool(rng, B, 57, 16, hk, d, dtype, 16)
+    pool.fill(rng, lens)
+    q = rng.standard_normal((B, hq, d)).astype(np.float32)
+    out = ops.attn_decode(torch.from_numpy(q).cuda(), pool.cache, pool.table, torch.from_numpy(lens).int().cuda(),
+                          window=window, sinks=5)
+    torch.cuda.synchronize()
+    got, raw = out.cpu().numpy(), pool.raw()
+    pool.raw = lambda: raw
+    check(pool, q, lens, got, window, 5)
