@@ -41,6 +41,11 @@ constexpr float kNone = -3.4e38f;
 // are then 0 times 0 (or NaN, where a value is not finite), its weights 0.
 __device__ __forceinline__ float inv_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
+// What a kernel is built for: chunks of whole sequences' tokens, of the tokens
+// seen under a window, or whole sequences (under a window or not).  The last as
+// an argument instead cost the others 0.3 us of 17 (8-bit, 32 of up to 8192).
+enum AttnMode { kAll, kWindow, kWhole };
+
 struct Item {
     int b, n;            // sequence and its length (as given)
     int seen;            // tokens that it sees: n, or under a window fewer
@@ -60,11 +65,18 @@ __device__ __forceinline__ uint32_t chunks_by(uint32_t tiles, uint32_t c, double
 
 // The (sequence, chunk) number w of the batch's plan; false past the last.
 // Every wave finds it from the lengths by itself (64 sequences a step).  Under
-// a window (WIN) a sequence counts as the tokens that it sees.  Sizes of a chunk past
+// a window a sequence counts as the tokens that it sees.  Sizes of a chunk past
 // the first are tried at once: one after the other, 24 sequences of 16 heads
 // took 2.6 us here.
-template <bool WIN>
+template <int MODE>
 __device__ __forceinline__ bool find_item(const AttnArgs& a, uint32_t w, Item* it) {
+    constexpr bool WIN = MODE != kAll;
+    if constexpr (MODE == kWhole) {
+        if (w >= uint32_t(a.B)) return false;
+        const int len = a.t.lens[w];
+        *it = Item{int(w), len, min(len, a.visible), 0, attn_tiles(a.visible), 1, 0};
+        return true;
+    }
     const int lane = threadIdx.x & 63;
     auto length = [&](int b) { return b < a.B ? a.t.lens[b] : 0; };
     auto tiles_of = [&](int n) { return n < 0 || n > a.t.cap ? 0u : attn_tiles(WIN ? min(n, a.visible) : n); };
@@ -182,7 +194,7 @@ struct Terms<IQ_KV_F16> {
 
 // The split kernel of an 8-bit cache (iq_attn8.hip), and how many workgroups
 // of it run at once on a CU.
-void launch_attn8(const AttnArgs& a, bool window, unsigned grid, hipStream_t s);
+void launch_attn8(const AttnArgs& a, AttnMode mode, unsigned grid, hipStream_t s);
 int attn8_groups(int head_dim);
 
 }  // namespace iq

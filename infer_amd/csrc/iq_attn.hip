@@ -44,9 +44,10 @@ namespace {
 // DP: head_dim rounded up to 32, 64, 128 or 256.  WIN: of a sequence longer
 // than a.visible only the first a.sinks tokens and the newest others are seen;
 // they are numbered without the gap.
-template <int TYPE, int DP, bool WIN>
+template <int TYPE, int DP, int MODE>
 __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel(AttnArgs a) {
     using T = Terms<TYPE>;
+    constexpr bool WIN = MODE != kAll;
     constexpr int CH = DP / 8, RPI = 64 / CH, NI = kAttnTile / RPI;  // 16-byte chunks of a row, rows of a load, loads
     constexpr int KC = DP / 32, VT = DP / 16;                       // steps of the first product, tiles of the second
     constexpr int ROWB = DP * 2, KVB = kAttnTile * ROWB;
@@ -58,11 +59,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
     // chunk: workgroups are dealt to the 8 of them in turn.
     const uint32_t turn = a.lines ? 8 : 1, round = blockIdx.x / (turn * a.nh), in = blockIdx.x % (turn * a.nh);
     const uint32_t hidx = in / turn;
-    if (!find_item<WIN>(a, round * turn + in % turn, &it)) return;
+    if (!find_item<MODE>(a, round * turn + in % turn, &it)) return;
     const int b = it.b, n = it.n, d = a.c.d;
     const int j = int(hidx) / a.ht, h0 = int(hidx) % a.ht * 16, gh = min(16, a.group - h0);
     float* out = a.out + (int64_t(b) * a.hq + j * a.group + h0) * d;
-    if (hidx == 0 && it.j == 0 && threadIdx.x == 0) a.plan[b] = make_uint2(it.chunks, it.first);
+    if (MODE != kWhole && hidx == 0 && it.j == 0 && threadIdx.x == 0) a.plan[b] = make_uint2(it.chunks, it.first);
     if (n <= 0 || n > a.t.cap) {
         const float x = n == 0 ? 0.0f : __builtin_nanf("");
         for (int i = threadIdx.x; i < gh * d; i += 64 * kAttnWaves) out[i] = x;
@@ -427,12 +428,35 @@ __global__ __launch_bounds__(TH) void attn_weights_kernel(AttnArgs a, float* wei
     if (t < n) weights[row * wld + t] += sum;
 }
 
-template <int TYPE, bool WIN>
-void launch_attn(const AttnArgs& a, unsigned grid, hipStream_t s) {
-    if (a.c.d <= 32) attn_kernel<TYPE, 32, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else if (a.c.d <= 64) attn_kernel<TYPE, 64, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else if (a.c.d <= 128) attn_kernel<TYPE, 128, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else attn_kernel<TYPE, 256, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+template <int TYPE, int MODE>
+void launch_mode(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    if (a.c.d <= 32) attn_kernel<TYPE, 32, MODE><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else if (a.c.d <= 64) attn_kernel<TYPE, 64, MODE><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else if (a.c.d <= 128) attn_kernel<TYPE, 128, MODE><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else attn_kernel<TYPE, 256, MODE><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+}
+
+template <int TYPE>
+void launch_attn(const AttnArgs& a, AttnMode mode, unsigned grid, hipStream_t s) {
+    (mode == kWhole ? launch_mode<TYPE, kWhole> : mode == kWindow ? launch_mode<TYPE, kWindow> : launch_mode<TYPE, kAll>)(a, grid, s);
+}
+
+// The most tiles of a batch whose sequences are each one chunk: where more tiles
+// in a row (0.4 us each) cost less than the search for a chunk, its sums' way
+// through memory, the second launch and, with more pairs (sequence, kv head) than
+// CUs, a second round of workgroups.  Split and whole, us, 4 heads of 128 of int8:
+// 1 sequence of 256 tokens 8.1, 6.2, of 384 8.4, 7.4, of 512 8.6, 9.3; 32 of 512
+// 12.1, 10.6, of 1024 15.1, 16.3; 64 of up to 512 17.4, 10.4, of 1024 19.8, 16.9,
+// of up to 1024 22.5, 16.1.  Heads of 256: 1 of 384 11.1, 14.4, 32 of 512 17.5,
+// 18.6, 64 of 1024 37.5, 35.1.  bf16 under a window: 1 of 384 9.0, 9.7, 32 of 512
+// 15.6, 13.7, 64 of 512 20.5, 16.2.  With more tiles a long sequence among short
+// ones would be waited for (2048 tokens: 9.2 us split, 22.7 whole).  (16-bit
+// caches without a window keep the order of their sums, the split's.)
+int64_t whole_tiles(int64_t pairs, int d, int bytes) {
+    const int64_t cus = device_cu_count();
+    if (pairs >= cus) return 32;
+    if (2 * pairs >= cus && d <= 128) return 16;
+    return d * bytes <= 128 ? 12 : 8;
 }
 
 // The call behind either entry point; a: cache, scales and table, checked.
@@ -493,11 +517,15 @@ int attn_decode(AttnArgs a, const float* q, int B, int q_heads, float scale, int
         a.out = out + b0 * row;
         a.t.table = t.table + b0 * t.ld;
         a.t.lens = t.lens + b0;
-        int64_t grid = attn_max_items(a.B, a.nh, a.visible, a.target);
+        const int64_t pairs = int64_t(a.B) * a.nh;
+        const bool whole = (bits8 || win) && capt <= whole_tiles(pairs, a.c.d, bits8 ? 1 : 2);
+        int64_t grid = whole ? pairs : attn_max_items(a.B, a.nh, a.visible, a.target);
         if (a.lines) grid = (grid / a.nh + 7) / 8 * 8 * a.nh;
-        if (bits8) launch_attn8(a, win, unsigned(grid), s);
-        else if (a.c.type == IQ_KV_BF16) (win ? launch_attn<IQ_KV_BF16, true> : launch_attn<IQ_KV_BF16, false>)(a, unsigned(grid), s);
-        else (win ? launch_attn<IQ_KV_F16, true> : launch_attn<IQ_KV_F16, false>)(a, unsigned(grid), s);
+        const AttnMode mode = whole ? kWhole : win ? kWindow : kAll;
+        if (bits8) launch_attn8(a, mode, unsigned(grid), s);
+        else if (a.c.type == IQ_KV_BF16) launch_attn<IQ_KV_BF16>(a, mode, unsigned(grid), s);
+        else launch_attn<IQ_KV_F16>(a, mode, unsigned(grid), s);
+        if (whole) continue;
         // (a sequence has at most target / nh chunks and one more)
         const bool many = a.B <= 4 && std::min<int64_t>(capt / kAttnWaves, a.target / a.nh) > 64;
         const int th = many ? 1024 : 256;

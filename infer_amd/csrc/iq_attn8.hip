@@ -57,9 +57,10 @@ __device__ __forceinline__ s16x8_t codes_bf16(uint32_t lo, uint32_t hi) {
 }
 
 // DP: head_dim rounded up to 32, 64, 128 or 256.
-template <int TYPE, int DP, bool WIN>
+template <int TYPE, int DP, int MODE>
 __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kernel(AttnArgs a) {
     using T = Terms<IQ_KV_BF16>;
+    constexpr bool WIN = MODE != kAll;
     constexpr int CH = DP / 16, RPI = 64 / CH, NI = kAttnTile / RPI;  // 16-byte chunks of a row, rows of a load, loads
     constexpr int KC = DP / 32, VT = DP / 16;                         // steps of the first product, tiles of the second
     constexpr int KVB = kAttnTile * DP;
@@ -72,11 +73,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
     Item it;
     const uint32_t turn = a.lines ? 8 : 1, round = blockIdx.x / (turn * a.nh), in = blockIdx.x % (turn * a.nh);
     const uint32_t hidx = in / turn;
-    if (!find_item<WIN>(a, round * turn + in % turn, &it)) return;
+    if (!find_item<MODE>(a, round * turn + in % turn, &it)) return;
     const int b = it.b, n = it.n, d = a.c.d;
     const int j = int(hidx) / a.ht, h0 = int(hidx) % a.ht * 16, gh = min(16, a.group - h0);
     float* out = a.out + (int64_t(b) * a.hq + j * a.group + h0) * d;
-    if (hidx == 0 && it.j == 0 && threadIdx.x == 0) a.plan[b] = make_uint2(it.chunks, it.first);
+    if (MODE != kWhole && hidx == 0 && it.j == 0 && threadIdx.x == 0) a.plan[b] = make_uint2(it.chunks, it.first);
     if (n <= 0 || n > a.t.cap) {
         const float x = n == 0 ? 0.0f : __builtin_nanf("");
         for (int i = threadIdx.x; i < gh * d; i += 64 * kAttnWaves) out[i] = x;
@@ -300,12 +301,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
     }
 }
 
-template <int TYPE, bool WIN>
-void launch(const AttnArgs& a, unsigned grid, hipStream_t s) {
-    if (a.c.d <= 32) attn8_kernel<TYPE, 32, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else if (a.c.d <= 64) attn8_kernel<TYPE, 64, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else if (a.c.d <= 128) attn8_kernel<TYPE, 128, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
-    else attn8_kernel<TYPE, 256, WIN><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+template <int TYPE, int MODE>
+void launch_mode(const AttnArgs& a, unsigned grid, hipStream_t s) {
+    if (a.c.d <= 32) attn8_kernel<TYPE, 32, MODE><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else if (a.c.d <= 64) attn8_kernel<TYPE, 64, MODE><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else if (a.c.d <= 128) attn8_kernel<TYPE, 128, MODE><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+    else attn8_kernel<TYPE, 256, MODE><<<grid, 64 * kAttnWaves, 0, s>>>(a);
+}
+
+template <int TYPE>
+void launch(const AttnArgs& a, AttnMode mode, unsigned grid, hipStream_t s) {
+    (mode == kWhole ? launch_mode<TYPE, kWhole> : mode == kWindow ? launch_mode<TYPE, kWindow> : launch_mode<TYPE, kAll>)(a, grid, s);
 }
 
 }  // namespace
@@ -317,9 +323,9 @@ void launch(const AttnArgs& a, unsigned grid, hipStream_t s) {
 // flight, more of them only add chunks.
 int attn8_groups(int head_dim) { return head_dim <= 64 ? 3 : 1; }
 
-void launch_attn8(const AttnArgs& a, bool window, unsigned grid, hipStream_t s) {
-    if (a.c.type == IQ_KV_I8) (window ? launch<IQ_KV_I8, true> : launch<IQ_KV_I8, false>)(a, grid, s);
-    else (window ? launch<IQ_KV_E4M3, true> : launch<IQ_KV_E4M3, false>)(a, grid, s);
+void launch_attn8(const AttnArgs& a, AttnMode mode, unsigned grid, hipStream_t s) {
+    if (a.c.type == IQ_KV_I8) launch<IQ_KV_I8>(a, mode, grid, s);
+    else launch<IQ_KV_E4M3>(a, mode, grid, s);
 }
 
 }  // namespace iq

@@ -299,3 +299,36 @@ def test_long_rows_of_more_sequences_than_lanes(dtype, B, hq, hk, d, window):
     got, raw = out.cpu().numpy(), pool.raw()
     pool.raw = lambda: raw
     check(pool, q, lens, got, window, 5)
+
+
+@pytest.mark.parametrize("dtype,B,hq,hk,d,tiles", [(I8, 1, 6, 1, 128, 12), (I8, 1, 6, 1, 128, 13), (F8, 2, 4, 2, 256, 8),
+                                                   (F8, 2, 4, 2, 256, 9), (I8, 43, 6, 3, 128, 16), (I8, 43, 6, 3, 128, 17),
+                                                   (F8, 300, 2, 1, 64, 32), (F8, 300, 2, 1, 64, 33), (I8, 70, 4, 4, 256, 32),
+                                                   (BF, 3, 4, 2, 64, 12), (FP, 2, 4, 1, 128, 8), (BF, 65, 8, 2, 80, 16),
+                                                   (BF, 70, 4, 4, 256, 32), (FP, 70, 4, 4, 256, 33), (F8, 9, 80, 2, 32, 12)])
+def test_sequences_whole_and_split(dtype, B, hq, hk, d, tiles):
+    """Tables of as many tiles of 32 tokens as one workgroup takes in a row, and
+    of one more; of 16-bit caches, windows of them in longer tables."""
+    rng = np.random.default_rng(B + tiles)
+    n = tiles * 32
+    if dtype in CODES:
+        lens = [n, 0, 1, n - 1, 33][:B] + rng.integers(0, n + 1, max(0, B - 5)).tolist()
+        run(rng, lens, hq, hk, d, 32, 32, dtype)
+    else:
+        lens = [n + 70, 0, n, n + 1, 5][:B] + rng.integers(0, n + 71, max(0, B - 5)).tolist()
+        run(rng, lens, hq, hk, d, 32, None, dtype, window=n - 3, sinks=3)
+
+
+@pytest.mark.parametrize("dtype,window", [(I8, 0), (BF, 300)])
+def test_lengths_out_of_range_of_whole_sequences(dtype, window):
+    rng = np.random.default_rng(8)
+    lens = [40, 0, 200, 320, 7]
+    pool, q, out = run(rng, lens, 4, 2, 64, 16, 16, dtype, window=window, width=21)
+    bad = [40, -1, 200, 337, 2 ** 31 - 1]
+    got = torch.empty_like(out)
+    ops.attn_decode(torch.from_numpy(q).cuda(), pool.cache, pool.table, torch.tensor(bad, dtype=torch.int32).cuda(), out=got, window=window)
+    for b in range(5):
+        if bad[b] == lens[b]:
+            assert torch.equal(got[b], out[b])
+        else:
+            assert torch.isnan(got[b]).all()
