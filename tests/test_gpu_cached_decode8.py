@@ -273,3 +273,31 @@ def test_a_ring_of_pages_under_a_window(dtypes):
             got.append(step.logits.clone())
     assert all(torch.equal(a, b) for a, b in zip(got[:120], got[120:]))
     assert torch.isfinite(got[-1]).all()
+
+
+def test_norms_with_kept_weights_and_evictions():
+    """Layers with norms over 16-bit caches whose rows are evicted: tokens go
+    behind what is left, at positions that go on; the weights of what was cached
+    add up to one per head and step."""
+    B = 3
+    rng, host, step, table = build(31, B, (BF, BF))
+    step = C.CachedDecodeStep(step.model, step.caches, step.table, weights=True)
+    c = host["cfg"]
+    group = c["heads"] // c["kv_heads"]
+    lens, pos = np.zeros(B, np.int64), np.zeros(B, np.int64)
+    for it in range(45):
+        before = [w.double().sum(-1).cpu().numpy() for w in step.weights]
+        step.step(rng.integers(0, c["vocab"], B).tolist())
+        torch.cuda.synchronize()
+        lens, pos = lens + 1, pos + 1
+        assert step.lens.cpu().tolist() == lens.tolist() == step.held.cpu().tolist()
+        assert step.positions.cpu().tolist() == pos.tolist()
+        check_layers(step, host, table, lens, pos - 1)
+        for w, old in zip(step.weights, before):
+            # a weight is 2^x / l with |x| below 64 (rows of norm 8 * 2.2 at most): two roundings of x and
+            # 64 half steps more (exp, sums, division), in it and in l; and the additions' own rounding
+            new = w.double().sum(-1).cpu().numpy()
+            assert np.all(np.abs(new - old - group) <= 2 * (2 * 64 + 64) * EPS32 * group + (group + 1) * EPS32 * new)
+        if it in (19, 33):
+            step.evict(9, 4)
+            lens = np.minimum(lens, 9)
