@@ -452,8 +452,7 @@ void launch_attn(const AttnArgs& a, AttnMode mode, unsigned grid, hipStream_t s)
 // 15.6, 13.7, 64 of 512 20.5, 16.2.  With more tiles a long sequence among short
 // ones would be waited for (2048 tokens: 9.2 us split, 22.7 whole).  (16-bit
 // caches without a window keep the order of their sums, the split's.)
-int64_t whole_tiles(int64_t pairs, int d, int bytes) {
-    const int64_t cus = device_cu_count();
+int64_t whole_tiles(int64_t pairs, int cus, int d, int bytes) {
     if (pairs >= cus) return 32;
     if (2 * pairs >= cus && d <= 128) return 16;
     return d * bytes <= 128 ? 12 : 8;
@@ -488,7 +487,8 @@ int attn_decode(AttnArgs a, const float* q, int B, int q_heads, float scale, int
     // 16.5, 16.9, 18.3; d = 32, 8 of 16384 46.9, 38.3, 37.7, 38.6.  (The choice goes
     // into the order of a result's sums; 8-bit caches have their own.)
     const int groups = bits8 ? attn8_groups(a.c.d) : a.c.d <= 32 ? 4 : a.c.d <= 64 ? 3 : a.c.d <= 128 ? 2 : 1;
-    a.target = uint32_t(groups * device_cu_count());
+    const int cus = device_cu_count();
+    a.target = uint32_t(groups * cus);
     // Neighbouring heads' rows meet in a cache line, or several head tiles read
     // the same rows: one XCD's L2 then serves them (8 sequences of 16384, 8 heads
     // of 32: 49.7 -> 38.8 us; of 8192, heads of 80: 50.1 -> 44.6).  Whole lines
@@ -518,7 +518,7 @@ int attn_decode(AttnArgs a, const float* q, int B, int q_heads, float scale, int
         a.t.table = t.table + b0 * t.ld;
         a.t.lens = t.lens + b0;
         const int64_t pairs = int64_t(a.B) * a.nh;
-        const bool whole = (bits8 || win) && capt <= whole_tiles(pairs, a.c.d, bits8 ? 1 : 2);
+        const bool whole = (bits8 || win) && capt <= whole_tiles(pairs, cus, a.c.d, bits8 ? 1 : 2);
         int64_t grid = whole ? pairs : attn_max_items(a.B, a.nh, a.visible, a.target);
         if (a.lines) grid = (grid / a.nh + 7) / 8 * 8 * a.nh;
         const AttnMode mode = whole ? kWhole : win ? kWindow : kAll;
