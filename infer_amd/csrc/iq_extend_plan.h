@@ -1,7 +1,8 @@
 // iq_extend_plan.h -- how the new tokens of sequences are split into units, a
 // block of a sequence's tokens each (or `span` of them, for a 16-bit cache):
 // arithmetic shared by extend_kernel (iq_kv8.hip), its host side and the CPU
-// tests (plain C++: g++ compiles it on its own).
+// tests (plain C++: g++ compiles it on its own).  Also the way of threads
+// through a block's older rows.
 #pragma once
 
 #include <algorithm>
@@ -50,5 +51,23 @@ IQ_HD Unit unit_at(uint32_t nth, int32_t len, NewTokens n, int32_t span, PageDiv
 // At most so many units of all sequences whose rows do not overlap: n tokens
 // touch at most (n - 1) / span + 2.
 inline int64_t max_units(int64_t T, int64_t B, int64_t span) { return T / span + 2 * std::min(B, T); }
+
+// The 16-byte pieces of rows, `per` each, dealt to threads in turn.  Row and
+// piece apart: a block may have 2^27 rows of 16 pieces and more, whose product
+// passes 32 bits, while a row (below 0x7fff0000) with a step stays inside them.
+struct Piece {
+    int32_t row, col;
+};
+IQ_HD Piece piece_of(int32_t n, int32_t per) { return {n / per, n % per}; }
+// The piece `step` (piece_of(threads, per)) behind p.
+IQ_HD Piece piece_behind(Piece p, Piece step, int32_t per) {
+    p.row += step.row;
+    p.col += step.col;
+    if (p.col >= per) {
+        p.col -= per;
+        p.row++;
+    }
+    return p;
+}
 
 }  // namespace iq

@@ -254,11 +254,11 @@ __device__ __forceinline__ uint32_t halved4(uint32_t u, int up) {
 // `rows` rows of 16 byte pieces from `base`, halved, by `threads` threads.
 template <int TYPE>
 __device__ __forceinline__ void halve_rows(char* base, int rows, int d, uint32_t stride, int up, int first, int threads) {
-    const int per = d / 16, n = rows * per;
+    const int per = d / 16;
+    const Piece step = piece_of(threads, per);
 #pragma unroll 4
-    for (int i = first; i < n; i += threads) {
-        const int r = i / per;
-        u32x4_t* at = reinterpret_cast<u32x4_t*>(base + uint64_t(uint32_t(r)) * stride + (i - r * per) * 16);
+    for (Piece p = piece_of(first, per); p.row < rows; p = piece_behind(p, step, per)) {
+        u32x4_t* at = reinterpret_cast<u32x4_t*>(base + uint64_t(uint32_t(p.row)) * stride + p.col * 16);
         u32x4_t x = *at;
 #pragma unroll
         for (int c = 0; c < 4; c++) x[c] = halved4<TYPE>(x[c], up);
