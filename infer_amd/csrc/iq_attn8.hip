@@ -177,7 +177,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn8_kerne
             *reinterpret_cast<u32x4_t*>(vl + r * DP + (ch ^ vsw(r)) * 16) = ahead.v[i];
         }
         if (lane < kAttnTile) {
-            tile_ks[wave][lane] = ahead.ks * a.mul;
+            // (an infinite one becomes NaN, by the sum with 0 times it: its negative
+            // products, -inf, would weigh nothing)
+            tile_ks[wave][lane] = fmaf(ahead.ks, a.mul, ahead.ks * 0.0f);
             tile_vs[wave][lane] = ahead.vs;
         }
         // the next tile's loads, and the id behind it ahead of them: a wait for it
