@@ -237,7 +237,10 @@ void iq_chain_destroy(iq_chain* chain);
  * -127..127, or e4m3 numbers up to 448) with a scale for every `block`
  * consecutive slots of a page and key/value head: the value of a code is code *
  * scale.  iq_kv_append, iq_attn_decode and iq_kv_evict take 16-bit caches
- * (IQ_EKIND); iq_kv_extend, iq_kv_read and iq_attn_decode_window take all. */
+ * (IQ_EKIND); iq_kv_extend, iq_kv_read and iq_attn_decode_window take all.
+ * What a call makes for its caller (q_out, out, k_out, v_out) must not overlap
+ * the cache's rows or scales (IQ_EALIAS); between them, in a larger tensor, it
+ * may lie. */
 enum { IQ_KV_BF16 = 0, IQ_KV_F16 = 1, IQ_KV_I8 = 2, IQ_KV_E4M3 = 3 };
 
 typedef struct iq_kv {

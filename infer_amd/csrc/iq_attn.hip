@@ -467,7 +467,7 @@ int attn_decode(AttnArgs a, const float* q, int B, int q_heads, float scale, int
     if (window < 0 || sinks < 0) return IQ_ESHAPE;
     if (weights && weights_ld < a.t.cap) return IQ_ESHAPE;
     const int64_t row = int64_t(q_heads) * a.c.d;
-    if (ranges_overlap(q, B * row * 4, out, B * row * 4)) return IQ_EALIAS;
+    if (ranges_overlap(q, B * row * 4, out, B * row * 4) || meets_cache(out, B * row * 4, a.c, a.scales)) return IQ_EALIAS;
     Workspace* ws = nullptr;
     const hipError_t e = get_workspace(s, &ws);
     if (e != hipSuccess) return e == hipErrorOutOfMemory ? IQ_ENOMEM : int(e);

@@ -7,6 +7,7 @@
 #include "../../include/iq.h"
 #include "iq_attn_plan.h"
 #include "iq_internal.h"
+#include "iq_overlap.h"
 
 namespace iq {
 
@@ -81,11 +82,6 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
     return uint32_t(__builtin_amdgcn_readlane(int(v), lane));
 }
 
-inline bool ranges_overlap(const void* a, int64_t abytes, const void* b, int64_t bbytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return a && b && x < y + uintptr_t(bbytes) && y < x + uintptr_t(abytes);
-}
-
 inline bool is_kv8(int type) { return type == IQ_KV_I8 || type == IQ_KV_E4M3; }
 
 // Strides over n things, of which a single one's is not used, in elements.
@@ -151,6 +147,17 @@ inline int check_any_kv(const iq_kv* kv, const iq_kv_scales* sc, KvView* out, Kv
     scales->v = sc->v;
     scales->div = page_div(uint32_t(sc->block));
     return IQ_OK;
+}
+
+// Whether an output meets the cache's values or scales.
+inline bool meets_cache(const void* a, int64_t bytes, const KvView& c, const KvScales& sc) {
+    const int64_t size = is_kv8(c.type) ? 1 : 2, n[3] = {c.pages, c.ps, c.hk};
+    const int64_t stride[3] = {c.pstr * size, c.sstr * size, c.hstr * size};
+    for (const void* pool : {static_cast<const void*>(c.k), static_cast<const void*>(c.v)})
+        if (meets_rows(a, bytes, pool, n, stride, c.d * size)) return true;
+    if (!sc.block) return false;
+    const int64_t ns[3] = {c.pages, c.ps / sc.block, c.hk}, strides[3] = {int64_t(sc.pstr) * 4, int64_t(sc.bstr) * 4, int64_t(sc.hstr) * 4};
+    return meets_rows(a, bytes, sc.k, ns, strides, 4) || meets_rows(a, bytes, sc.v, ns, strides, 4);
 }
 
 inline int check_table(const KvView& c, const int32_t* table, int64_t ld, int64_t max_pages, const int32_t* lens,

@@ -579,6 +579,7 @@ int iq_kv_append(const float* q, const float* k, const float* v, const int64_t* 
     if (q_heads) {
         if (q_out != q && iq::ranges_overlap(q_out, qn, q, qn)) return IQ_EALIAS;
         if (iq::ranges_overlap(q_out, qn, k, kn) || iq::ranges_overlap(q_out, qn, v, kn)) return IQ_EALIAS;
+        if (iq::meets_cache(q_out, qn, a.c, iq::KvScales{})) return IQ_EALIAS;
     }
     a.freqs = freqs;
     a.hq = q_heads;

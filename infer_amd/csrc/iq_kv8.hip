@@ -658,7 +658,7 @@ int iq_kv_extend(const float* q, const float* k, const float* v, int64_t T, int 
     if (!k || !v || (q_heads && (!q || !q_out)) || (rot_dim && (!positions || !freqs))) return IQ_ENULL;
     const int64_t qb = T * q_heads * a.c.d * 4, kb = T * a.c.hk * a.c.d * 4;
     if (q_heads && ((q_out != q && iq::ranges_overlap(q, qb, q_out, qb)) || iq::ranges_overlap(k, kb, q_out, qb) ||
-                    iq::ranges_overlap(v, kb, q_out, qb)))
+                    iq::ranges_overlap(v, kb, q_out, qb) || iq::meets_cache(q_out, qb, a.c, a.sc)))
         return IQ_EALIAS;
     const bool codes = iq::is_kv8(kv->type);
     a.q = q;
@@ -732,6 +732,7 @@ int iq_kv_read(const iq_kv* kv, const iq_kv_scales* scales, const int32_t* table
     const int64_t bytes = T * a.c.hk * a.c.d * (out_type == IQ_READ_F32 ? 4 : 2);
     if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16) return IQ_ESHAPE;
     if (iq::ranges_overlap(k_out, bytes, v_out, bytes)) return IQ_EALIAS;
+    if (iq::meets_cache(k_out, bytes, a.c, a.sc) || iq::meets_cache(v_out, bytes, a.c, a.sc)) return IQ_EALIAS;
     a.t.lens = first;
     a.starts = starts;
     a.B = B;
