@@ -52,16 +52,7 @@ struct Item {
     uint32_t j, c, chunks, first;  // chunk, tiles of a chunk, chunks of the sequence, its first partial
 };
 
-// attn_chunks with 1 / c: (tiles - 1/2) / c + 1 lies at least 1 / 2c from a whole
-// number, and its error (2^-46 of at most 2^26 / c, from a reciprocal of 23 bits
-// and a Newton step) is far less.  An integer division takes five times as long.
-__device__ __forceinline__ double chunk_rcp(uint32_t c) {
-    const double x = double(c), r = __builtin_amdgcn_rcp(x);
-    return fma(r, fma(-x, r, 1.0), r);
-}
-__device__ __forceinline__ uint32_t chunks_by(uint32_t tiles, uint32_t c, double rcp) {
-    return tiles <= c ? 1 : uint32_t(fma(double(tiles) - 0.5, rcp, 1.0));
-}
+__device__ __forceinline__ double chunk_rcp(uint32_t c) { return attn_rcp(c, __builtin_amdgcn_rcp(double(c))); }
 
 // The (sequence, chunk) number w of the batch's plan; false past the last.
 // Every wave finds it from the lengths by itself (64 sequences a step).  Under
@@ -89,34 +80,28 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, uint32_t w, Item* i
     double rcp = chunk_rcp(c);
     auto items_of = [&](int b0, uint32_t size, double r) {
         const uint32_t t = tiles_of(b0 ? length(b0 + lane) : n0);
-        return lane_of(wave_scan(b0 + lane < a.B ? chunks_by(t, size, r) : 0), 63);
+        return lane_of(wave_scan(b0 + lane < a.B ? attn_chunks_by(t, size, r) : 0), 63);
     };
     if (uint32_t(a.B) * a.nh <= a.target) {
-        uint32_t items = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 64) items += items_of(b0, c, rcp);
-        if (items * a.nh > a.target) {
-            uint32_t more[kAttnTries] = {};
+        uint32_t items[kAttnTries] = {};
+        for (int b0 = 0; b0 < a.B; b0 += 64) items[0] += items_of(b0, c, rcp);
+        if (items[0] * a.nh > a.target) {
             for (int b0 = 0; b0 < a.B; b0 += 64) {
                 uint32_t size = least;
 #pragma unroll
                 for (int i = 1; i < kAttnTries; i++) {
                     size = attn_more_tiles(size, least);
-                    more[i] += items_of(b0, size, chunk_rcp(size));
+                    items[i] += items_of(b0, size, chunk_rcp(size));
                 }
             }
-            c = attn_more_tiles(c, least);
-#pragma unroll
-            for (int i = 1; i < kAttnTries; i++) {
-                if (more[i] * a.nh <= a.target) break;
-                c = attn_more_tiles(c, least);
-            }
+            c = attn_pick_tiles(least, items, a.nh, a.target);
             rcp = chunk_rcp(c);
         }
     }
     uint32_t before = 0, first = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         if (b0) n = length(b0 + lane);
-        const uint32_t k = b0 + lane < a.B ? chunks_by(tiles_of(n), c, rcp) : 0;
+        const uint32_t k = b0 + lane < a.B ? attn_chunks_by(tiles_of(n), c, rcp) : 0;
         const uint32_t upto = wave_scan(k), many = k > 1 ? k : 0, pupto = wave_scan(many);
         const uint64_t past = __ballot(w < before + upto);
         if (past) {

@@ -52,7 +52,32 @@ IQ_HD uint32_t attn_chunk_tiles(uint32_t total, uint32_t heads, uint32_t target)
 }
 IQ_HD uint32_t attn_more_tiles(uint32_t c, uint32_t least) { return c + (least + 7) / 8; }
 
+// Of the sizes tried, least and kAttnTries - 1 behind it, with items[i] chunks
+// of all sequences each: the first that is at most `target` work items, or the
+// one behind the last.
+IQ_HD uint32_t attn_pick_tiles(uint32_t least, const uint32_t (&items)[kAttnTries], uint32_t heads, uint32_t target) {
+    uint32_t c = least;
+    for (int i = 0; i < kAttnTries; i++) {
+        if (items[i] * heads <= target) break;
+        c = attn_more_tiles(c, least);
+    }
+    return c;
+}
+
+// A sequence's chunks; the kernels have them from attn_chunks_by.
 IQ_HD uint32_t attn_chunks(uint32_t tiles, uint32_t c) { return tiles <= c ? 1 : (tiles + c - 1) / c; }
+
+// The same with 1 / c: (tiles - 1/2) / c + 1 lies at least 1 / 2c from a whole
+// number, and its error (2^-46 of at most 2^26 / c, from a reciprocal of 23 bits,
+// `near`, and a Newton step) is far less.  An integer division takes five times
+// as long.
+IQ_HD double attn_rcp(uint32_t c, double near) {
+    const double x = double(c);
+    return __builtin_fma(near, __builtin_fma(-x, near, 1.0), near);
+}
+IQ_HD uint32_t attn_chunks_by(uint32_t tiles, uint32_t c, double rcp) {
+    return tiles <= c ? 1 : uint32_t(__builtin_fma(double(tiles) - 0.5, rcp, 1.0));
+}
 
 // Bounds over all lengths up to `cap` tokens: work items, and those of
 // sequences with more than one chunk (which have a partial result each).
