@@ -362,7 +362,14 @@ int iq_kv_evict(const iq_kv* kv, const int32_t* table, int64_t table_ld, int64_t
  *     scale if a <= Q * s; otherwise s doubles until it is so and the older
  *     tokens' codes are halved as often, at once, to nearest even.  So a stored
  *     value is off by less than one step of its block's scale (int8; half a
- *     step where the scale did not grow), however often it grew.
+ *     step where the scale did not grow), however often it grew.  The comparison
+ *     is exact and s a quotient rounded to nearest: where Q * s came out below the
+ *     a that made it (two in five to one half of all a), the same a in a later call
+ *     doubles the scale, once.  Tokens of one call, and blocks of one slot, do not
+ *     meet this.
+ * A unit of work is a block's tokens of a call and one key/value head: blocks of
+ * 8 to 64 slots are fast, larger ones leave few units of many steps, and a scale that
+ * grows costs its block's older tokens read and written.
  * Codes are x / s to nearest even.  A value that is not finite makes its block's
  * scale NaN, and all that is read from the block, until the block starts anew. */
 int iq_kv_extend(const float* q, const float* k, const float* v, int64_t T, int q_heads, const uint16_t* q_norm,
