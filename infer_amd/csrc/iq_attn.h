@@ -177,8 +177,8 @@ struct Terms<IQ_KV_F16> {
     }
 };
 
-// The split kernel of an 8-bit cache (iq_attn8.hip), and how many workgroups
-// of it run at once on a CU.
+// The split kernel of an 8-bit cache (iq_attn8.hip), and for how many workgroups
+// of it a CU the batch is split (no more than run at once).
 void launch_attn8(const AttnArgs& a, AttnMode mode, unsigned grid, hipStream_t s);
 int attn8_groups(int head_dim);
 

@@ -41,9 +41,9 @@
 namespace iq {
 namespace {
 
-// DP: head_dim rounded up to 32, 64, 128 or 256.  WIN: of a sequence longer
-// than a.visible only the first a.sinks tokens and the newest others are seen;
-// they are numbered without the gap.
+// DP: head_dim rounded up to 32, 64, 128 or 256.  MODE: AttnMode.  Under a window
+// (WIN) of a sequence longer than a.visible only the first a.sinks tokens and the
+// newest others are seen; they are numbered without the gap.
 template <int TYPE, int DP, int MODE>
 __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel(AttnArgs a) {
     using T = Terms<TYPE>;
@@ -229,6 +229,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void attn_kernel
         }
         s16x8_t pt[T::N];
         T::cut(p, pt);
+        // (all VT tiles of columns, also past head_dim: a branch around those costs whole
+        // heads 1 to 4 %, 24 sequences of up to 2047, 16 heads of 256 120.5 -> 125.9 us, of
+        // 128 40.5 -> 40.8, and gains the others about 1 % at most, 16 heads of 80 31.9 -> 31.8, of
+        // 144 110.2 -> 109.0, of 160 110.3 -> 110.8)
 #pragma unroll
         for (int v = 0; v < VT; v++) {
             // rows 4g..4g+3 of either half: lane 4r + c of 16 gives row r's
@@ -444,14 +448,25 @@ void launch_attn(const AttnArgs& a, AttnMode mode, unsigned grid, hipStream_t s)
 // The most tiles of a batch whose sequences are each one chunk: where more tiles
 // in a row (0.4 us each) cost less than the search for a chunk, its sums' way
 // through memory, the second launch and, with more pairs (sequence, kv head) than
-// CUs, a second round of workgroups.  Split and whole, us, 4 heads of 128 of int8:
-// 1 sequence of 256 tokens 8.1, 6.2, of 384 8.4, 7.4, of 512 8.6, 9.3; 32 of 512
-// 12.1, 10.6, of 1024 15.1, 16.3; 64 of up to 512 17.4, 10.4, of 1024 19.8, 16.9,
-// of up to 1024 22.5, 16.1.  Heads of 256: 1 of 384 11.1, 14.4, 32 of 512 17.5,
-// 18.6, 64 of 1024 37.5, 35.1.  bf16 under a window: 1 of 384 9.0, 9.7, 32 of 512
-// 15.6, 13.7, 64 of 512 20.5, 16.2.  With more tiles a long sequence among short
-// ones would be waited for (2048 tokens: 9.2 us split, 22.7 whole).  (16-bit
-// caches without a window keep the order of their sums, the split's.)
+// CUs, a second round of workgroups.  Split and whole, us a call in a graph, by
+// sequences x tiles, 4 key/value heads:
+//   int8, 128     1 x 8 8.9, 7.0   1 x 12 9.0, 8.5     1 x 16 9.1, 9.9   32 x 16 11.7, 10.4
+//                 32 x 32 15.0, 16.5   64 x 16 13.3, 11.1   64 x 32 19.1, 17.0   128 x 32 31.1, 27.9
+//   int8, 32      1 x 12 7.3, 5.5  1 x 16 7.4, 6.3     32 x 32 10.7, 9.9 64 x 32 12.7, 10.3
+//   int8, 256     1 x 8 11.3, 11.3 1 x 12 11.5, 14.9   32 x 16 16.9, 19.2
+//                 64 x 16 22.2, 20.3   64 x 32 34.0, 32.5   (e4m3: 1 x 8 10.9, 10.3)
+//   bf16 under a window
+//        32       1 x 8 7.5, 5.2   1 x 12 7.7, 6.1     32 x 16 8.8, 7.2  64 x 32 13.3, 11.9
+//        64       1 x 8 8.1, 6.2   1 x 12 8.2, 7.4     1 x 13 8.3, 8.5   64 x 32 19.8, 15.9
+//        128      1 x 8 9.5, 8.4   1 x 12 9.6, 10.3    32 x 16 14.5, 13.5
+//                 64 x 16 21.1, 16.9   64 x 32 30.4, 26.1   256 x 32 107, 102
+//        256      1 x 4 10.4, 9.9  1 x 8 13.0, 14.3    32 x 16 24.9, 26.9   64 x 32 55.3, 53.3
+// (1 x 8 of 256 in 16 bits is the one size where the rule takes the slower side.)
+// With more tiles a long sequence among short ones would be waited for (2048
+// tokens: 9.2 us split, 22.7 whole).  It goes by the table's width, the lengths
+// being on the device: in a wide table a short sequence is split and pays 2 us for
+// it (17 tokens 5.6, in a table of 128 pages of 16 and more 7.7).  (16-bit caches
+// without a window keep the order of their sums, the split's.)
 int64_t whole_tiles(int64_t pairs, int cus, int d, int bytes) {
     if (pairs >= cus) return 32;
     if (2 * pairs >= cus && d <= 128) return 16;

@@ -9,15 +9,16 @@
 // mantissa hold -127..127; e4m3 is a part of bf16), so a tile's rows go through
 // LDS as bytes and become bf16 operands in registers.  A key's scale multiplies
 // its score, a value's its weight before that is cut into three bf16 terms,
-// which have fp32's range, so that scales of any size lose nothing.
+// which have fp32's range, so that scales from 2^-86 on lose nothing.
 //
 // What bounds it is the read of the cache: 131072 tokens of 4 int8 heads of 128 in
-// 31 us (4.3 TB/s over all, 5.6 behind the first tile, where a plain read reaches
-// 5.5 on as many bytes), every byte read once, the vector units busy for 56 % of it
-// (int8 to bf16: 1.5 operations a code; e4m3: 0.5), the matrix cores for 21 %, no
+// 31 us (4.3 TB/s over all, 5.2 behind the first tile, where a plain read reaches
+// 5.5 on as many bytes), every byte read once, the vector units busy for 45 % of it
+// (int8 to bf16: 1.5 operations a code; e4m3: 0.5), the matrix cores for 18 %, no
 // bank conflicts.  The rest is a launch with its chain of length, page id and
-// rows (6 us) and the chunk's end (3 us): 32 sequences of up to 8192, 2 e4m3 heads,
-// 13.4 us (3.2 TB/s).  Two tiles ahead instead of one gain nothing (131072 tokens,
+// rows (4.2 us; 5.6 for 24 sequences of up to 2047, 16 heads of 64), a tile's products
+// (1.2 to 1.5) and the chunk's end (1): 32 sequences of up to 8192, 2 e4m3 heads, 15.1 us
+// (2.9 TB/s).  Two tiles ahead instead of one gain nothing (131072 tokens,
 // both launches, 33.2 and 33.9 us).
 //
 // K: a lane's 16 bytes are two 8-value operands, so the 32-value steps of the

@@ -3,12 +3,20 @@
 // block of tokens and head), and cached tokens read back.
 //
 // Both move bytes; what they take beyond that is latency.  One token each of 16
-// sequences (28 query and 2 x 4 cached heads, e4m3) 4.1 us, of which an empty launch
+// sequences (28 query and 2 x 4 cached heads, e4m3) 4.0 us, of which an empty launch
 // is 1.4 and three dependent loads (length, page id, scale) most of the rest; 945
-// tokens in runs (int8, blocks of 32) 9.6 us for 32 MB, 2.5 us and 4.8 TB/s by what
+// tokens in runs (int8, blocks of 32) 9.7 us for 32 MB, 2.5 us and 4.8 TB/s by what
 // 2950 take (23.2), a large copy's rate; 684 with norms (12 + 2 x 2 heads, e4m3,
-// blocks of 8) 5.9.  Reading back 24155 tokens of 4 e4m3 heads as bf16: 16.5 us for
-// 74 MB (4.5 TB/s).
+// blocks of 8) 5.9.  Into a bf16 cache, calls of a graph: the 945 tokens 7.7 us (33 MB,
+// 4.3 TB/s), 2048 in one run 15.3 (4.7 TB/s; int8 in blocks of 8 to 64 14.1 to 15.4).
+// Reading back 24155 tokens of 4 e4m3 heads as bf16: 16.7 us for 74 MB (4.4 TB/s).
+//
+// A scale that grows has its block's older codes read and written: the 16 tokens
+// 5.9 us in int8 blocks of 16 (3.3 where none grows), 13.3 in blocks of 64, 43 of 256, by
+// the threads of one row; in runs, where a workgroup has them, 4 x 200 tokens behind
+// half a block 10.6 either way in blocks of 16, 24.0 and 22.1 of 256.  A block of a
+// head is one workgroup's: with few large ones it goes through them in many steps
+// (2048 tokens in blocks of 128 20.7 us, of 256 35, of 1024 125).
 #include <algorithm>
 
 #include "iq_extend_plan.h"
