@@ -461,7 +461,9 @@ void launch_attn(const AttnArgs& a, AttnMode mode, unsigned grid, hipStream_t s)
 //        128      1 x 8 9.5, 8.4   1 x 12 9.6, 10.3    32 x 16 14.5, 13.5
 //                 64 x 16 21.1, 16.9   64 x 32 30.4, 26.1   256 x 32 107, 102
 //        256      1 x 4 10.4, 9.9  1 x 8 13.0, 14.3    32 x 16 24.9, 26.9   64 x 32 55.3, 53.3
-// (1 x 8 of 256 in 16 bits is the one size where the rule takes the slower side.)
+// Where the rule takes the slower side: whole, few pairs of 256 in 16 bits (1 x 8);
+// split, heads of 32 and 64 a few tiles past the bounds and many pairs just past 32
+// (bf16 of 64, 32 x 17 11.0, 10.1, 128 x 33 31.2, 26.8).
 // With more tiles a long sequence among short ones would be waited for (2048
 // tokens: 9.2 us split, 22.7 whole).  It goes by the table's width, the lengths
 // being on the device: in a wide table a short sequence is split and pays 2 us for
